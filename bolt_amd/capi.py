@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(HERE, "libbolt_gfx950.so")
 
 # DataType (common/uni/include/data_type.h:67-85)
 DT_U8, DT_I8, DT_U32, DT_I32, DT_F16, DT_F16_8Q, DT_F32, DT_BIN01, DT_BIN11, DT_F32_8Q, DT_U8_Q = range(11)
+DT_BF16 = 14
 # DataFormat (common/uni/include/tensor_desc.h:33-78)
 DF_NCHW, DF_NCHWC8, DF_NCHWN16C8 = 0, 2, 9
 DF_TRANSPOSE, DF_NORMAL, DF_NK, DF_NKN32K4, DF_NKNxKx, DF_NCHWC16, DF_NCHWC2NxC4 = 13, 14, 17, 21, 39, 41, 42
@@ -144,6 +145,23 @@ class BoltEncoderLayerInt8(C.Structure):
                                                      "ln1_beta", "ln2_gamma", "ln2_beta")])
 
 
+class BoltPagedKvCache(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("dt", "numPages", "pageSize", "kvHeads", "headDim")] +
+                [(n, C.c_void_p) for n in ("k", "v", "kScale", "vScale")])
+
+
+class BoltPagedBatch(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("batch", "maxPages", "numTokens")] +
+                [(n, C.c_void_p) for n in ("pageTable", "lengths", "offsets")])
+
+
+class BoltRotary(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("dim", "positions", "interleaved")] + [(n, C.c_void_p) for n in ("cosine", "sine")]
+
+
+_PAGED = [C.POINTER(BoltPagedKvCache), C.POINTER(BoltPagedBatch)]
+_PAGED_ATTENTION = (C.c_int, _PAGED + [C.c_int, _u32, _vp, _u32, _vp, _u32, C.c_float, _u32, _vp, C.c_size_t])
+
 SIGNATURES = {
     "bolt_gfx950_init": (C.c_int, []),
     "bolt_gfx950_get_counter": (C.c_int, [C.c_char_p, C.POINTER(C.c_ulonglong)]),
@@ -244,6 +262,11 @@ SIGNATURES = {
     "bolt_gfx950_attention_f32": (C.c_int, [_vp, _u32, _u32, _u32, _u32, _vp]),
     "bolt_gfx950_add_layernorm_f32": (C.c_int, [_vp, _vp, _vp, _vp, _u32, _u32, _vp]),
     "bolt_gfx950_gelu_f32": (C.c_int, [_vp, C.c_size_t]),
+    "bolt_gfx950_kv_cache_append": (C.c_int, _PAGED + [C.c_int, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _vp, _u32,
+                                                       C.POINTER(BoltRotary)]),
+    "bolt_gfx950_paged_attention_workspace_bytes": (C.c_int, _PAGED + [_u32, C.POINTER(C.c_size_t)]),
+    "bolt_gfx950_paged_attention_decode": _PAGED_ATTENTION,
+    "bolt_gfx950_paged_attention_prompt": _PAGED_ATTENTION,
     "bolt_gfx950_quantize_f32_async": (C.c_int, [_vp, _u32, C.c_int, _vp, _vp, C.c_int]),
     "bolt_gfx950_quantize_f32_noalloc": (C.c_int, [_vp, _u32, C.c_int, _vp, _vp, C.c_int]),
     "bolt_gfx950_mmm_int8_perchannel": (C.c_int, [_u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),

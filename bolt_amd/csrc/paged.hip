@@ -1,0 +1,325 @@
+// Paged key / value cache: storing the keys and values of new tokens (with the position rotation of keys and queries on
+// the way), and attention over what is stored.
+#include "paged.h"
+
+namespace bg {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float bf16_to_f32(uint32_t h)
+{
+    return __uint_as_float(h << 16);
+}
+
+// round to nearest even; NaN keeps its sign and becomes quiet
+__device__ __forceinline__ uint32_t f32_to_bf16(float f)
+{
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) {
+        return (u >> 16) | 0x40u;
+    }
+    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
+
+// eight consecutive elements (16-byte aligned) <-> fp32
+template <int T>
+__device__ __forceinline__ void load8(const void *p, size_t at, float *x)
+{
+    if (T == PT_F32) {
+        const v4f a = ((const v4f *)((const float *)p + at))[0], b = ((const v4f *)((const float *)p + at))[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+        }
+    } else if (T == PT_F16) {
+        const v8h a = *(const v8h *)((const uint16_t *)p + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = (float)a[i];
+        }
+    } else {
+        const v4u a = *(const v4u *)((const uint16_t *)p + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(a[i] << 16);
+            x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+        }
+    }
+}
+
+template <int T>
+__device__ __forceinline__ void store8(void *p, size_t at, const float *x)
+{
+    if (T == PT_F32) {
+        v4f a, b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] = x[i];
+            b[i] = x[4 + i];
+        }
+        ((v4f *)((float *)p + at))[0] = a;
+        ((v4f *)((float *)p + at))[1] = b;
+    } else if (T == PT_F16) {
+        v8h a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            a[i] = (_Float16)x[i];
+        }
+        *(v8h *)((uint16_t *)p + at) = a;
+    } else {
+        v4u a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] = f32_to_bf16(x[2 * i]) | (f32_to_bf16(x[2 * i + 1]) << 16);
+        }
+        *(v4u *)((uint16_t *)p + at) = a;
+    }
+}
+
+__device__ __forceinline__ float load1(const void *p, size_t at, int type)
+{
+    if (type == PT_F32) {
+        return ((const float *)p)[at];
+    }
+    if (type == PT_F16) {
+        return (float)((const _Float16 *)p)[at];
+    }
+    if (type == PT_BF16) {
+        return bf16_to_f32(((const uint16_t *)p)[at]);
+    }
+    return (float)((const int8_t *)p)[at];
+}
+
+// ---- append -----------------------------------------------------------------------------------------
+// One workgroup per packed row; DIM / 16 lanes per head row, query heads first, then keys, then values. A lane owns two
+// runs of eight elements: the two halves of eight rotated pairs (pairs i, i + rot / 2), or 16 neighbours (pairs 2i, 2i + 1,
+// and the elements behind the rotated part). Every step is one fp32 operation in the order the plain formula has it:
+//   a' = a * cos - b * sin,  b' = b * cos + a * sin
+// rounded once to the stored type. An int8 slot gets s = (1 / max|x|) * 127 (1 for an all-zero row) and q = rne(x * s).
+template <int ACT, int CT, int DIM>
+__global__ void paged_append_kernel(PagedAppendArgs a)
+{
+    constexpr uint32_t kLanes = DIM / 16;
+    const uint32_t row = blockIdx.x;
+    const uint32_t b = paged_owner(a.batch, row);
+    const PagedSeq s = paged_seq(a.batch, b);
+    const int64_t i = (int64_t)row - s.first, pos = s.pos + i;
+    if (i < 0 || i >= s.count || pos < 0 || pos >= (int64_t)a.batch.max_pages << a.pool.shift ||
+        (a.rot && pos >= (int64_t)a.angles)) {
+        return;
+    }
+    const uint32_t kvh = a.pool.kv_heads, heads = a.heads + 2 * kvh;
+    for (uint32_t item = threadIdx.x; item < heads * kLanes; item += blockDim.x) {
+        const uint32_t head = item / kLanes, l = item % kLanes;
+        const bool is_q = head < a.heads, is_v = head >= a.heads + kvh;
+        const uint32_t h = is_q ? head : is_v ? head - a.heads - kvh : head - a.heads;
+        const bool turned = !is_v && 16 * l < a.rot;
+        const uint32_t e0 = turned && !a.interleaved ? 8 * l : 16 * l;
+        const uint32_t e1 = turned && !a.interleaved ? a.rot / 2 + 8 * l : 16 * l + 8;
+        const void *src = is_q ? a.q : is_v ? a.v : a.k;
+        const size_t base = (size_t)row * (is_q ? a.qstride : is_v ? a.vstride : a.kstride) + (size_t)h * DIM;
+        float x[16];
+        load8<ACT>(src, base + e0, x);
+        load8<ACT>(src, base + e1, x + 8);
+        if (turned) {
+            const size_t at = (size_t)pos * (a.rot / 2) + 8 * l;
+            float c[8], sn[8];
+            load8<PT_F32>(a.cos, at, c);
+            load8<PT_F32>(a.sin, at, sn);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float u = a.interleaved ? x[2 * j] : x[j], w = a.interleaved ? x[2 * j + 1] : x[8 + j];
+                const float ra = u * c[j] - w * sn[j], rb = w * c[j] + u * sn[j];
+                if (a.interleaved) {
+                    x[2 * j] = ra;
+                    x[2 * j + 1] = rb;
+                } else {
+                    x[j] = ra;
+                    x[8 + j] = rb;
+                }
+            }
+        }
+        if (is_q) {
+            const size_t to = (size_t)row * a.qostride + (size_t)h * DIM;
+            store8<ACT>(a.qout, to + e0, x);
+            store8<ACT>(a.qout, to + e1, x + 8);
+            continue;
+        }
+        const int64_t slot = paged_slot(a.batch.table + (size_t)b * a.batch.max_pages, (uint32_t)pos, a.pool.shift, a.pool.pages, kvh, h);
+        void *dst = is_v ? a.pool.v : a.pool.k;
+        if (CT == PT_I8) {
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float v = fabsf(x[j]);
+                top = v > top || v != v ? v : top;  // a NaN makes the slot's scale NaN, so that what reads it shows it
+            }
+#pragma unroll
+            for (uint32_t off = 1; off < kLanes; off <<= 1) {
+                const float v = __shfl_xor(top, off, kLanes);
+                top = v > top || v != v ? v : top;
+            }
+            // (the reciprocal of a subnormal maximum is infinite: the largest number stands in for it)
+            float scale = 1.0f / top * 127.0f;
+            scale = top == 0.0f ? 1.0f : scale > 3.40282347e38f ? 3.40282347e38f : scale;
+            if (slot >= 0) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = 0;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        int v = rne_i32(x[4 * j + t] * scale);
+                        v = v < -127 ? -127 : (v > 127 ? 127 : v);
+                        w[j] |= ((uint32_t)v & 0xffu) << (8 * t);
+                    }
+                }
+                int8_t *o = (int8_t *)dst + (size_t)slot * DIM;
+                *(v2u *)(o + e0) = (v2u){w[0], w[1]};
+                *(v2u *)(o + e1) = (v2u){w[2], w[3]};
+                if (l == 0) {
+                    (is_v ? a.pool.vs : a.pool.ks)[slot] = scale;
+                }
+            }
+        } else if (slot >= 0) {
+            store8<CT>(dst, (size_t)slot * DIM + e0, x);
+            store8<CT>(dst, (size_t)slot * DIM + e1, x + 8);
+        }
+    }
+}
+
+// ---- attention, one row of one head per wave -------------------------------------------------------
+// The streaming softmax: lanes hold the scores of 64 keys, then the output's DIM values.
+template <int ACT, int CT, int DIM>
+__global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttentionArgs a)
+{
+    __shared__ float sp[64];
+    __shared__ int64_t ss[64];
+    __shared__ float sq[DIM];
+    const uint32_t row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+    const uint32_t b = paged_owner(a.batch, row);
+    const PagedSeq s = paged_seq(a.batch, b);
+    const int64_t i = (int64_t)row - s.first;
+    if (i < 0 || i >= s.count) {
+        return;
+    }
+    const uint32_t kvh = h / (a.heads / a.pool.kv_heads);
+    const PagedSpan span = paged_span(s.pos + i, a.window, a.batch.max_pages << a.pool.shift);
+    const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
+    for (uint32_t d = lane; d < DIM; d += 64) {
+        sq[d] = load1(a.q, (size_t)row * a.qstride + (size_t)h * DIM + d, ACT);
+    }
+    float m = -INFINITY, l = 0.0f, o[DIM / 64];
+    for (int t = 0; t < DIM / 64; ++t) {
+        o[t] = 0.0f;
+    }
+    for (uint32_t k0 = span.lo; k0 < span.hi; k0 += 64) {
+        __syncthreads();
+        const uint32_t key = k0 + lane;
+        const int64_t slot = key < span.hi ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
+        float dot = 0.0f, x = -INFINITY;
+        if (slot >= 0) {
+            for (int d = 0; d < DIM; ++d) {
+                dot = __builtin_fmaf(sq[d], load1(a.pool.k, (size_t)slot * DIM + d, CT), dot);
+            }
+            if (CT == PT_I8) {
+                dot *= 1.0f / a.pool.ks[slot];
+            }
+            x = dot * a.scale2;
+        }
+        float top = x;
+        for (int off = 32; off; off >>= 1) {
+            top = fmaxf(top, __shfl_xor(top, off, 64));
+        }
+        top = fmaxf(top, m);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        const float p = slot >= 0 ? exp2f(x - ref) : 0.0f, corr = exp2f(m - ref);
+        float sum = p;
+        for (int off = 32; off; off >>= 1) {
+            sum += __shfl_xor(sum, off, 64);
+        }
+        l = l * corr + sum;
+        m = top;
+        sp[lane] = CT == PT_I8 && slot >= 0 ? p * (1.0f / a.pool.vs[slot]) : p;
+        ss[lane] = slot;
+        __syncthreads();
+        for (int t = 0; t < DIM / 64; ++t) {
+            o[t] *= corr;
+        }
+        for (uint32_t j = 0; j < 64; ++j) {
+            if (ss[j] >= 0) {
+                for (int t = 0; t < DIM / 64; ++t) {
+                    o[t] = __builtin_fmaf(sp[j], load1(a.pool.v, (size_t)ss[j] * DIM + 64 * t + lane, CT), o[t]);
+                }
+            }
+        }
+    }
+    for (int t = 0; t < DIM / 64; ++t) {
+        const size_t at = (size_t)row * a.ostride + (size_t)h * DIM + 64 * t + lane;
+        const float v = l == 0.0f ? 0.0f : o[t] / l;
+        if (ACT == PT_F32) {
+            ((float *)a.out)[at] = v;
+        } else if (ACT == PT_F16) {
+            ((_Float16 *)a.out)[at] = (_Float16)v;
+        } else {
+            ((uint16_t *)a.out)[at] = (uint16_t)f32_to_bf16(v);
+        }
+    }
+}
+
+namespace {
+
+// (activation type, cache type, head size) -> instantiation; the C-ABI layer refuses every other combination
+template <template <int, int, int> class F, typename A>
+hipError_t dispatch(int act, int ct, uint32_t dim, const A &a, hipStream_t st)
+{
+#define BG_PAGED(X, C)                                  \
+    if (act == X && ct == C) {                          \
+        return dim == 64 ? F<X, C, 64>::run(a, st) : F<X, C, 128>::run(a, st); \
+    }
+    BG_PAGED(PT_F32, PT_F16)
+    BG_PAGED(PT_F32, PT_I8)
+    BG_PAGED(PT_F16, PT_F16)
+    BG_PAGED(PT_F16, PT_I8)
+    BG_PAGED(PT_BF16, PT_BF16)
+    BG_PAGED(PT_BF16, PT_I8)
+#undef BG_PAGED
+    return hipErrorInvalidValue;
+}
+
+template <int ACT, int CT, int DIM>
+struct Append {
+    static hipError_t run(const PagedAppendArgs &a, hipStream_t st)
+    {
+        const uint32_t items = (a.heads + 2 * a.pool.kv_heads) * (DIM / 16);
+        const uint32_t threads = items >= 512 ? 512 : (items + 63) / 64 * 64;
+        hipLaunchKernelGGL((paged_append_kernel<ACT, CT, DIM>), dim3(a.batch.rows), dim3(threads), 0, st, a);
+        return hipGetLastError();
+    }
+};
+
+template <int ACT, int CT, int DIM>
+struct Rows {
+    static hipError_t run(const PagedAttentionArgs &a, hipStream_t st)
+    {
+        hipLaunchKernelGGL((paged_rows_kernel<ACT, CT, DIM>), dim3(a.batch.rows, a.heads), dim3(64), 0, st, a);
+        return hipGetLastError();
+    }
+};
+
+}  // namespace
+
+hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t st)
+{
+    return a.batch.rows && a.batch.batch ? dispatch<Append>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
+}
+
+hipError_t launch_paged_rows(const PagedAttentionArgs &a, hipStream_t st)
+{
+    return a.batch.rows && a.batch.batch ? dispatch<Rows>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
+}
+
+}  // namespace bg

@@ -1,0 +1,154 @@
+"""Host-side mirrors of the paged key / value cache entry points on torch CUDA tensors: append with position rotation,
+attention of one new token per sequence, attention of prompts. All arithmetic is in libbolt_gfx950.so; the calls enqueue
+on the library's stream (bolt_gfx950_set_stream) and return.
+
+    cache = PagedKvCache(k, v)                                   # [pages, kv_heads, page_size, head_dim]
+    batch = PagedBatch(page_table, lengths)                      # lengths include the new tokens
+    q = kv_cache_append(cache, batch, k_new, v_new, q_new, Rotary(cos, sin))
+    out = paged_attention_decode(cache, batch, q, workspace=paged_attention_workspace(cache, batch, heads))
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import capi
+from .capi import BoltError, BoltPagedBatch, BoltPagedKvCache, BoltRotary, check, lib
+
+DT_OF = {torch.float32: capi.DT_F32, torch.float16: capi.DT_F16, torch.bfloat16: capi.DT_BF16, torch.int8: capi.DT_I8}
+
+
+def _want(ok, why):
+    if not ok:
+        raise BoltError(why)
+
+
+def _list32(t, name, shape):
+    _want(t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape, "%s: contiguous int32 %s" % (name, list(shape)))
+
+
+class PagedKvCache:
+    """k, v: contiguous [pages, kv_heads, page_size, head_dim] of float16, bfloat16 or int8; int8 with fp32 scales
+    [pages, kv_heads, page_size] (stored = real * scale). The tensors are updated in place."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        _want(k.dtype in DT_OF and k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
+              "k and v: contiguous [pages, kv_heads, page_size, head_dim] of one type")
+        for s in (k_scale, v_scale):
+            _want((s is None) == (k.dtype != torch.int8), "an int8 cache has scales, another has none")
+            _want(s is None or (s.dtype == torch.float32 and s.is_contiguous() and s.shape == k.shape[:3]),
+                  "scales: contiguous float32 [pages, kv_heads, page_size]")
+        self.keep = (k, v, k_scale, v_scale)
+        self.device = _one_device(*self.keep)
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.struct = BoltPagedKvCache(DT_OF[k.dtype], self.pages, self.page_size, self.kv_heads, self.head_dim, k.data_ptr(), v.data_ptr(),
+                                       None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr())
+        self.ref = C.byref(self.struct)
+
+
+class PagedBatch:
+    """page_table: int32 [batch, max_pages]; lengths: int32 [batch], the new tokens included; offsets: int32 [batch + 1], the
+    first packed row of every sequence's new tokens, with `rows` rows in all (at least offsets[batch]); None: one new token
+    per sequence. The contents may change between calls and between replays of a captured graph."""
+
+    def __init__(self, page_table, lengths, offsets=None, rows=None):
+        batch = lengths.shape[0]
+        _want(page_table.dim() == 2, "page_table: [batch, max_pages]")
+        _list32(page_table, "page_table", (batch, page_table.shape[1]))
+        _list32(lengths, "lengths", (batch,))
+        if offsets is not None:
+            _list32(offsets, "offsets", (batch + 1,))
+            _want(rows is not None, "rows: how many packed rows the buffers have")
+        self.keep = (page_table, lengths, offsets)
+        self.device = _one_device(*self.keep)
+        self.rows = batch if rows is None else int(rows)
+        self.struct = BoltPagedBatch(batch, page_table.shape[1], self.rows, page_table.data_ptr(), lengths.data_ptr(),
+                                     None if offsets is None else offsets.data_ptr())
+        self.ref = C.byref(self.struct)
+
+
+class Rotary:
+    """cos, sin: contiguous float32 [positions, dim / 2]."""
+
+    def __init__(self, cos, sin, interleaved=False):
+        _want(cos.dim() == 2 and cos.shape == sin.shape and all(t.dtype == torch.float32 and t.is_contiguous() for t in (cos, sin)),
+              "cos and sin: contiguous float32 [positions, dim / 2]")
+        self.keep = (cos, sin)
+        self.device = _one_device(cos, sin)
+        self.struct = BoltRotary(2 * cos.shape[1], cos.shape[0], int(bool(interleaved)), cos.data_ptr(), sin.data_ptr())
+        self.ref = C.byref(self.struct)
+
+
+def _one_device(*tensors):
+    found = {t.device for t in tensors if t is not None}
+    _want(len(found) == 1 and next(iter(found)).type == "cuda", "tensors of one GPU")
+    return next(iter(found))
+
+
+def _rows(t, name, batch, heads, dim, dtype, device):
+    """Checks rows of heads, [rows, heads, dim] with dense heads; returns the elements between rows."""
+    _want(t.shape == (batch.rows, heads, dim), "%s: [%d, %d, %d]" % (name, batch.rows, heads, dim))
+    _want(t.dtype == dtype and t.device == device, "%s: %s on %s" % (name, dtype, device))
+    s = t.stride()
+    _want(s[2] == 1 and (s[1] == dim or heads == 1), "%s: the heads of a row are dense" % name)
+    return s[0] if batch.rows > 1 else max(s[0], heads * dim)
+
+
+def _here(cache, batch):
+    _want(cache.device == batch.device and cache.device.index == torch.cuda.current_device(),
+          "cache and batch belong to the current GPU")
+
+
+def kv_cache_append(cache, batch, k, v, q=None, rotary=None, q_out=None):
+    """k, v: [rows, kv_heads, head_dim], q: [rows, heads, head_dim], rows any number of elements apart. Returns q_out, the
+    rotated queries (None without q). Rows that belong to no sequence are left as they are in q_out."""
+    _here(cache, batch)
+    _want(rotary is None or rotary.device == cache.device, "the angles are on the cache's GPU")
+    ks = _rows(k, "k", batch, cache.kv_heads, cache.head_dim, k.dtype, cache.device)
+    vs = _rows(v, "v", batch, cache.kv_heads, cache.head_dim, k.dtype, cache.device)
+    heads, qs, qo, qp, qop = 0, 0, 0, None, None
+    if q is not None:
+        heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((batch.rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
+        qs = _rows(q, "q", batch, heads, cache.head_dim, k.dtype, cache.device)
+        qo = _rows(q_out, "q_out", batch, heads, cache.head_dim, k.dtype, cache.device)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
+    _want(k.dtype in DT_OF, "float32, float16 or bfloat16 rows")
+    check(lib().bolt_gfx950_kv_cache_append(cache.ref, batch.ref, DT_OF[k.dtype], k.data_ptr(), ks, v.data_ptr(), vs, heads, qp, qs, qop, qo,
+                                            None if rotary is None else rotary.ref), "kv_cache_append")
+    return q_out
+
+
+def paged_attention_workspace(cache, batch, heads):
+    """Device memory for the attention calls of this cache and batch shape; calls that may overlap need one each."""
+    n = C.c_size_t(0)
+    check(lib().bolt_gfx950_paged_attention_workspace_bytes(cache.ref, batch.ref, heads, C.byref(n)), "paged_attention_workspace_bytes")
+    return torch.empty(n.value, dtype=torch.uint8, device=cache.device)
+
+
+def _attention(fn, what, cache, batch, q, out, scale, window, workspace):
+    _here(cache, batch)
+    _want(q.dim() == 3 and q.dtype in DT_OF, "q: [rows, heads, head_dim] of float32, float16 or bfloat16")
+    heads = q.shape[1]
+    if workspace is None:
+        workspace = paged_attention_workspace(cache, batch, heads)
+    if out is None:
+        out = torch.empty((batch.rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
+    qs = _rows(q, "q", batch, heads, cache.head_dim, q.dtype, cache.device)
+    os = _rows(out, "out", batch, heads, cache.head_dim, q.dtype, cache.device)
+    _want(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == cache.device, "workspace: contiguous uint8 on the cache's GPU")
+    check(fn(cache.ref, batch.ref, DT_OF[q.dtype], heads, q.data_ptr(), qs, out.data_ptr(), os,
+             1.0 / math.sqrt(cache.head_dim) if scale is None else scale, window, workspace.data_ptr(), workspace.numel()), what)
+    return out
+
+
+def paged_attention_decode(cache, batch, q, out=None, scale=None, window=0, workspace=None):
+    """One new token per sequence (batch without offsets): q and out [batch, heads, head_dim]. scale: 1 / sqrt(head_dim)."""
+    return _attention(lib().bolt_gfx950_paged_attention_decode, "paged_attention_decode", cache, batch, q, out, scale, window, workspace)
+
+
+def paged_attention_prompt(cache, batch, q, out=None, scale=None, window=0, workspace=None):
+    """Any number of new tokens per sequence (batch with offsets): q and out [rows, heads, head_dim]. Rows that belong to no
+    sequence are left as they are."""
+    return _attention(lib().bolt_gfx950_paged_attention_prompt, "paged_attention_prompt", cache, batch, q, out, scale, window, workspace)

@@ -501,6 +501,72 @@ EE bolt_gfx950_add_layernorm_f32(const float *a, const float *b, const float *ga
     U32 hidden, float *out);
 EE bolt_gfx950_gelu_f32(float *x, size_t n);
 
+/* ---- attention over a paged key / value cache (device pointers only, asynchronous) ---- */
+/* What a decoder that generates text needs beside the int8 projections above: storing the keys and values of new tokens,
+ * and attention of new tokens over everything stored. No counterpart in the reference, whose attention runs over dense
+ * tensors that are built anew for every call.
+ *
+ * The cache is a pool of pages; a sequence owns pages in any order, listed in its row of the page table.
+ *   dt            DT_F16, DT_BF16 or DT_I8 (one fp32 scale per slot and head, Bolt convention: stored = real * scale)
+ *   k, v          [numPages][kvHeads][pageSize][headDim];  kScale, vScale  DT_I8: [numPages][kvHeads][pageSize], else NULL
+ *   headDim       64 or 128;  pageSize  a power of two up to 4096
+ * A batch says where the new tokens of `batch` sequences are: they are packed rows, sequence b owning rows offsets[b] up to
+ * offsets[b + 1] (ascending), and they are the LAST ones of the sequence's lengths[b] keys. offsets == NULL: one new token
+ * per sequence, row b (numTokens == batch). numTokens is the number of rows the buffers have: rows behind
+ * offsets[batch] belong to nobody and are neither read nor written. lengths, offsets and pageTable are read by the
+ * kernels, so that a captured graph can be replayed with other values; nothing in them is trusted: a page number
+ * outside the pool, a position in front of the sequence or behind the page table (maxPages pages) is a key that is not
+ * stored and not seen, never an address. lengths[b] == 0: a place of a padded batch that nobody uses.
+ * Activations (q, k, v, out; `dt` of the calls) are DT_F32 or DT_F16 over a DT_F16 or DT_I8 cache, DT_BF16 over a DT_BF16
+ * or DT_I8 cache. Strides count elements between rows, so that q, k and v can be parts of the rows of one merged
+ * projection; inside a row the heads are dense. Base pointers and strides are multiples of 16 bytes.
+ * Errors: NULL_POINTER; NOT_MATCH for sizes that contradict each other (heads no multiple of kvHeads, a stride shorter
+ * than a row, a workspace too small); NOT_SUPPORTED for the rest, with the reason in bolt_gfx950_last_error(). */
+typedef struct {
+    DataType dt;
+    U32 numPages, pageSize, kvHeads, headDim;
+    void *k, *v;
+    F32 *kScale, *vScale;
+} BoltPagedKvCache;
+typedef struct {
+    U32 batch, maxPages, numTokens;
+    const I32 *pageTable; /* [batch][maxPages] */
+    const I32 *lengths;   /* [batch] */
+    const I32 *offsets;   /* [batch + 1] or NULL */
+} BoltPagedBatch;
+/* Tables of cosines and sines, fp32 [positions][dim / 2]: pair j of a head at position p is turned by the angle (p, j). The
+ * pairs are elements (j, j + dim / 2), or (2j, 2j + 1) when interleaved; elements from dim on stay as they are. dim is a
+ * multiple of 16 up to headDim. The tables are the caller's, so any base, scaling or extension of the angles is. */
+typedef struct {
+    U32 dim, positions, interleaved;
+    const F32 *cosine, *sine;
+} BoltRotary;
+/* Stores k and v, rows of kvHeads heads, at their positions; keys are rotated on the way (rotary == NULL: not). With heads
+ * > 0 the queries are rotated too, from q to qOut (which may be q itself). Every step is one fp32 operation,
+ * a' = a cos - b sin, b' = b cos + a sin, rounded once to the stored type; an int8 slot gets
+ * s = (1 / max|x|) * 127 (the reciprocal first; 1 for a row of zeros) and rne(x * s). A token whose position lies behind the
+ * tables of angles is left out like one without a page. Slots must be distinct: two sequences that append to a shared
+ * page race. */
+EE bolt_gfx950_kv_cache_append(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataType dt, const void *k,
+    U32 kStride, const void *v, U32 vStride, U32 heads, const void *q, U32 qStride, void *qOut, U32 qOutStride,
+    const BoltRotary *rotary);
+/* out = softmax(scale * q K^T) V per head, head h reading the keys of head h / (heads / kvHeads). A token at position p sees
+ * the keys 0 .. p of its sequence, with window > 0 the last `window` of them; a row that sees no key becomes zeros. What the
+ * cache holds elsewhere has no influence, infinities and NaN included. Scores, the softmax and its sums are fp32; with
+ * fp32 activations every product is accurate to fp32 too. The result does not depend on what else is in the batch run
+ * beyond fp32 rounding of how the keys are split; the same call gives the same bytes.
+ *   decode  one new token per sequence (offsets == NULL): the keys are split over the machine and the parts joined
+ *   prompt  any number of new tokens per sequence (offsets != NULL), each seeing those before it; they must be stored
+ *           (bolt_gfx950_kv_cache_append) before the call
+ * out must not overlap q. workspace: 256-byte aligned device memory of the queried size, used until the call's work
+ * is done; calls that can overlap (two streams, two graphs replayed side by side) need one each. */
+EE bolt_gfx950_paged_attention_workspace_bytes(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, U32 heads,
+    size_t *bytes);
+EE bolt_gfx950_paged_attention_decode(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataType dt, U32 heads,
+    const void *q, U32 qStride, void *out, U32 outStride, F32 scale, U32 window, void *workspace, size_t workspaceBytes);
+EE bolt_gfx950_paged_attention_prompt(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataType dt, U32 heads,
+    const void *q, U32 qStride, void *out, U32 outStride, F32 scale, U32 window, void *workspace, size_t workspaceBytes);
+
 /* ---- asynchronous forms with device-resident scales (AMD_GFX950_DEVICE only) -------- */
 /* No counterpart in the reference: Bolt keeps a tensor's scale in host memory
  * (common/memory/include/tensor.hpp:83-96). These keep it on the GPU so that

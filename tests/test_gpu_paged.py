@@ -1,0 +1,476 @@
+"""Paged key / value cache on the GPU against tests/checkers_paged.py: append bit for bit, attention within the bound that
+its roundings give (derived there)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+import torch  # noqa: E402
+
+from bolt_amd import capi, host_paged as hp  # noqa: E402
+from checkers_paged import COMBOS, TYPES, Case, assert_attention, quantised, rotated  # noqa: E402
+
+
+@pytest.fixture(scope="module", autouse=True)
+def ready():
+    assert torch.cuda.is_available()
+    capi.check(capi.lib().bolt_gfx950_init(), "init")
+
+
+def sync():
+    capi.check(capi.lib().bolt_gfx950_synchronize(), "sync")
+    torch.cuda.synchronize()
+
+
+def bits(t):
+    t = t.cpu().contiguous()
+    return t.view({4: torch.int32, 2: torch.int16, 1: torch.int8}[t.element_size()])
+
+
+def angles(positions, rot, seed=0, interleaved=False):
+    g = torch.Generator().manual_seed(seed)
+    a = torch.rand(positions, rot // 2, generator=g, dtype=torch.float64) * 6.3
+    return a.cos().float(), a.sin().float()
+
+
+def attend(case, prompt, **kw):
+    cache, batch, q = case.gpu(offsets=prompt)
+    out = torch.full_like(q, 77.0)
+    fn = hp.paged_attention_prompt if prompt else hp.paged_attention_decode
+    fn(cache, batch, q, out=out, window=case.window, **kw)
+    sync()
+    return out
+
+
+# ---- append -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("act,cache", COMBOS)
+@pytest.mark.parametrize("dim,page,rot,interleaved,new,past", [
+    (64, 16, 64, False, (5, 0, 17, 1), (0, 9, 30, 15)),
+    (128, 8, 128, True, (1, 33), (7, 0)),
+    (128, 64, 32, False, (70,), (60,)),
+    (64, 1, 16, True, (3, 2), (0, 5)),
+    (128, 4096, 0, False, (2, 9), (4094, 0)),
+])
+def test_append(act, cache, dim, page, rot, interleaved, new, past):
+    print("append", act, cache, dim, page, rot, interleaved, new, past, flush=True)
+    heads, kv = 6, 3
+    total = [p + n for p, n in zip(past, new)]
+    c = Case(act, cache, heads, kv, dim, page, total, new, seed=dim + page + rot, rows=sum(new) + 3)
+    pc, pb, _ = c.gpu()
+    g = torch.Generator().manual_seed(9)
+    qkv = (torch.randn(c.rows, (heads + 2 * kv) * dim, generator=g) * 3).to(TYPES[act])
+    qkv[0, heads * dim:heads * dim + dim] = 0                                  # a key row of zeros
+    if act != "f16":
+        qkv[0, heads * dim + dim:heads * dim + 2 * dim] = 1e-39                # one of subnormal numbers
+    q, k, v = qkv.view(c.rows, heads + 2 * kv, dim).split((heads, kv, kv), 1)
+    cos, sin = angles(max(total), max(rot, 16))
+    rotary = hp.Rotary(cos.cuda(), sin.cuda(), interleaved) if rot else None
+    dq, dk, dv = qkv.cuda().view(c.rows, heads + 2 * kv, dim).split((heads, kv, kv), 1)
+    q_out = torch.full((c.rows, heads, dim), 55.0, dtype=TYPES[act], device="cuda")
+    hp.kv_cache_append(pc, pb, dk, dv, dq, rotary, q_out)
+    sync()
+    mine = int(c.offsets[-1])
+    seq = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new))
+    pos = torch.tensor([t - n + i for t, n in zip(total, new) for i in range(n)])
+    turn = (lambda x: rotated(x, cos[pos], sin[pos], interleaved)) if rot else (lambda x: x)
+    assert torch.equal(bits(q_out[:mine]), bits(turn(q[:mine].float()).to(TYPES[act]))) and (q_out[mine:] == 55).all()
+    at, slot = c.table[seq, pos // page].long(), pos % page
+    for x, was, scale, now, now_scale in ((turn(k[:mine].float()), c.k, c.ks, pc.keep[0], pc.keep[2]), (v[:mine].float(), c.v, c.vs, pc.keep[1], pc.keep[3])):
+        want, want_scale = was.clone(), None if scale is None else scale.clone()
+        if cache == "i8":
+            want[at, :, slot], want_scale[at, :, slot] = quantised(x)
+            assert torch.equal(bits(now_scale), bits(want_scale))
+        else:
+            want[at, :, slot] = x.to(TYPES[cache])
+        assert torch.equal(bits(now), bits(want))                              # every other slot as it was
+
+
+def test_append_without_queries_in_place_and_one_row_each():
+    c = Case("f32", "f16", 4, 2, 64, 16, (5, 0, 33), (1, 1, 1), seed=3)
+    pc, pb, _ = c.gpu(offsets=False)
+    cos, sin = angles(64, 64)
+    r = hp.Rotary(cos.cuda(), sin.cuda())
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(3, h, 64, generator=g) for h in (4, 2, 2))
+    dq = q.cuda()
+    assert hp.kv_cache_append(pc, pb, k.cuda(), v.cuda(), dq, r, dq) is dq
+    sync()
+    pos = torch.tensor([4, 0, 32])
+    want = rotated(q, cos[pos], sin[pos], False)
+    want[1] = q[1]                                                             # length 0: nobody's row
+    assert torch.equal(dq.cpu(), want)
+    first = pc.keep[0].clone()
+    assert hp.kv_cache_append(pc, pb, k.cuda(), v.cuda(), None, r) is None
+    sync()
+    assert torch.equal(bits(pc.keep[0]), bits(first))
+
+
+@pytest.mark.parametrize("cache", ["f16", "i8"])
+def test_append_leaves_out_what_has_no_place(cache):
+    """page numbers outside the pool, positions behind the page table, in front of the sequence and behind the angles"""
+    c = Case("f32", cache, 2, 1, 64, 8, (20, 30, 3, 16), (20, 6, 5, 2), seed=5, max_pages=3)
+    c.table[0, 1], c.table[0, 2], c.table[3, 0] = -5, c.pages, 0x7fffffff
+    pc, pb, _ = c.gpu()
+    cos, sin = angles(14, 64)                                                  # sequence 3: position 14, 15 not covered
+    g = torch.Generator().manual_seed(6)
+    q, k, v = (torch.randn(c.rows, h, 64, generator=g) for h in (2, 1, 1))
+    q_out = torch.full_like(q, 9.0).cuda()
+    hp.kv_cache_append(pc, pb, k.cuda(), v.cuda(), q.cuda(), hp.Rotary(cos.cuda(), sin.cuda()), q_out)
+    sync()
+    want_k, want_v, want_q = c.k.clone(), c.v.clone(), torch.full_like(q, 9.0)
+    ks, vs = (None, None) if c.ks is None else (c.ks.clone(), c.vs.clone())
+    for b in range(4):
+        for i in range(c.new[b]):
+            p, row = c.lengths[b] - c.new[b] + i, int(c.offsets[b]) + i
+            if p < 0 or p >= 14:
+                continue
+            want_q[row] = rotated(q[row:row + 1], cos[p:p + 1], sin[p:p + 1], False)[0]
+            page = int(c.table[b, p // 8])
+            if 0 <= page < c.pages:
+                kk = rotated(k[row:row + 1], cos[p:p + 1], sin[p:p + 1], False)[0, 0]
+                if cache == "i8":
+                    want_k[page, 0, p % 8], ks[page, 0, p % 8] = quantised(kk)
+                    want_v[page, 0, p % 8], vs[page, 0, p % 8] = quantised(v[row, 0])
+                else:
+                    want_k[page, 0, p % 8], want_v[page, 0, p % 8] = kk.half(), v[row, 0].half()
+    assert torch.equal(q_out.cpu(), want_q)
+    for now, want in zip(pc.keep, (want_k, want_v, ks, vs)):
+        assert want is None or torch.equal(bits(now), bits(want))
+
+
+def test_append_of_infinities_and_nan_shows_them():
+    c = Case("f32", "i8", 1, 1, 64, 8, (3,), (3,), seed=5)
+    pc, pb, _ = c.gpu()
+    k = torch.ones(3, 1, 64)
+    k[0, 0, 5], k[1, 0, 9] = float("nan"), float("-inf")
+    hp.kv_cache_append(pc, pb, k.cuda(), k.cuda())
+    sync()
+    scale = pc.keep[2].cpu()[c.table[0, 0].long(), 0, :3]
+    assert torch.isnan(scale[0]) and scale[1] == 0 and scale[2] == 127
+
+
+# ---- attention --------------------------------------------------------------------------------------
+DECODE = [
+    # heads, kv_heads, dim, page, lengths, window
+    (12, 12, 64, 16, (1, 2, 0, 16, 17, 130), 0),
+    (8, 1, 128, 8, (1, 63, 64, 65, 300), 0),
+    (28, 4, 128, 32, (257, 31, 1000), 0),
+    (6, 2, 64, 1, (45, 7), 0),
+    (40, 2, 128, 128, (700, 129), 100),
+    (3, 3, 64, 4096, (1, 4097, 515), 33),
+    (16, 8, 128, 64, (2500, 1, 0, 640), 1),
+]
+
+
+@pytest.mark.parametrize("act,cache", COMBOS)
+@pytest.mark.parametrize("shape", DECODE, ids=str)
+def test_decode(act, cache, shape):
+    heads, kv, dim, page, lengths, window = shape
+    print("decode", act, cache, shape, flush=True)
+    c = Case(act, cache, heads, kv, dim, page, lengths, [1] * len(lengths), seed=heads + sum(lengths), window=window)
+    out = attend(c, False)
+    assert assert_attention(out, c).all()
+    for b, n in enumerate(lengths):
+        assert n or not out[b].any()                                           # no keys: zeros
+
+
+PROMPT = [
+    # heads, kv_heads, dim, page, past, new, window, rows behind the last sequence
+    (12, 12, 64, 16, (0, 0, 0), (1, 2, 37), 0, 0),
+    (4, 1, 128, 8, (0, 5, 64), (70, 1, 33), 0, 5),
+    (14, 2, 128, 32, (31, 0, 100), (1, 0, 130), 0, 1),
+    (6, 2, 64, 1, (3,), (29,), 0, 0),
+    (8, 2, 128, 128, (300, 0), (65, 129), 40, 2),
+    (3, 3, 64, 4096, (4090, 0), (9, 64), 0, 0),
+    (10, 2, 64, 64, (0, 17), (200, 3), 1, 0),
+]
+
+
+@pytest.mark.parametrize("act,cache", COMBOS)
+@pytest.mark.parametrize("shape", PROMPT, ids=str)
+def test_prompt(act, cache, shape):
+    heads, kv, dim, page, past, new, window, spare = shape
+    print("prompt", act, cache, shape, flush=True)
+    c = Case(act, cache, heads, kv, dim, page, [p + n for p, n in zip(past, new)], new, seed=heads + sum(new), window=window, rows=sum(new) + spare)
+    out = attend(c, True)
+    mine = assert_attention(out, c)
+    assert mine.sum() == sum(new) and (out[torch.from_numpy(~mine).cuda()] == 77).all()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("act,cache", [("f32", "f16"), ("bf16", "bf16"), ("f16", "i8")])
+def test_attention_with_lists_that_point_outside(prompt, act, cache):
+    """Page numbers outside the pool are keys that nobody sees; lengths behind the page table end with it; more new tokens than
+    the sequence is long: the first ones see nothing"""
+    new = (3, 2, 4, 1) if prompt else (1, 1, 1, 1)
+    c = Case(act, cache, 4, 2, 64, 8, (30, 21, 2, 8), new, seed=8, max_pages=3)
+    c.table[0, 1], c.table[1, 0], c.table[1, 1], c.table[1, 2], c.table[3, 0] = -1, c.pages, -(1 << 31), 0x7fffffff, 12345678
+    out = attend(c, prompt)
+    assert_attention(out, c)
+    assert not out[int(c.offsets[1])].any() and not out[int(c.offsets[3])].any()
+
+
+@pytest.mark.parametrize("act,cache", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "i8")])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_token_sees_nothing_of_later_ones(act, cache, bad):
+    """infinities and NaN in the key and the value of a later token, in the same tile: the rows before it are those of the clean
+    cache, the rows from it on show them; and behind a window they are gone again"""
+    new, spot = 90, 41
+    c = Case(act, cache, 4, 2, 64, 16, (new + 3,), (new,), seed=11)
+    clean = attend(c, True)
+    page, slot = int(c.table[0, (spot + 3) // 16]), (spot + 3) % 16
+    for which in ("k", "v"):
+        scales, store = (c.ks, c.ks) if which == "k" else (c.vs, c.vs)
+        target = store if cache == "i8" else (c.k if which == "k" else c.v)
+        keep = target.clone()
+        if cache == "i8":
+            target[page, :, slot] = bad
+        else:
+            target[page, :, slot, 7] = bad
+        out = attend(c, True)
+        assert torch.equal(bits(out[:spot]), bits(clean[:spot])), which
+        if not (cache == "i8" and np.isinf(bad)):                              # a scale of infinity stands for zeros
+            assert not torch.isfinite(out[spot:].float()).all(dim=-1).any() if which == "v" else True
+        c.window = 20
+        windowed = attend(c, True)
+        target.copy_(keep)
+        again = attend(c, True)
+        assert torch.equal(bits(windowed[:spot]), bits(again[:spot])) and torch.equal(bits(windowed[spot + 20:]), bits(again[spot + 20:])), which
+        c.window = 0
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("act,cache", COMBOS)
+def test_large_and_small_scores(prompt, act, cache):
+    """queries whose scores span hundreds: the softmax is nearly one key; and nearly equal ones; fp16's largest and smallest"""
+    for size in (60.0, 1e-4, 0.0):
+        c = Case(act, cache, 4, 2, 64, 16, (150, 40), (20, 1) if prompt else (1, 1), seed=12)
+        c.q = (c.q.float() * size).to(TYPES[act])
+        if cache != "i8":
+            c.k[c.k.isfinite()] *= 0.01 if size == 60.0 else 1.0
+        assert_attention(attend(c, prompt), c)
+
+
+def test_queries_beyond_the_range_of_fp16():
+    for size in (3e6, 1e-9, 3e30):
+        c = Case("f32", "f16", 4, 2, 64, 16, (70,), (9,), seed=13)
+        c.q = c.q * size
+        for prompt in (True, False):
+            c.new, c.offsets, c.rows = ([9], torch.tensor([0, 9], dtype=torch.int32), 9) if prompt else ([1], torch.tensor([0, 1], dtype=torch.int32), 1)
+            c.q = c.q[:c.rows]
+            assert_attention(attend(c, prompt, scale=0.125 / size), c, 0.125 / size)
+    c = Case("bf16", "i8", 4, 2, 64, 16, (70,), (9,), seed=13)
+    c.q = (c.q.float() * 1e30).bfloat16()
+    assert_attention(attend(c, True, scale=1e-31), c, 1e-31)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_strided_rows(prompt):
+    """q and out as parts of wider rows, around which nothing changes"""
+    c = Case("f16", "f16", 6, 2, 128, 16, (50, 33), (7, 3) if prompt else (1, 1), seed=14)
+    cache, batch, q = c.gpu(offsets=prompt)
+    wide_q = torch.full((c.rows, 10, 128), float("nan"), dtype=torch.float16, device="cuda")
+    wide_q[:, 2:8] = q
+    wide = torch.full((c.rows, 9, 128), 5.0, dtype=torch.float16, device="cuda")
+    fn = hp.paged_attention_prompt if prompt else hp.paged_attention_decode
+    fn(cache, batch, wide_q[:, 2:8], out=wide[:, 1:7])
+    sync()
+    assert_attention(wide[:, 1:7], c)
+    assert (wide[:, 0] == 5).all() and (wide[:, 7:] == 5).all()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_same_bytes_again_and_on_another_stream(prompt):
+    c = Case("f16", "f16", 16, 4, 128, 16, (3000, 700, 90), (40, 200, 90) if prompt else (1, 1, 1), seed=15)
+    first = attend(c, prompt)
+    cache, batch, q = c.gpu(offsets=prompt)
+    fn = hp.paged_attention_prompt if prompt else hp.paged_attention_decode
+    ws = hp.paged_attention_workspace(cache, batch, 16)
+    ws.fill_(255)                                                              # what a workspace holds before does not matter
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    capi.check(capi.lib().bolt_gfx950_set_stream(stream.cuda_stream), "set_stream")
+    try:
+        outs = [torch.empty_like(q) for _ in range(3)]
+        torch.cuda.synchronize()
+        for o in outs:
+            fn(cache, batch, q, out=o, workspace=ws)
+        sync()
+    finally:
+        capi.check(capi.lib().bolt_gfx950_set_stream(None), "set_stream")
+    mine = slice(0, int(c.offsets[-1]))
+    for o in outs:
+        assert torch.equal(bits(o[mine]), bits(first[mine]))
+
+
+@pytest.mark.parametrize("cache_type", ["f16", "i8"])
+def test_offsets_beyond_32_bits(cache_type):
+    """a pool of more than 2^32 elements, the sequence in its last pages"""
+    page, dim = 4096, 128
+    pages = (1 << 32) // (page * dim) + 5
+    dtype = TYPES[cache_type]
+    k, v = (torch.zeros(pages, 1, page, dim, dtype=dtype, device="cuda") for _ in range(2))
+    scales = [torch.ones(pages, 1, page, device="cuda") for _ in range(2)] if cache_type == "i8" else [None, None]
+    cache = hp.PagedKvCache(k, v, *scales)
+    c = Case("f16", cache_type, 4, 1, dim, page, (page + 77,), (page + 77,), seed=16, spare=0)
+    table = torch.tensor([[pages - 1, pages - 2]], dtype=torch.int32, device="cuda")
+    c.table = torch.tensor([[1, 0]], dtype=torch.int32)                        # the same two pages of a small pool
+    lengths = torch.tensor([page + 77], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(17)
+    kn, vn = (torch.randn(page + 77, 1, dim, generator=g, device="cuda", dtype=torch.float16) for _ in range(2))
+    hp.kv_cache_append(cache, hp.PagedBatch(table, lengths, torch.tensor([0, page + 77], dtype=torch.int32, device="cuda"), page + 77), kn, vn)
+    q = torch.randn(1, 4, dim, generator=g, device="cuda", dtype=torch.float16)
+    out = hp.paged_attention_decode(cache, hp.PagedBatch(table, lengths), q)
+    last = hp.paged_attention_prompt(cache, hp.PagedBatch(table, lengths, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 1), q)
+    sync()
+    c.k, c.v = k[-2:].cpu(), v[-2:].cpu()
+    if cache_type == "i8":
+        c.ks, c.vs = scales[0][-2:].cpu(), scales[1][-2:].cpu()
+    c.pages, c.new, c.offsets, c.rows, c.q = 2, [1], torch.tensor([0, 1], dtype=torch.int32), 1, q.cpu()
+    assert_attention(out, c)
+    assert_attention(last, c)
+    assert not k[:-2].any() and not v[:-2].any()
+
+
+def test_captured_step_replayed_with_other_lengths():
+    """append and attention of one step in a graph; lengths, pages and inputs change between the replays, and the library's
+    eager calls run in between; a second graph with a workspace of its own is replayed beside it"""
+    heads, kv, dim, page, batch = 8, 2, 64, 16, 5
+    g = torch.Generator(device="cuda").manual_seed(18)
+    pages = 60
+    cos, sin = angles(160, dim)
+    rotary = hp.Rotary(cos.cuda(), sin.cuda())
+
+    def fresh():
+        k, v = (torch.randn(pages, kv, page, dim, generator=g, device="cuda", dtype=torch.float16) for _ in range(2))
+        return hp.PagedKvCache(k, v)
+    lengths = torch.ones(batch, dtype=torch.int32, device="cuda")
+    table = torch.randperm(pages, generator=g, device="cuda")[:batch * 10].to(torch.int32).view(batch, 10).contiguous()
+    b = hp.PagedBatch(table, lengths)
+    qkv = torch.zeros(batch, heads + 2 * kv, dim, device="cuda")
+    q, k, v = qkv.split((heads, kv, kv), 1)
+
+    def step(cache, ws, q_out, out):
+        hp.kv_cache_append(cache, b, k, v, q, rotary, q_out)
+        hp.paged_attention_decode(cache, b, q_out, out=out, workspace=ws)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    capi.check(capi.lib().bolt_gfx950_set_stream(side.cuda_stream), "set_stream")
+    try:
+        sides = []
+        for _ in range(2):
+            cache = fresh()
+            ws = hp.paged_attention_workspace(cache, b, heads)
+            q_out, out = (torch.zeros(batch, heads, dim, device="cuda") for _ in range(2))
+            torch.cuda.synchronize()
+            step(cache, ws, q_out, out)                                        # nothing left to initialise inside the capture
+            sync()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                step(cache, ws, q_out, out)
+            sides.append((cache, ws, q_out, out, graph))
+        for n in (1, 0, 7, 150, 16, 33):
+            lengths.copy_(torch.tensor([n, max(n - 1, 0), (3 * n) % 160, 1, 0], dtype=torch.int32))
+            qkv.copy_(torch.randn(qkv.shape, generator=g, device="cuda"))
+            eager = []
+            for cache, _, q_out, _, _ in sides:                                # rows of empty places are nobody's: both start from the same
+                twin, q_twin, out = hp.PagedKvCache(cache.keep[0].clone(), cache.keep[1].clone()), q_out.clone(), torch.zeros(batch, heads, dim, device="cuda")
+                ws = hp.paged_attention_workspace(twin, b, heads)
+                torch.cuda.synchronize()
+                step(twin, ws, q_twin, out)
+                sync()
+                eager.append((twin, out))
+            for one in sides:
+                one[4].replay()
+            torch.cuda.synchronize()
+            for one, (twin, out) in zip(sides, eager):
+                assert torch.equal(bits(one[0].keep[0]), bits(twin.keep[0])) and torch.equal(bits(one[0].keep[1]), bits(twin.keep[1])), n
+                assert torch.equal(bits(one[3]), bits(out)), n
+    finally:
+        capi.check(capi.lib().bolt_gfx950_set_stream(None), "set_stream")
+
+
+@pytest.mark.parametrize("cache_type", ["f16", "i8"])
+def test_generation_over_an_int8_projection(cache_type):
+    """What the operators are for: hidden states go through the library's int8 QKV product, prompts are stored and attended, then
+    tokens one by one; every row is held against attention over the cache's own contents, in which a token that came in a
+    prompt and one that came alone are the same bytes"""
+    from bolt_amd import host
+    heads, kv, dim, page, hidden = 4, 2, 64, 16, 128
+    width = (heads + 2 * kv) * dim
+    rng = np.random.default_rng(19)
+    weight = torch.from_numpy(rng.integers(-127, 128, size=(width, hidden), dtype=np.int8)).cuda()
+    blob, bdesc, rhs = host.mmm_transform_rhs(weight, capi.DF_TRANSPOSE, hidden, width)
+    column = torch.full((width,), 200.0, device="cuda")
+    lengths, steps = [21, 1, 40], 5
+    most = max(lengths) + steps
+    x = torch.from_numpy(rng.standard_normal((3, most, hidden)).astype(np.float32)).cuda()
+    scale_in = torch.tensor([40.0], device="cuda")                             # static: the products of a row do not depend on its batch
+
+    def project(rows):
+        n = rows.shape[0]
+        u8 = (rows * 40.0 + 128.0).round().clamp(1, 255).to(torch.uint8)
+        out = torch.empty(n, width, device="cuda")
+        capi.check(capi.lib().bolt_gfx950_mmm_int8_perchannel(n, width, hidden, u8.data_ptr(), blob.data_ptr(), blob.data_ptr() + rhs,
+                                                             out.data_ptr(), scale_in.data_ptr(), column.data_ptr(), None), "project")
+        return out.view(n, heads + 2 * kv, dim).split((heads, kv, kv), 1)
+    held = -(-most // page)
+    dtype = TYPES[cache_type]
+
+    def pool():
+        k, v = (torch.zeros(3 * held, kv, page, dim, dtype=dtype, device="cuda") for _ in range(2))
+        s = [torch.ones(3 * held, kv, page, device="cuda") for _ in range(2)] if cache_type == "i8" else [None, None]
+        return hp.PagedKvCache(k, v, *s)
+    table = torch.randperm(3 * held, device="cuda").to(torch.int32).view(3, held).contiguous()
+    cos, sin = angles(most, dim)
+    rotary = hp.Rotary(cos.cuda(), sin.cuda())
+
+    def check(cache, batch_lengths, new, q, out):
+        c = Case("f32", cache_type, heads, kv, dim, page, batch_lengths, new, seed=1)
+        c.table, c.pages, c.max_pages = table.cpu(), 3 * held, held
+        c.k, c.v, c.ks, c.vs = (None if t is None else t.cpu() for t in cache.keep)
+        c.q = q.cpu()
+        assert assert_attention(out, c).all()
+
+    def prompt(cache, upto):
+        n = torch.tensor(upto, dtype=torch.int32, device="cuda")
+        offsets = torch.cat([n.new_zeros(1), n.cumsum(0, dtype=torch.int32)])
+        b = hp.PagedBatch(table, n, offsets, sum(upto))
+        q, k, v = project(torch.cat([x[i, :u] for i, u in enumerate(upto)]))
+        q = hp.kv_cache_append(cache, b, k, v, q, rotary)
+        out = hp.paged_attention_prompt(cache, b, q)
+        sync()
+        return q, out
+    cache = pool()
+    q, out = prompt(cache, lengths)
+    check(cache, lengths, lengths, q, out)
+    for step in range(steps):
+        now = [n + step + 1 for n in lengths]
+        b = hp.PagedBatch(table, torch.tensor(now, dtype=torch.int32, device="cuda"))
+        q, k, v = project(torch.stack([x[i, n - 1] for i, n in enumerate(now)]))
+        q = hp.kv_cache_append(cache, b, k, v, q, rotary)
+        out = hp.paged_attention_decode(cache, b, q)
+        sync()
+        check(cache, now, [1, 1, 1], q, out)
+    whole = pool()
+    prompt(whole, [n + steps for n in lengths])
+    for one, other in zip(cache.keep, whole.keep):
+        assert one is None or torch.equal(bits(one), bits(other))
+
+
+def test_host_mirror_refuses():
+    c = Case("f16", "f16", 4, 2, 64, 16, (9, 5), (1, 1), seed=1)
+    cache, batch, q = c.gpu(offsets=False)
+    ragged = c.gpu()[1]
+    k = torch.zeros(2, 2, 64, dtype=torch.float16, device="cuda")
+    for call in (lambda: hp.paged_attention_decode(cache, batch, q[:1]), lambda: hp.paged_attention_decode(cache, batch, q.float()[..., :32]),
+                 lambda: hp.paged_attention_decode(cache, batch, q.transpose(1, 2)), lambda: hp.paged_attention_decode(cache, batch, q.cpu()),
+                 lambda: hp.paged_attention_decode(cache, batch, q.bfloat16()), lambda: hp.paged_attention_decode(cache, ragged, q),
+                 lambda: hp.paged_attention_prompt(cache, batch, q), lambda: hp.paged_attention_decode(cache, batch, q, out=q),
+                 lambda: hp.paged_attention_decode(cache, batch, q, out=torch.empty_like(q).float()), lambda: hp.paged_attention_decode(cache, batch, q[:, :3]),
+                 lambda: hp.paged_attention_decode(cache, batch, q, workspace=torch.empty(0, dtype=torch.uint8, device="cuda")),
+                 lambda: hp.kv_cache_append(cache, batch, k[:1], k), lambda: hp.kv_cache_append(cache, batch, k.bfloat16(), k.bfloat16()),
+                 lambda: hp.kv_cache_append(cache, batch, k, k.float()), lambda: hp.kv_cache_append(cache, batch, k, k, q.float()),
+                 lambda: hp.kv_cache_append(cache, batch, k, k, q, hp.Rotary(torch.zeros(9, 4, device="cuda"), torch.zeros(9, 4, device="cuda")))):
+        with pytest.raises(capi.BoltError):
+            call()
