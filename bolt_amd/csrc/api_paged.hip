@@ -130,9 +130,9 @@ EE check_heads(U32 heads, const PagedPool &pool)
         }                       \
     } while (0)
 
-size_t workspace_bytes(const PagedPool &, const PagedBatch &, U32)
+size_t workspace_bytes(const PagedPool &pool, const PagedBatch &, U32 heads)
 {
-    return 256;
+    return paged_decode_workspace(pool, heads);
 }
 
 EE attention(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataType dt, U32 heads, const void *q, U32 qStride, void *out,
@@ -177,7 +177,7 @@ EE attention(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataTyp
     a.window = window;
     a.scale2 = scale * 1.44269504088896340736f;  // exp(x) = exp2(x log2(e))
     a.ws = workspace;
-    HIP_TRY(launch_paged_rows(a, ctx().stream));
+    HIP_TRY(decode ? launch_paged_decode(a, ctx().stream) : launch_paged_rows(a, ctx().stream));
     return SUCCESS;
 }
 

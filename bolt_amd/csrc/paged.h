@@ -41,6 +41,8 @@ struct PagedAttentionArgs {
     float scale2 = 0;                       // score scale * log2(e)
     void *ws = nullptr;
 };
+hipError_t launch_paged_decode(const PagedAttentionArgs &a, hipStream_t st);
+size_t paged_decode_workspace(const PagedPool &pool, uint32_t heads);  // bytes
 hipError_t launch_paged_rows(const PagedAttentionArgs &a, hipStream_t st);
 
 }  // namespace bg

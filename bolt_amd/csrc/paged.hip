@@ -1,97 +1,8 @@
 // Paged key / value cache: storing the keys and values of new tokens (with the position rotation of keys and queries on
 // the way), and attention over what is stored.
-#include "paged.h"
+#include "paged_device.h"
 
 namespace bg {
-
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ float bf16_to_f32(uint32_t h)
-{
-    return __uint_as_float(h << 16);
-}
-
-// round to nearest even; NaN keeps its sign and becomes quiet
-__device__ __forceinline__ uint32_t f32_to_bf16(float f)
-{
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) {
-        return (u >> 16) | 0x40u;
-    }
-    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-}
-
-// eight consecutive elements (16-byte aligned) <-> fp32
-template <int T>
-__device__ __forceinline__ void load8(const void *p, size_t at, float *x)
-{
-    if (T == PT_F32) {
-        const v4f a = ((const v4f *)((const float *)p + at))[0], b = ((const v4f *)((const float *)p + at))[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = a[i];
-            x[4 + i] = b[i];
-        }
-    } else if (T == PT_F16) {
-        const v8h a = *(const v8h *)((const uint16_t *)p + at);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = (float)a[i];
-        }
-    } else {
-        const v4u a = *(const v4u *)((const uint16_t *)p + at);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(a[i] << 16);
-            x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
-        }
-    }
-}
-
-template <int T>
-__device__ __forceinline__ void store8(void *p, size_t at, const float *x)
-{
-    if (T == PT_F32) {
-        v4f a, b;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a[i] = x[i];
-            b[i] = x[4 + i];
-        }
-        ((v4f *)((float *)p + at))[0] = a;
-        ((v4f *)((float *)p + at))[1] = b;
-    } else if (T == PT_F16) {
-        v8h a;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            a[i] = (_Float16)x[i];
-        }
-        *(v8h *)((uint16_t *)p + at) = a;
-    } else {
-        v4u a;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a[i] = f32_to_bf16(x[2 * i]) | (f32_to_bf16(x[2 * i + 1]) << 16);
-        }
-        *(v4u *)((uint16_t *)p + at) = a;
-    }
-}
-
-__device__ __forceinline__ float load1(const void *p, size_t at, int type)
-{
-    if (type == PT_F32) {
-        return ((const float *)p)[at];
-    }
-    if (type == PT_F16) {
-        return (float)((const _Float16 *)p)[at];
-    }
-    if (type == PT_BF16) {
-        return bf16_to_f32(((const uint16_t *)p)[at]);
-    }
-    return (float)((const int8_t *)p)[at];
-}
 
 // ---- append -----------------------------------------------------------------------------------------
 // One workgroup per packed row; DIM / 16 lanes per head row, query heads first, then keys, then values. A lane owns two
@@ -272,24 +183,6 @@ __global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttentionArgs a)
 
 namespace {
 
-// (activation type, cache type, head size) -> instantiation; the C-ABI layer refuses every other combination
-template <template <int, int, int> class F, typename A>
-hipError_t dispatch(int act, int ct, uint32_t dim, const A &a, hipStream_t st)
-{
-#define BG_PAGED(X, C)                                  \
-    if (act == X && ct == C) {                          \
-        return dim == 64 ? F<X, C, 64>::run(a, st) : F<X, C, 128>::run(a, st); \
-    }
-    BG_PAGED(PT_F32, PT_F16)
-    BG_PAGED(PT_F32, PT_I8)
-    BG_PAGED(PT_F16, PT_F16)
-    BG_PAGED(PT_F16, PT_I8)
-    BG_PAGED(PT_BF16, PT_BF16)
-    BG_PAGED(PT_BF16, PT_I8)
-#undef BG_PAGED
-    return hipErrorInvalidValue;
-}
-
 template <int ACT, int CT, int DIM>
 struct Append {
     static hipError_t run(const PagedAppendArgs &a, hipStream_t st)
@@ -314,12 +207,12 @@ struct Rows {
 
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t st)
 {
-    return a.batch.rows && a.batch.batch ? dispatch<Append>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
+    return a.batch.rows && a.batch.batch ? paged_dispatch<Append>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
 }
 
 hipError_t launch_paged_rows(const PagedAttentionArgs &a, hipStream_t st)
 {
-    return a.batch.rows && a.batch.batch ? dispatch<Rows>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
+    return a.batch.rows && a.batch.batch ? paged_dispatch<Rows>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
 }
 
 }  // namespace bg

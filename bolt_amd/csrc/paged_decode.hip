@@ -1,0 +1,498 @@
+// Attention of one new token per sequence over a paged cache. What bounds it is reading the keys and values once; the
+// arithmetic is on the matrix cores so that it hides behind that, with the heads of a group (which share keys) as columns.
+//
+// A wave walks over its keys in steps of 32, all operands in registers (v_mfma_f32_16x16x32):
+//   scores^T = K Q^T    lane (c = lane % 16, g = lane / 16) feeds eight d of key c and of query c; the result leaves it
+//                       the scores of keys 4g .. 4g + 3 of both 16-key halves, for query c
+//   out^T = V^T P^T     contraction over the 32 keys in the order the scores already lie in, so P goes in as it is. Row t of
+//                       the lane's V operand is d = (DIM / 16) c + t of its own eight keys: each lane loads DIM / 16
+//                       neighbouring d of eight keys (a 16-lane group reads whole rows) and pairs two keys' values per
+//                       register with one byte permutation. Which d a result row means is then (DIM / 16) m + t.
+// Neither LDS nor a transposed copy of V is needed. Weights are split into two 16-bit parts (their rounding would
+// otherwise be as large as the output's); fp32 queries are, too, after a power of two brought their row into fp16's range.
+// The running maximum is only raised once a score exceeds it by 2 (base 2): weights are scaled by 2^13 and stay below
+// 2^15, inside fp16; a weight of less than 2^-37 of the row's largest is lost. An int8 cache's steps (1 / scale) are part of
+// the weights, divided by a power of two that no step exceeds, so that they add nothing to that range.
+//
+// The keys of all sequences are cut into chunks of equal length, chosen on the device from the lengths themselves (a
+// captured launch serves any lengths): about kTarget workgroups in all. A sequence with one chunk writes its output;
+// several leave (maximum, sum, output) parts, which a second launch joins.
+#include "paged_device.h"
+
+namespace bg {
+
+namespace {
+
+constexpr uint32_t kTarget = 1024;   // workgroups that a launch aims at
+constexpr uint32_t kTile = 128;      // keys of one round of a workgroup's four waves
+constexpr uint32_t kMinTiles = 2;    // shortest chunk, in tiles
+constexpr float kLow = -1.7e38f;     // running maximum before the first key
+constexpr float kSlack = 2.0f, kLift = 13.0f;  // see above: 2^(kSlack + kLift) fits fp16
+
+struct Chunk {
+    uint32_t b, index, count, part;  // sequence; which of its chunks, of how many; its first part's number
+};
+
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v)
+{
+#pragma unroll
+    for (int off = 32; off; off >>= 1) {
+        v += __shfl_xor(v, off, 64);
+    }
+    return v;
+}
+
+__device__ __forceinline__ PagedSpan span_of(const PagedAttentionArgs &a, uint32_t b)
+{
+    return paged_span((int64_t)a.batch.lens[b] - 1, a.window, a.batch.max_pages << a.pool.shift);
+}
+
+// tiles of a sequence, counted from its first key rounded down to a step of 32
+__device__ __forceinline__ uint32_t tiles_of(const PagedAttentionArgs &a, uint32_t b)
+{
+    const PagedSpan s = span_of(a, b);
+    return (s.hi - (s.lo & ~31u) + kTile - 1) / kTile;
+}
+
+__device__ __forceinline__ uint32_t chunks_of(uint32_t tiles, uint32_t per)
+{
+    return tiles ? (tiles - 1) / per + 1 : 1;
+}
+
+// Tiles per chunk. per_head: chunks that a key head's share of the launch has room for beside one per sequence.
+__device__ __forceinline__ uint32_t tiles_per_chunk(const PagedAttentionArgs &a, uint32_t per_head, uint32_t lane)
+{
+    // a launch has at most 65535 sequences of 2^24 tiles: summed in units that fit 32 bits
+    uint32_t sum = 0;
+    for (uint32_t b = lane; b < a.batch.batch; b += 64) {
+        sum += (tiles_of(a, b) + 511) / 512;
+    }
+    const uint32_t coarse = wave_sum_u32(sum);
+    uint32_t per;
+    if (coarse < (1u << 22)) {
+        sum = 0;
+        for (uint32_t b = lane; b < a.batch.batch; b += 64) {
+            sum += tiles_of(a, b);
+        }
+        per = (wave_sum_u32(sum) + per_head - 1) / per_head;
+    } else {
+        per = (coarse / per_head + 1) * 512;
+    }
+    return per < kMinTiles ? kMinTiles : per;
+}
+
+// Chunk number x of the launch's list (false: behind the last); every wave finds out by itself.
+__device__ __forceinline__ bool find_chunk(const PagedAttentionArgs &a, uint32_t per, uint32_t x, uint32_t lane, Chunk *out)
+{
+    uint32_t base = 0, part = 0;
+    for (uint32_t b0 = 0; b0 < a.batch.batch; b0 += 64) {
+        const uint32_t b = b0 + lane;
+        const uint32_t n = b < a.batch.batch ? chunks_of(tiles_of(a, b), per) : 0;
+        uint32_t upto = n;
+#pragma unroll
+        for (uint32_t off = 1; off < 64; off <<= 1) {
+            const uint32_t v = __shfl_up(upto, off, 64);
+            upto += lane >= off ? v : 0;
+        }
+        const uint32_t all = __shfl(upto, 63, 64), parts = n > 1 ? n : 0;
+        if (x < base + all) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(base + upto > x));
+            out->b = b0 + at;
+            out->count = __builtin_amdgcn_readlane(n, at);
+            out->index = x - base - (__builtin_amdgcn_readlane(upto, at) - out->count);
+            out->part = part + wave_sum_u32(lane < at ? parts : 0);
+            return true;
+        }
+        base += all;
+        part += wave_sum_u32(parts);
+    }
+    return false;
+}
+
+// Parts of split sequences: room for 2 * per_head of them per key head and query tile (a sequence with n > 1 chunks has more
+// than (n - 1) * per tiles, so n <= 2 (n - 1) < 2 tiles / per in the sum). A part: 16 rows of DIM values, 16 maxima, 16 sums.
+__device__ __forceinline__ float *part_at(const PagedAttentionArgs &a, uint32_t per_head, uint32_t column, uint32_t part, uint32_t dim)
+{
+    return (float *)a.ws + ((size_t)column * 2 * per_head + part) * 16 * (dim + 2);
+}
+
+template <int ACT>
+__device__ __forceinline__ void store_out4(void *out, size_t at, v4f v)
+{
+    if (ACT == PT_F32) {
+        *(v4f *)((float *)out + at) = v;
+    } else if (ACT == PT_F16) {
+        typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+        *(v4h *)((uint16_t *)out + at) = (v4h){(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    } else {
+        *(v2u *)((uint16_t *)out + at) = (v2u){f32_to_bf16(v[0]) | (f32_to_bf16(v[1]) << 16), f32_to_bf16(v[2]) | (f32_to_bf16(v[3]) << 16)};
+    }
+}
+
+// PAGE16: pages of 16 keys and more, so that each 16-key half of a step lies in one page and its address is the wave's.
+template <int ACT, int CT, int DIM, bool PAGE16>
+__global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttentionArgs a, uint32_t per_head)
+{
+    typedef CacheOperand<CT> Op;
+    constexpr int kSteps = DIM / 32, kVec = DIM / 16;
+    constexpr uint32_t kRowBytes = DIM * (CT == PT_I8 ? 1 : 2), kRow = DIM + 4;
+    constexpr bool kSplitQ = ACT == PT_F32, kShiftQ = ACT == PT_F32 || (ACT == PT_BF16 && CT == PT_I8);
+    __shared__ __attribute__((aligned(16))) float sO[4][16 * kRow];
+    __shared__ float sM[4][16], sL[4][16];
+
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t c = lane & 15, g = lane >> 4;
+    Chunk ch;
+    const uint32_t per = tiles_per_chunk(a, per_head, lane);
+    if (!find_chunk(a, per, blockIdx.x, lane, &ch)) {
+        return;
+    }
+    const uint32_t group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
+    const uint32_t kvh = blockIdx.y / qtiles, q0 = blockIdx.y % qtiles * 16;
+    const uint32_t nq = group - q0 < 16 ? group - q0 : 16;
+    const uint32_t b = __builtin_amdgcn_readfirstlane(ch.b);
+    const PagedSpan span = span_of(a, b);
+    const uint32_t first = span.lo & ~31u, tiles = (span.hi - first + kTile - 1) / kTile;
+    const uint32_t mine = (tiles + ch.count - 1) / ch.count;  // tiles per chunk, evenly
+    const uint32_t from = first + ch.index * mine * kTile;
+    const uint32_t to = min(from + mine * kTile, span.hi);
+    const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
+
+    // queries
+    typename Op::V qh[kSteps], ql[kSteps];
+    float xscale = a.scale2;
+    {
+        float x[kSteps][8];
+        const size_t at = (size_t)b * a.qstride + (size_t)(kvh * group + q0 + c) * DIM;
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (c < nq) {
+                load8<ACT>(a.q, at + Op::d_of(s, g), x[s]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[s][j] = 0.0f;
+                }
+            }
+            if (kShiftQ) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    top = fmaxf(top, fabsf(x[s][j]));
+                }
+            }
+        }
+        float up = 1.0f;
+        if (kShiftQ) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            int e = 0;
+            up = shift_into_f16(top, &e);
+            xscale = ldexpf(a.scale2, e);
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            Op::split(x[s], up, &qh[s], &ql[s]);
+        }
+    }
+
+    v4f o[kVec];
+#pragma unroll
+    for (int t = 0; t < kVec; ++t) {
+        o[t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float m = kLow, l = 0.0f, unit = CT == PT_I8 ? kFirstUnit : 1.0f;  // unit: the power of two that o's int8 steps are divided by
+
+    for (uint32_t k0 = from + 32 * wave; k0 < to; k0 += kTile) {
+        typename Op::Raw kr[2][Op::kRawK(DIM)];
+        typename Op::template RawV<DIM> vr[8];
+        v4f ksc[2], vsc[2];
+        uint32_t seen = 0xff;  // bit j: key 16 (j / 4) + 4g + j % 4 of the step takes part
+        if (PAGE16) {
+            const uint8_t *kb[2], *vb[2];
+            bool whole = k0 >= span.lo && k0 + 32 <= to;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t key = k0 + 16 * h;
+                int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
+                if (slot < 0) {
+                    seen &= h ? 0x0f : 0xf0;
+                    whole = false;
+                    slot = 0;
+                }
+                kb[h] = (const uint8_t *)a.pool.k + slot * kRowBytes;
+                vb[h] = (const uint8_t *)a.pool.v + slot * kRowBytes;
+                if (CT == PT_I8) {
+                    ksc[h] = load_scales(a.pool.ks + slot + 4 * g);
+                    vsc[h] = load_scales(a.pool.vs + slot + 4 * g);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                Op::load_k(kb[h] + c * kRowBytes, g, kr[h]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                vr[j] = Op::template load_v<DIM>(vb[j >> 2] + (4 * g + (j & 3)) * kRowBytes, c);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                    if (key < span.lo || key >= to) {
+                        seen &= ~(1u << j);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t key = k0 + 16 * h + c;
+                int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
+                Op::load_k((const uint8_t *)a.pool.k + (slot < 0 ? 0 : slot) * kRowBytes, g, kr[h]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                int64_t slot = key >= span.lo && key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
+                if (slot < 0) {
+                    seen &= ~(1u << j);
+                    slot = 0;
+                }
+                vr[j] = Op::template load_v<DIM>((const uint8_t *)a.pool.v + slot * kRowBytes, c);
+                if (CT == PT_I8) {
+                    ksc[j >> 2][j & 3] = a.pool.ks[slot];
+                    vsc[j >> 2][j & 3] = a.pool.vs[slot];
+                }
+            }
+        }
+        v4f s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            s[h] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int t = 0; t < kSteps; ++t) {
+                const typename Op::V kv = Op::k_operand(kr[h], t);
+                s[h] = Op::mfma(kv, qh[t], s[h]);
+                if (kSplitQ) {
+                    s[h] = Op::mfma(kv, ql[t], s[h]);
+                }
+            }
+        }
+        float x[8], step[8], top = -INFINITY, wide = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float f = xscale;
+            if (CT == PT_I8) {
+                f *= __builtin_amdgcn_rcpf(ksc[j >> 2][j & 3]);
+                step[j] = __builtin_amdgcn_rcpf(vsc[j >> 2][j & 3]);
+            }
+            x[j] = s[j >> 2][j & 3] * f;
+        }
+        if (seen != 0xff) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (!(seen >> j & 1)) {
+                    x[j] = -INFINITY;
+                    if (CT == PT_I8) {
+                        step[j] = 0.0f;
+                    } else {
+                        vr[j] = Op::template zero_v<DIM>();
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            top = fmaxf(top, x[j]);
+            if (CT == PT_I8) {
+                wide = fmaxf(wide, step[j]);
+            }
+        }
+        if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float up = fmaxf(top, m);
+            float corr = __builtin_amdgcn_exp2f(m - up);
+            l *= corr;
+            m = up;
+            if (CT == PT_I8) {
+                const float was = unit;
+                wide = fmaxf(wide, unit);
+#pragma unroll
+                for (int off = 32; off; off >>= 1) {
+                    wide = fmaxf(wide, __shfl_xor(wide, off, 64));
+                }
+                unit = power_above(wide);
+                corr *= was * __builtin_amdgcn_rcpf(unit);
+            }
+#pragma unroll
+            for (int t = 0; t < kVec; ++t) {
+                o[t] = o[t] * corr;
+            }
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(x[j] - m + kLift);
+            l += p[j];
+        }
+        if (CT == PT_I8) {
+            const float per_unit = __builtin_amdgcn_rcpf(unit);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] *= step[j] * per_unit;
+            }
+        }
+        typename Op::V ph, pl;
+        Op::split(p, 1.0f, &ph, &pl);
+#pragma unroll
+        for (int t = 0; t < kVec; ++t) {
+            const typename Op::V vt = Op::template v_operand<DIM>(vr, t);
+            o[t] = Op::mfma(vt, ph, o[t]);
+            o[t] = Op::mfma(vt, pl, o[t]);
+        }
+    }
+
+    // the four waves' parts
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g == 0) {
+        sM[wave][c] = m;
+        sL[wave][c] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int t = 0; t < kVec; t += 4) {
+            *(v4f *)(&sO[wave][c * kRow + kVec * (4 * g + i) + t]) = (v4f){o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]} * unit;
+        }
+    }
+    __syncthreads();
+    float *part = part_at(a, per_head, blockIdx.y, ch.part + ch.index, DIM);
+    for (uint32_t at = threadIdx.x; at < nq * (DIM / 4); at += 256) {
+        const uint32_t r = at / (DIM / 4), d = at % (DIM / 4) * 4;
+        const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
+        float sum = 0.0f;
+        v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sM[w][r] - top);
+            sum += sL[w][r] * f;
+            v += *(const v4f *)(&sO[w][r * kRow + d]) * f;
+        }
+        if (ch.count == 1) {
+            v = sum == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
+            store_out4<ACT>(a.out, (size_t)b * a.ostride + (size_t)(kvh * group + q0 + r) * DIM + d, v);
+        } else {
+            *(v4f *)(part + r * DIM + d) = v;
+            if (d == 0) {
+                part[16 * DIM + r] = top;
+                part[16 * DIM + 16 + r] = sum;
+            }
+        }
+    }
+}
+
+// Joins the parts of split sequences: a workgroup per query head and sequence, DIM / 4 lanes to a part.
+template <int ACT, int DIM>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionArgs a, uint32_t per_head)
+{
+    constexpr uint32_t kLanes = DIM / 4, kWays = 256 / kLanes;
+    __shared__ __attribute__((aligned(16))) float sO[kWays][DIM];
+    __shared__ float sL[kWays], sM[kWays];
+    const uint32_t lane = threadIdx.x & 63, h = blockIdx.x, b = blockIdx.y;
+    const uint32_t per = tiles_per_chunk(a, per_head, lane);
+    const uint32_t count = chunks_of(tiles_of(a, b), per);
+    if (count == 1) {
+        return;
+    }
+    uint32_t before = 0;
+    for (uint32_t i = lane; i < b; i += 64) {
+        const uint32_t n = chunks_of(tiles_of(a, i), per);
+        before += n > 1 ? n : 0;
+    }
+    before = wave_sum_u32(before);
+    const uint32_t group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
+    const uint32_t kvh = h / group, in = h % group, r = in % 16;
+    const float *part = part_at(a, per_head, kvh * qtiles + in / 16, before, DIM);
+    const uint32_t way = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    float top = kLow, sum = 0.0f;
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i = way; i < count; i += kWays) {
+        const float *p = part + (size_t)i * 16 * (DIM + 2);
+        const float m = p[16 * DIM + r], up = fmaxf(top, m);
+        const float f = __builtin_amdgcn_exp2f(top - up), e = __builtin_amdgcn_exp2f(m - up);
+        sum = sum * f + p[16 * DIM + 16 + r] * e;
+        v = v * f + *(const v4f *)(p + r * DIM + d) * e;
+        top = up;
+    }
+    *(v4f *)(&sO[way][d]) = v;
+    if (d == 0) {
+        sM[way] = top;
+        sL[way] = sum;
+    }
+    __syncthreads();
+    if (way == 0) {
+        float up = sM[0];
+#pragma unroll
+        for (uint32_t w = 1; w < kWays; ++w) {
+            up = fmaxf(up, sM[w]);
+        }
+        sum = 0.0f;
+        v = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t w = 0; w < kWays; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sM[w] - up);
+            sum += sL[w] * f;
+            v += *(const v4f *)(&sO[w][d]) * f;
+        }
+        v = sum == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
+        store_out4<ACT>(a.out, (size_t)b * a.ostride + (size_t)h * DIM + d, v);
+    }
+}
+
+uint32_t columns(uint32_t heads, uint32_t kv_heads)
+{
+    return kv_heads * ((heads / kv_heads + 15) / 16);
+}
+
+uint32_t chunks_per_head(uint32_t heads, uint32_t kv_heads)
+{
+    const uint32_t n = columns(heads, kv_heads);
+    return n >= kTarget ? 1 : (kTarget + n - 1) / n;
+}
+
+template <int ACT, int CT, int DIM>
+struct Decode {
+    static hipError_t run(const PagedAttentionArgs &a, hipStream_t st)
+    {
+        const uint32_t per_head = chunks_per_head(a.heads, a.pool.kv_heads);
+        const dim3 grid(per_head + a.batch.batch, columns(a.heads, a.pool.kv_heads));
+        if (a.pool.shift >= 4) {
+            hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, true>), grid, dim3(256), 0, st, a, per_head);
+        } else {
+            hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, false>), grid, dim3(256), 0, st, a, per_head);
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) {
+            return e;
+        }
+        hipLaunchKernelGGL((paged_join_kernel<ACT, DIM>), dim3(a.heads, a.batch.batch), dim3(256), 0, st, a, per_head);
+        return hipGetLastError();
+    }
+};
+
+}  // namespace
+
+size_t paged_decode_workspace(const PagedPool &pool, uint32_t heads)
+{
+    return (size_t)columns(heads, pool.kv_heads) * 2 * chunks_per_head(heads, pool.kv_heads) * 16 * (pool.dim + 2) * sizeof(float);
+}
+
+hipError_t launch_paged_decode(const PagedAttentionArgs &a, hipStream_t st)
+{
+    return a.batch.rows && a.batch.batch ? paged_dispatch<Decode>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
+}
+
+}  // namespace bg

@@ -8,7 +8,11 @@ off that rounds where the operator says it does. For a row with weights w, value
   du: the rounding of the weights to the type the products run in (16-bit types round to nearest: eps / 2; fp32
       activations carry two 16-bit parts, 2^-21)
   dn: the sums over n keys in fp32, (n + 16) 2^-24
-  |error| <= (2 ds + 2 du + 2 dn) A + (eps / 2) |out| + tiny    (weights and their sum each are off by ds + du + dn)
+  da: fp16 products (an fp16 or int8 cache) hold the weights scaled so that the row's largest is 2^13 at least, where fp16's
+      smallest step is 2^-24: each of n weights is off by up to 2^-37 of the largest, whatever it is itself, and the
+      sum of the weights is no smaller than the largest: n 2^-37 max |v|. int8 values carry their slot's step in the weight,
+      over a power of two up to twice the largest step: n 2^-37 2 127 max step
+  |error| <= da + (2 ds + 2 du + 2 dn) A + (eps / 2) |out| + tiny    (weights and their sum each are off by ds + du + dn)
   tiny: below the smallest normal number n the output type's steps are n eps wide and stay that wide towards zero, so that
       rounding to the nearest is off by up to n eps / 2 there, however small the value (fp16: 2^-14 2^-10 / 2 = 2^-25)"""
 import numpy as np
@@ -62,7 +66,7 @@ class Case:
         return cache, batch, self.q.cuda()
 
     def stored(self, b, j):
-        """(positions with a page, keys, values) of sequence b, key head j, in 64 bits"""
+        """(positions with a page, keys, values, steps of the values) of sequence b, key head j, in 64 bits"""
         pos = [p for p in range(min(self.lengths[b], self.max_pages * self.page)) if 0 <= int(self.table[b, p // self.page]) < self.pages]
         page = self.table[b, torch.tensor([p // self.page for p in pos], dtype=torch.long)].long()
         slot = torch.tensor([p % self.page for p in pos], dtype=torch.long)
@@ -70,7 +74,8 @@ class Case:
         if self.ks is not None:
             k = k / self.ks[page, j, slot].double()[:, None]
             v = v / self.vs[page, j, slot].double()[:, None]
-        return np.array(pos, dtype=np.int64), k.numpy(), v.numpy()
+        steps = np.ones(len(pos)) if self.vs is None else 1 / self.vs[page, j, slot].double().numpy()
+        return np.array(pos, dtype=np.int64), k.numpy(), v.numpy(), steps
 
     def attention(self, scale=None):
         """(out, bound) as float64 arrays [rows, heads, dim]; rows that nobody owns are NaN"""
@@ -84,7 +89,7 @@ class Case:
         q = self.q.double().numpy()
         for b, (total, n) in enumerate(zip(self.lengths, self.new)):
             for j in range(self.kv_heads):
-                pos, k, v = self.stored(b, j)
+                pos, k, v, steps = self.stored(b, j)
                 for i in range(n):
                     p = total - n + i
                     sees = (pos <= p) & (pos > p - self.window if self.window else True)
@@ -103,7 +108,8 @@ class Case:
                         if wide:  # two 16-bit parts of q
                             ds += 2.0 ** -21 * (np.abs(kk) @ np.abs(q[row, h])).max() * abs(scale)
                         out[row, h] = w @ vv
-                        bound[row, h] = 2 * (ds + unit + (len(w) + 16) * 2.0 ** -24) * a + half * np.abs(out[row, h]) + tiny
+                        da = 0.0 if self.cache == "bf16" else len(w) * 2.0 ** -37 * (np.abs(vv).max(0) if self.cache == "f16" else 254 * steps[sees].max())
+                        bound[row, h] = da + 2 * (ds + unit + (len(w) + 16) * 2.0 ** -24) * a + half * np.abs(out[row, h]) + tiny
         return out, bound
 
 
