@@ -122,6 +122,11 @@ EE check_heads(U32 heads, const PagedPool &pool)
     return heads % pool.kv_heads ? contradict("the query heads are a multiple of the key heads") : SUCCESS;
 }
 
+EE check_grid(const PagedPool &pool, const PagedBatch &batch, U32 heads)
+{
+    return !batch.offsets || paged_prompt_fits(pool, batch, heads) ? SUCCESS : refuse("more rows times heads than a launch can have");
+}
+
 #define EE_TRY(expr)            \
     do {                        \
         const EE ee__ = (expr); \
@@ -130,9 +135,13 @@ EE check_heads(U32 heads, const PagedPool &pool)
         }                       \
     } while (0)
 
-size_t workspace_bytes(const PagedPool &pool, const PagedBatch &, U32 heads)
+// zero rows or sequences: nothing is launched
+size_t workspace_bytes(const PagedPool &pool, const PagedBatch &batch, U32 heads)
 {
-    return paged_decode_workspace(pool, heads);
+    if (batch.batch == 0 || batch.rows == 0) {
+        return 256;
+    }
+    return batch.offsets ? paged_prompt_workspace(pool, batch, heads) : paged_decode_workspace(pool, heads);
 }
 
 EE attention(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataType dt, U32 heads, const void *q, U32 qStride, void *out,
@@ -144,6 +153,7 @@ EE attention(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataTyp
     EE_TRY(check_batch(batch, a.pool, &a.batch));
     EE_TRY(check_types(dt, a.pool, &esize));
     EE_TRY(check_heads(heads, a.pool));
+    EE_TRY(check_grid(a.pool, a.batch, heads));
     if (decode && a.batch.offsets) {
         return contradict("decode takes one row per sequence: offsets == NULL");
     }
@@ -177,7 +187,7 @@ EE attention(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataTyp
     a.window = window;
     a.scale2 = scale * 1.44269504088896340736f;  // exp(x) = exp2(x log2(e))
     a.ws = workspace;
-    HIP_TRY(decode ? launch_paged_decode(a, ctx().stream) : launch_paged_rows(a, ctx().stream));
+    HIP_TRY(decode ? launch_paged_decode(a, ctx().stream) : launch_paged_prompt(a, ctx().stream));
     return SUCCESS;
 }
 
@@ -253,6 +263,7 @@ EE bolt_gfx950_paged_attention_workspace_bytes(const BoltPagedKvCache *cache, co
     EE_TRY(check_pool(cache, &pool));
     EE_TRY(check_batch(batch, pool, &b));
     EE_TRY(check_heads(heads, pool));
+    EE_TRY(check_grid(pool, b, heads));
     *bytes = workspace_bytes(pool, b, heads);
     return SUCCESS;
 }

@@ -1,5 +1,5 @@
-// Paged key / value cache: storing the keys and values of new tokens (with the position rotation of keys and queries on
-// the way), and attention over what is stored.
+// Paged key / value cache: storing the keys and values of new tokens, with the position rotation of keys and queries on the
+// way.
 #include "paged_device.h"
 
 namespace bg {
@@ -102,85 +102,6 @@ __global__ void paged_append_kernel(PagedAppendArgs a)
     }
 }
 
-// ---- attention, one row of one head per wave -------------------------------------------------------
-// The streaming softmax: lanes hold the scores of 64 keys, then the output's DIM values.
-template <int ACT, int CT, int DIM>
-__global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttentionArgs a)
-{
-    __shared__ float sp[64];
-    __shared__ int64_t ss[64];
-    __shared__ float sq[DIM];
-    const uint32_t row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const uint32_t b = paged_owner(a.batch, row);
-    const PagedSeq s = paged_seq(a.batch, b);
-    const int64_t i = (int64_t)row - s.first;
-    if (i < 0 || i >= s.count) {
-        return;
-    }
-    const uint32_t kvh = h / (a.heads / a.pool.kv_heads);
-    const PagedSpan span = paged_span(s.pos + i, a.window, a.batch.max_pages << a.pool.shift);
-    const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
-    for (uint32_t d = lane; d < DIM; d += 64) {
-        sq[d] = load1(a.q, (size_t)row * a.qstride + (size_t)h * DIM + d, ACT);
-    }
-    float m = -INFINITY, l = 0.0f, o[DIM / 64];
-    for (int t = 0; t < DIM / 64; ++t) {
-        o[t] = 0.0f;
-    }
-    for (uint32_t k0 = span.lo; k0 < span.hi; k0 += 64) {
-        __syncthreads();
-        const uint32_t key = k0 + lane;
-        const int64_t slot = key < span.hi ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
-        float dot = 0.0f, x = -INFINITY;
-        if (slot >= 0) {
-            for (int d = 0; d < DIM; ++d) {
-                dot = __builtin_fmaf(sq[d], load1(a.pool.k, (size_t)slot * DIM + d, CT), dot);
-            }
-            if (CT == PT_I8) {
-                dot *= 1.0f / a.pool.ks[slot];
-            }
-            x = dot * a.scale2;
-        }
-        float top = x;
-        for (int off = 32; off; off >>= 1) {
-            top = fmaxf(top, __shfl_xor(top, off, 64));
-        }
-        top = fmaxf(top, m);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        const float p = slot >= 0 ? exp2f(x - ref) : 0.0f, corr = exp2f(m - ref);
-        float sum = p;
-        for (int off = 32; off; off >>= 1) {
-            sum += __shfl_xor(sum, off, 64);
-        }
-        l = l * corr + sum;
-        m = top;
-        sp[lane] = CT == PT_I8 && slot >= 0 ? p * (1.0f / a.pool.vs[slot]) : p;
-        ss[lane] = slot;
-        __syncthreads();
-        for (int t = 0; t < DIM / 64; ++t) {
-            o[t] *= corr;
-        }
-        for (uint32_t j = 0; j < 64; ++j) {
-            if (ss[j] >= 0) {
-                for (int t = 0; t < DIM / 64; ++t) {
-                    o[t] = __builtin_fmaf(sp[j], load1(a.pool.v, (size_t)ss[j] * DIM + 64 * t + lane, CT), o[t]);
-                }
-            }
-        }
-    }
-    for (int t = 0; t < DIM / 64; ++t) {
-        const size_t at = (size_t)row * a.ostride + (size_t)h * DIM + 64 * t + lane;
-        const float v = l == 0.0f ? 0.0f : o[t] / l;
-        if (ACT == PT_F32) {
-            ((float *)a.out)[at] = v;
-        } else if (ACT == PT_F16) {
-            ((_Float16 *)a.out)[at] = (_Float16)v;
-        } else {
-            ((uint16_t *)a.out)[at] = (uint16_t)f32_to_bf16(v);
-        }
-    }
-}
-
 namespace {
 
 template <int ACT, int CT, int DIM>
@@ -194,25 +115,11 @@ struct Append {
     }
 };
 
-template <int ACT, int CT, int DIM>
-struct Rows {
-    static hipError_t run(const PagedAttentionArgs &a, hipStream_t st)
-    {
-        hipLaunchKernelGGL((paged_rows_kernel<ACT, CT, DIM>), dim3(a.batch.rows, a.heads), dim3(64), 0, st, a);
-        return hipGetLastError();
-    }
-};
-
 }  // namespace
 
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t st)
 {
     return a.batch.rows && a.batch.batch ? paged_dispatch<Append>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
-}
-
-hipError_t launch_paged_rows(const PagedAttentionArgs &a, hipStream_t st)
-{
-    return a.batch.rows && a.batch.batch ? paged_dispatch<Rows>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
 }
 
 }  // namespace bg

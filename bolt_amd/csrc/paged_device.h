@@ -9,11 +9,6 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float bf16_to_f32(uint32_t h)
-{
-    return __uint_as_float(h << 16);
-}
-
 // round to nearest even; NaN keeps its sign and becomes quiet
 __device__ __forceinline__ uint32_t f32_to_bf16(float f)
 {
@@ -78,20 +73,6 @@ __device__ __forceinline__ void store8(void *p, size_t at, const float *x)
         }
         *(v4u *)((uint16_t *)p + at) = a;
     }
-}
-
-__device__ __forceinline__ float load1(const void *p, size_t at, int type)
-{
-    if (type == PT_F32) {
-        return ((const float *)p)[at];
-    }
-    if (type == PT_F16) {
-        return (float)((const _Float16 *)p)[at];
-    }
-    if (type == PT_BF16) {
-        return bf16_to_f32(((const uint16_t *)p)[at]);
-    }
-    return (float)((const int8_t *)p)[at];
 }
 
 // ---- operands of the matrix instructions ------------------------------------------------------------

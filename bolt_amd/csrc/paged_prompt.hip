@@ -1,0 +1,668 @@
+// Attention of prompts over a paged cache: many new tokens per sequence, each seeing the keys up to its own. What bounds it
+// is the matrix cores.
+//
+// Rows of a tile are (token, head of a group) pairs, R = token * group + head: the heads of a group share keys, so a short
+// prompt of a grouped model still fills a tile. A workgroup owns 128 rows of one (sequence, key head), each of its four waves
+// 32, and walks over the keys it needs in tiles of 64 (v_mfma_f32_32x32x16):
+//   scores^T = K Q^T   lane (c = lane % 32, h = lane / 32) feeds eight d of key c (from LDS) and of row c (registers); the
+//                      result leaves it, for row c, the scores of keys 8 i + 4 h + 0..3, i = 0..3, of each half of the tile
+//   out^T = V^T P^T    contraction over the keys in the order the scores lie in: P goes from the accumulators into the
+//                      operand with no exchange between lanes; V^T comes from LDS through the transposing read
+//                      (ds_read_b64_tr_b16: a lane gets four keys' values of one d)
+// Key and value tiles go from memory to LDS without passing registers, one tile ahead, in pieces of 16 bytes; the pieces of
+// a row are permuted so that 16 lanes of either read pattern touch all banks. An int8 cache passes registers on the way
+// and lies in LDS as fp16, which holds its values exactly; its steps multiply scores and weights.
+// Where few tiles meet many keys, several workgroups share a tile's keys and a second launch joins their parts.
+#include "paged_device.h"
+
+namespace bg {
+
+namespace {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(1))) void *gptr_t;
+typedef __attribute__((address_space(3))) void *lptr_t;
+
+constexpr uint32_t kRows = 128, kKeys = 64;
+constexpr uint32_t kSpread = 512;  // workgroups below which a tile's keys are shared out
+constexpr uint32_t kLeast = 4;     // fewest key tiles per share
+constexpr float kLow = -1.7e38f;
+constexpr float kSlack = 2.0f, kLift = 13.0f;
+
+__device__ __attribute__((aligned(16))) uint32_t g_zeros[4];  // what stands in for a key that nobody stored
+
+struct Tile {
+    uint32_t b, index;
+};
+
+__device__ __forceinline__ uint32_t row_tiles(const PagedAttentionArgs &a, uint32_t b, uint32_t group)
+{
+    const PagedSeq s = paged_seq(a.batch, b);
+    const uint64_t n = s.count < (int64_t)a.batch.rows ? (uint64_t)s.count : a.batch.rows;
+    return (uint32_t)((n * group + kRows - 1) / kRows);
+}
+
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v)
+{
+#pragma unroll
+    for (int off = 32; off; off >>= 1) {
+        v += __shfl_xor(v, off, 64);
+    }
+    return v;
+}
+
+// Row tile number x of the launch, counted from the last one: the later tiles of a sequence see the most keys and start
+// first. Every wave finds out by itself.
+__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t group, uint32_t x, uint32_t lane, Tile *out)
+{
+    uint32_t all = 0;
+    for (uint32_t b = lane; b < a.batch.batch; b += 64) {
+        all += row_tiles(a, b, group);
+    }
+    all = wave_sum_u32(all);
+    if (x >= all) {
+        return false;
+    }
+    x = all - 1 - x;
+    uint32_t base = 0;
+    for (uint32_t b0 = 0; b0 < a.batch.batch; b0 += 64) {
+        const uint32_t n = b0 + lane < a.batch.batch ? row_tiles(a, b0 + lane, group) : 0;
+        uint32_t upto = n;
+#pragma unroll
+        for (uint32_t off = 1; off < 64; off <<= 1) {
+            const uint32_t v = __shfl_up(upto, off, 64);
+            upto += lane >= off ? v : 0;
+        }
+        const uint32_t sum = __builtin_amdgcn_readlane(upto, 63);
+        if (x < base + sum) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(base + upto > x));
+            out->b = b0 + at;
+            out->index = x - base - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
+            return true;
+        }
+        base += sum;
+    }
+    return false;
+}
+
+// What a tile's rows see: positions of the first and last row, keys [lo, hi) with lo rounded down to a tile
+struct Reach {
+    int64_t first, last;
+    uint32_t lo, hi, tiles;
+};
+
+__device__ __forceinline__ Reach reach_of(const PagedAttentionArgs &a, const PagedSeq &s, uint32_t tile, uint32_t group)
+{
+    Reach r;
+    const int64_t rows = s.count * group, r0 = (int64_t)tile * kRows, r1 = r0 + kRows < rows ? r0 + kRows : rows;
+    r.first = s.pos + r0 / group;
+    r.last = s.pos + (r1 - 1) / group;
+    const uint32_t capacity = a.batch.max_pages << a.pool.shift;
+    r.hi = paged_span(r.last, a.window, capacity).hi;
+    r.lo = paged_span(r.first > 0 ? r.first : 0, a.window, capacity).lo & ~(kKeys - 1);
+    r.tiles = r.hi > r.lo ? (r.hi - r.lo + kKeys - 1) / kKeys : 0;
+    return r;
+}
+
+__device__ __forceinline__ uint32_t tiles_per_share(uint32_t tiles, uint32_t shares)
+{
+    const uint32_t n = (tiles + shares - 1) / shares;
+    return n < kLeast ? kLeast : n;
+}
+
+// A share's part: 128 rows of DIM values, 128 maxima, 128 sums
+__device__ __forceinline__ float *part_at(const PagedAttentionArgs &a, uint32_t x, uint32_t kvh, uint32_t share, uint32_t shares, uint32_t dim)
+{
+    return (float *)a.ws + (((size_t)x * a.pool.kv_heads + kvh) * shares + share) * kRows * (dim + 2);
+}
+
+// place of 16-byte piece `piece` of row `row` in a tile's LDS image (units of 16 bytes)
+template <int DIM>
+__device__ __forceinline__ uint32_t swizzle_k(uint32_t row)
+{
+    return DIM == 128 ? row & 15 : (row >> 1) & 7;
+}
+
+template <int DIM>
+__device__ __forceinline__ uint32_t swizzle_v(uint32_t row)
+{
+    return DIM == 128 ? (row & 3) << 2 | ((row >> 2) & 3) : ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
+}
+
+template <int CT>
+struct Product {
+    typedef v8h V;
+    static __device__ __forceinline__ v16f mfma(V a, V b, v16f c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    // two values rounded to nearest
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2h));
+    }
+};
+template <>
+struct Product<PT_BF16> {
+    typedef v8b V;
+    static __device__ __forceinline__ v16f mfma(V a, V b, v16f c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2b));
+    }
+};
+
+template <int ACT>
+__device__ __forceinline__ void store_out4(void *out, size_t at, float a, float b, float c, float d)
+{
+    if (ACT == PT_F32) {
+        *(v4f *)((float *)out + at) = (v4f){a, b, c, d};
+    } else if (ACT == PT_F16) {
+        *(v2u *)((uint16_t *)out + at) = (v2u){Product<PT_F16>::pack(a, b), Product<PT_F16>::pack(c, d)};
+    } else {
+        *(v2u *)((uint16_t *)out + at) = (v2u){Product<PT_BF16>::pack(a, b), Product<PT_BF16>::pack(c, d)};
+    }
+}
+
+template <int CT, int DIM>
+constexpr uint32_t prompt_lds()
+{
+    return 4 * kKeys * DIM * 2 + (CT == PT_I8 ? 4 * kKeys * 4 : DIM * 8);
+}
+
+template <int ACT, int CT, int DIM>
+__global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs a, uint32_t shares)
+{
+    typedef Product<CT> Op;
+    typedef typename Op::V V;
+    constexpr bool kWide = ACT == PT_F32;                                            // two parts per operand
+    constexpr bool kShiftQ = kWide || (ACT == PT_BF16 && CT == PT_I8);
+    constexpr uint32_t kTileBytes = kKeys * DIM * 2, kRowBytes = DIM * (CT == PT_I8 ? 1 : 2), kPieces = DIM / 8;
+    constexpr int kSteps = DIM / 16, kOut = DIM / 32, kLoads = kTileBytes / 16 / 256;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    uint8_t *const sK = smem, *const sV = smem + 2 * kTileBytes;                     // two buffers each
+    float *const sStep = (float *)(smem + 4 * kTileBytes);                           // int8: [2][keys' 64, values' 64]
+    unsigned long long *const sBad = (unsigned long long *)(smem + 4 * kTileBytes);  // else: [DIM] keys whose value is not finite
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t c = lane & 31, h = lane >> 5;
+    const uint32_t kvh = blockIdx.x % a.pool.kv_heads, share = blockIdx.x / a.pool.kv_heads % shares, x = blockIdx.x / a.pool.kv_heads / shares;
+    const uint32_t group = a.heads / a.pool.kv_heads;
+    Tile tile;
+    if (!find_tile(a, group, x, lane, &tile)) {
+        return;
+    }
+    const uint32_t b = __builtin_amdgcn_readfirstlane(tile.b);
+    const PagedSeq seq = paged_seq(a.batch, b);
+    const Reach all = reach_of(a, seq, __builtin_amdgcn_readfirstlane(tile.index), group);
+    const uint32_t per = tiles_per_share(all.tiles, shares);
+    const uint32_t t0 = share * per, t1 = min(t0 + per, all.tiles);
+    if (share && t0 >= all.tiles) {
+        return;
+    }
+    const bool alone = per >= all.tiles;
+    const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
+
+    // this lane's row
+    const int64_t r = (int64_t)tile.index * kRows + 32 * wave + c, token = r / group;
+    const int64_t row = seq.first + token, pos = seq.pos + token;
+    const bool mine = r < seq.count * group && row >= 0 && row < (int64_t)a.batch.rows;
+    const uint32_t head = kvh * group + (uint32_t)(r % group);
+    const PagedSpan span = paged_span(mine ? pos : -1, a.window, all.hi);
+
+    V qh[kSteps], ql[kWide ? kSteps : 1];
+    float xscale = a.scale2;
+    {
+        const float sign = a.scale2 == 0.0f ? 0.0f : a.scale2 < 0.0f ? -1.0f : 1.0f;  // the factor of the scores is positive
+        xscale = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);
+        const size_t at = (size_t)(mine ? row : 0) * a.qstride + (size_t)(mine ? head : 0) * DIM + 8 * h;
+        float top = 0.0f, up = 1.0f;
+        if (kShiftQ) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                float v[8];
+                load8<ACT>(a.q, at + 16 * s, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    top = fmaxf(top, fabsf(v[j]));
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            int e = 0;
+            up = shift_into_f16(top, &e);
+            xscale = ldexpf(xscale, e);
+            xscale = xscale < 1.17549435e-38f ? 1.17549435e-38f : xscale;  // not zero: it meets scores of -inf
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            float v[8];
+            load8<ACT>(a.q, at + 16 * s, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] *= sign;
+            }
+            V lo;
+            Operand<CT>::split(v, up, &qh[s], &lo);
+            if (kWide) {
+                ql[s] = lo;
+            }
+        }
+    }
+
+    v16f o[kOut];
+#pragma unroll
+    for (int t = 0; t < kOut; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            o[t][i] = 0.0f;
+        }
+    }
+    float m = kLow, l = 0.0f, unit = CT == PT_I8 ? kFirstUnit : 1.0f;
+
+    // page of key k0 + lane; none: -1
+    auto page_of = [&](uint32_t k0) -> int32_t {
+        const uint32_t key = k0 + lane;
+        if (key >= all.hi) {
+            return -1;
+        }
+        const uint32_t p = (uint32_t)table[key >> a.pool.shift];
+        return p < a.pool.pages ? (int32_t)p : -1;
+    };
+    auto slot_of = [&](int32_t page, uint32_t key) -> size_t {
+        return (((size_t)(uint32_t)page * a.pool.kv_heads + kvh) << a.pool.shift) | (key & ((1u << a.pool.shift) - 1));
+    };
+    // 16-bit caches: straight into buffer `buf`
+    auto fetch = [&](uint32_t k0, int32_t pages, uint32_t buf) {
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const uint32_t at = (n * 4 + wave) * 64, rowk = (at + lane) / kPieces, piece = (at + lane) % kPieces;
+            const int32_t page = __shfl(pages, rowk, 64);
+            const size_t off = slot_of(page, k0 + rowk) * kRowBytes;
+            const uint8_t *kp = (const uint8_t *)a.pool.k + off + 16 * (piece ^ swizzle_k<DIM>(rowk));
+            const uint8_t *vp = (const uint8_t *)a.pool.v + off + 16 * (piece ^ swizzle_v<DIM>(rowk));
+            kp = page < 0 ? (const uint8_t *)g_zeros : kp;
+            vp = page < 0 ? (const uint8_t *)g_zeros : vp;
+            __builtin_amdgcn_global_load_lds((gptr_t)kp, (lptr_t)(sK + buf * kTileBytes + at * 16), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr_t)vp, (lptr_t)(sV + buf * kTileBytes + at * 16), 16, 0, 0);
+        }
+    };
+    // int8: eight values of a row per piece into registers, then as fp16 into the buffer
+    v2u rk[CT == PT_I8 ? kLoads : 1], rv[CT == PT_I8 ? kLoads : 1];
+    float rs = 0.0f;
+    auto fetch8 = [&](uint32_t k0, int32_t pages) {
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const uint32_t at = (n * 4 + wave) * 64, rowk = (at + lane) / kPieces, piece = (at + lane) % kPieces;
+            const int32_t page = __shfl(pages, rowk, 64);
+            const size_t off = page < 0 ? 0 : slot_of(page, k0 + rowk) * kRowBytes;
+            rk[n] = *(const v2u *)((const uint8_t *)a.pool.k + off + 8 * piece);
+            rv[n] = *(const v2u *)((const uint8_t *)a.pool.v + off + 8 * piece);
+        }
+        if (wave < 2) {
+            rs = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[slot_of(pages, k0 + lane)];
+        }
+    };
+    auto put8 = [&](uint32_t buf) {
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const uint32_t at = (n * 4 + wave) * 64, rowk = (at + lane) / kPieces, piece = (at + lane) % kPieces;
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                const v2u w = kv ? rv[n] : rk[n];
+                v4u f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f[i] = bytes_to_f16(__builtin_amdgcn_perm(0, w[i / 2], i & 1 ? 0x0c030c02 : 0x0c010c00));
+                }
+                const uint32_t place = rowk * kPieces + (piece ^ (kv ? swizzle_v<DIM>(rowk) : swizzle_k<DIM>(rowk)));
+                *(v4u *)((kv ? sV : sK) + buf * kTileBytes + place * 16) = f;
+            }
+        }
+        if (wave < 2) {
+            sStep[buf * 2 * kKeys + wave * kKeys + lane] = __builtin_amdgcn_rcpf(rs);
+        }
+    };
+
+    int32_t pages = t0 < t1 ? page_of(all.lo + t0 * kKeys) : -1, next = t0 + 1 < t1 ? page_of(all.lo + (t0 + 1) * kKeys) : -1;
+    if (t0 < t1) {
+        if (CT == PT_I8) {
+            fetch8(all.lo + t0 * kKeys, pages);
+        } else {
+            fetch(all.lo + t0 * kKeys, pages, 0);
+        }
+    }
+    for (uint32_t t = t0; t < t1; ++t) {
+        const uint32_t k0 = all.lo + t * kKeys, buf = (t - t0) & 1;
+        const unsigned long long stored = __ballot(pages >= 0);
+        if (CT == PT_I8) {
+            put8(buf);
+        }
+        __syncthreads();  // the tile is there; everyone is done with the other buffer
+        pages = next;
+        if (t + 1 < t1) {
+            if (CT == PT_I8) {
+                fetch8(k0 + kKeys, pages);
+            } else {
+                fetch(k0 + kKeys, pages, buf ^ 1);
+            }
+            next = t + 2 < t1 ? page_of(k0 + 2 * kKeys) : -1;
+        }
+        // does every row of the workgroup see every key of the tile?
+        const uint32_t last_lo = paged_span(all.last, a.window, all.hi).lo;
+        const bool whole = stored == ~0ull && (int64_t)k0 + kKeys - 1 <= all.first && k0 >= last_lo;
+        bool bad = false;
+        if (CT != PT_I8 && !whole) {
+            // a value that is infinite or NaN must not reach the rows that do not see its key (0 * inf): it is taken out of the tile
+            // and put into the rows that do
+            constexpr uint32_t kExp = CT == PT_BF16 ? 0x7f80u : 0x7c00u;
+            uint8_t *const base = sV + buf * kTileBytes;
+            bool hit = false;
+            for (uint32_t at = tid; at < kTileBytes / 4; at += 256) {
+                const uint32_t w = *(const uint32_t *)(base + at * 4);
+                hit |= (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
+            }
+            bad = __syncthreads_or(hit);
+            if (bad) {
+                for (uint32_t d = tid; d < DIM; d += 256) {
+                    sBad[d] = 0;
+                }
+                __syncthreads();
+                for (uint32_t at = tid; at < kKeys * DIM; at += 256) {
+                    const uint32_t rowk = at / DIM, d = at % DIM;
+                    uint16_t *const p = (uint16_t *)(base + (rowk * kPieces + (d / 8 ^ swizzle_v<DIM>(rowk))) * 16) + d % 8;
+                    if ((*p & kExp) == kExp) {
+                        atomicOr(&sBad[d], 1ull << rowk);
+                        *p = 0;
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        if (!__any(span.hi > k0 && span.lo < k0 + kKeys)) {
+            continue;  // nothing for this wave
+        }
+        // scores
+        v16f s[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                s[i][j] = 0.0f;
+            }
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+                const uint32_t rowk = 32 * i + c, place = rowk * kPieces + ((2 * st + h) ^ swizzle_k<DIM>(rowk));
+                const V kv = *(const V *)(sK + buf * kTileBytes + place * 16);
+                s[i] = Op::mfma(kv, qh[st], s[i]);
+                if (kWide) {
+                    s[i] = Op::mfma(kv, ql[st], s[i]);
+                }
+            }
+        }
+        float step[2][16], wide = 0.0f;
+        if (CT == PT_I8) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const uint32_t key = 32 * i + 2 * j + 4 * h;
+                    const v4f ks = *(const v4f *)(sStep + buf * 2 * kKeys + key), vs = *(const v4f *)(sStep + buf * 2 * kKeys + kKeys + key);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[i][j + e] *= ks[e];
+                        step[i][j + e] = vs[e];
+                    }
+                }
+            }
+        }
+        unsigned long long seen = ~0ull;
+        if (!whole) {
+            const uint32_t from = span.lo > k0 ? span.lo - k0 : 0, upto = span.hi > k0 ? span.hi - k0 : 0;  // keys of the tile this row sees
+            seen = from >= kKeys || upto <= from ? 0 : (upto >= kKeys ? ~0ull : (1ull << upto) - 1) & (~0ull << from);
+            seen &= stored;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t half = (uint32_t)(seen >> (32 * i)) >> (4 * h);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (!(half >> (8 * (j / 4) + j % 4) & 1)) {
+                        s[i][j] = -INFINITY;
+                        if (CT == PT_I8) {
+                            step[i][j] = 0.0f;
+                        }
+                    }
+                }
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                top = fmaxf(top, s[i][j]);
+                if (CT == PT_I8) {
+                    wide = fmaxf(wide, step[i][j]);
+                }
+            }
+        }
+        top *= xscale;
+        if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float up = fmaxf(top, m);
+            float corr = __builtin_amdgcn_exp2f(m - up);
+            l *= corr;
+            m = up;
+            if (CT == PT_I8) {
+                const float was = unit;
+                wide = fmaxf(wide, unit);
+#pragma unroll
+                for (int off = 32; off; off >>= 1) {
+                    wide = fmaxf(wide, __shfl_xor(wide, off, 64));
+                }
+                unit = power_above(wide);
+                corr *= was * __builtin_amdgcn_rcpf(unit);
+            }
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) {
+                o[i] = o[i] * corr;
+            }
+        }
+        const float shift = kLift - m, per_unit = __builtin_amdgcn_rcpf(unit);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], xscale, shift));
+                l += p;
+                if (CT == PT_I8) {
+                    p *= step[i][j] * per_unit;
+                }
+                s[i][j] = p;
+            }
+        }
+        // weights times values, 16 keys a step
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            V ph, pl;
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] = s[u / 2][8 * (u % 2) + j];
+            }
+            if (kWide) {
+                Operand<CT>::split(p, 1.0f, &ph, &pl);
+            } else {
+                Words<4> w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w.w[j] = Op::pack(p[2 * j], p[2 * j + 1]);
+                }
+                ph = __builtin_bit_cast(V, w);
+            }
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) {
+                // 16 lanes read four keys of 16 d: lane e of them the d 4 (e % 4) .. + 3 of key e / 4, and get d e of all four
+                const uint32_t e = lane & 15, sub = (lane >> 4) & 1;
+                const uint32_t piece = 4 * i + 2 * sub + e % 4 / 2;
+                const uint32_t ra = 16 * u + 4 * h + e / 4, rb = ra + 8;
+                const uint8_t *const base = sV + buf * kTileBytes + 8 * (e % 2);
+                const uint8_t *const pa = base + (ra * kPieces + (piece ^ swizzle_v<DIM>(ra))) * 16;
+                const uint8_t *const pb = base + (rb * kPieces + (piece ^ swizzle_v<DIM>(rb))) * 16;
+                struct {
+                    v4s a, b;
+                } w;
+                w.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)pa);
+                w.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)pb);
+                const V vv = __builtin_bit_cast(V, w);
+                o[i] = Op::mfma(vv, ph, o[i]);
+                if (kWide) {
+                    o[i] = Op::mfma(vv, pl, o[i]);
+                }
+            }
+        }
+        if (CT != PT_I8 && bad) {
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (sBad[32 * i + 8 * (j / 4) + 4 * h + j % 4] & seen) {
+                        o[i][j] = NAN;
+                    }
+                }
+            }
+        }
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    if (alone) {
+        if (!mine) {
+            return;
+        }
+        const float inv = l == 0.0f ? 0.0f : unit / l;
+        const size_t at = (size_t)row * a.ostride + (size_t)head * DIM + 4 * h;
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                store_out4<ACT>(a.out, at + 32 * i + 2 * j, o[i][j] * inv, o[i][j + 1] * inv, o[i][j + 2] * inv, o[i][j + 3] * inv);
+            }
+        }
+        return;
+    }
+    float *const part = part_at(a, x, kvh, share, shares, DIM);
+    const uint32_t pr = 32 * wave + c;
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            *(v4f *)(part + (size_t)pr * DIM + 32 * i + 2 * j + 4 * h) =
+                (v4f){o[i][j] * unit, o[i][j + 1] * unit, o[i][j + 2] * unit, o[i][j + 3] * unit};
+        }
+    }
+    if (h == 0) {
+        part[kRows * DIM + pr] = m;
+        part[kRows * DIM + kRows + pr] = l;
+    }
+}
+
+// Joins the shares of a tile's keys: a workgroup per eight rows of a tile, DIM / 4 lanes to a row
+template <int ACT, int DIM>
+__global__ __launch_bounds__(8 * DIM / 4) void paged_prompt_join_kernel(PagedAttentionArgs a, uint32_t shares)
+{
+    const uint32_t lane = threadIdx.x & 63, kvh = blockIdx.x % a.pool.kv_heads, x = blockIdx.x / a.pool.kv_heads;
+    const uint32_t group = a.heads / a.pool.kv_heads;
+    Tile tile;
+    if (!find_tile(a, group, x, lane, &tile)) {
+        return;
+    }
+    const PagedSeq seq = paged_seq(a.batch, tile.b);
+    const Reach all = reach_of(a, seq, tile.index, group);
+    const uint32_t per = tiles_per_share(all.tiles, shares);
+    if (per >= all.tiles) {
+        return;
+    }
+    const uint32_t count = (all.tiles + per - 1) / per;
+    const uint32_t pr = blockIdx.y * 8 + threadIdx.x / (DIM / 4), d = threadIdx.x % (DIM / 4) * 4;
+    const int64_t r = (int64_t)tile.index * kRows + pr, row = seq.first + r / group;
+    if (r >= seq.count * group || row < 0 || row >= (int64_t)a.batch.rows) {
+        return;
+    }
+    float top = kLow, sum = 0.0f;
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i = 0; i < count; ++i) {
+        const float *const p = part_at(a, x, kvh, i, shares, DIM);
+        const float m = p[kRows * DIM + pr], up = fmaxf(top, m);
+        const float f = __builtin_amdgcn_exp2f(top - up), e = __builtin_amdgcn_exp2f(m - up);
+        sum = sum * f + p[kRows * DIM + kRows + pr] * e;
+        v = v * f + *(const v4f *)(p + (size_t)pr * DIM + d) * e;
+        top = up;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    store_out4<ACT>(a.out, (size_t)row * a.ostride + (size_t)(kvh * group + r % group) * DIM + d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+}
+
+// row tiles that a launch may have, and how many workgroups share a tile's keys
+uint64_t most_tiles(const PagedBatch &b, uint32_t group)
+{
+    return (uint64_t)b.rows * group / kRows + b.batch;
+}
+
+uint32_t shares_of(const PagedPool &pool, const PagedBatch &b, uint32_t heads)
+{
+    const uint64_t grid = most_tiles(b, heads / pool.kv_heads) * pool.kv_heads;
+    const uint64_t keys = (((uint64_t)b.max_pages << pool.shift) + kKeys * kLeast - 1) / (kKeys * kLeast);
+    const uint64_t n = grid >= kSpread ? 1 : kSpread / grid;
+    return (uint32_t)(n < keys ? n : keys);
+}
+
+template <int ACT, int CT, int DIM>
+struct Prompt {
+    static hipError_t run(const PagedAttentionArgs &a, hipStream_t st)
+    {
+        const uint32_t shares = shares_of(a.pool, a.batch, a.heads);
+        const uint64_t tiles = most_tiles(a.batch, a.heads / a.pool.kv_heads);
+        constexpr uint32_t lds = prompt_lds<CT, DIM>();
+        static const hipError_t ready = hipFuncSetAttribute((const void *)paged_prompt_kernel<ACT, CT, DIM>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (ready != hipSuccess) {
+            return ready;
+        }
+        const uint64_t blocks = tiles * a.pool.kv_heads;
+        hipLaunchKernelGGL((paged_prompt_kernel<ACT, CT, DIM>), dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || shares == 1) {
+            return e;
+        }
+        hipLaunchKernelGGL((paged_prompt_join_kernel<ACT, DIM>), dim3((uint32_t)blocks, kRows / 8), dim3(8 * DIM / 4), 0, st, a, shares);
+        return hipGetLastError();
+    }
+};
+
+}  // namespace
+
+bool paged_prompt_fits(const PagedPool &pool, const PagedBatch &batch, uint32_t heads)
+{
+    const uint32_t group = heads / pool.kv_heads;
+    return (uint64_t)batch.rows * group <= 0x7fffffffull && most_tiles(batch, group) * pool.kv_heads <= 0x7fffffffull;
+}
+
+size_t paged_prompt_workspace(const PagedPool &pool, const PagedBatch &batch, uint32_t heads)
+{
+    const uint32_t shares = shares_of(pool, batch, heads);
+    const uint64_t parts = shares == 1 ? 0 : most_tiles(batch, heads / pool.kv_heads) * pool.kv_heads * shares;
+    return parts * kRows * (pool.dim + 2) * sizeof(float) + 256;
+}
+
+hipError_t launch_paged_prompt(const PagedAttentionArgs &a, hipStream_t st)
+{
+    return a.batch.rows && a.batch.batch ? paged_dispatch<Prompt>(a.act, a.pool.type, a.pool.dim, a, st) : hipSuccess;
+}
+
+}  // namespace bg
