@@ -20,6 +20,7 @@ namespace bg {
 namespace {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(1))) void *gptr_t;
 typedef __attribute__((address_space(3))) void *lptr_t;
@@ -29,8 +30,6 @@ constexpr uint32_t kSpread = 512;  // workgroups below which a tile's keys are s
 constexpr uint32_t kLeast = 4;     // fewest key tiles per share
 constexpr float kLow = -1.7e38f;
 constexpr float kSlack = 2.0f, kLift = 13.0f;
-
-__device__ __attribute__((aligned(16))) uint32_t g_zeros[4];  // what stands in for a key that nobody stored
 
 struct Tile {
     uint32_t b, index;
@@ -130,6 +129,12 @@ __device__ __forceinline__ uint32_t swizzle_v(uint32_t row)
     return DIM == 128 ? (row & 3) << 2 | ((row >> 2) & 3) : ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
 }
 
+// no instruction is moved across
+__device__ __forceinline__ void in_order()
+{
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 template <int CT>
 struct Product {
     typedef v8h V;
@@ -137,10 +142,15 @@ struct Product {
     {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
+    // l + both values of a pair
+    static __device__ __forceinline__ float add_pair(uint32_t w, float l)
+    {
+        typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), (v2h){(_Float16)1.0f, (_Float16)1.0f}, l, false);
+    }
     // two values rounded to nearest
     static __device__ __forceinline__ uint32_t pack(float a, float b)
     {
-        typedef float v2f __attribute__((ext_vector_type(2)));
         typedef _Float16 v2h __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2h));
     }
@@ -152,9 +162,13 @@ struct Product<PT_BF16> {
     {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ float add_pair(uint32_t w, float l)
+    {
+        typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, w), (v2b){(__bf16)1.0f, (__bf16)1.0f}, l, false);
+    }
     static __device__ __forceinline__ uint32_t pack(float a, float b)
     {
-        typedef float v2f __attribute__((ext_vector_type(2)));
         typedef __bf16 v2b __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2b));
     }
@@ -175,7 +189,7 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float a, float 
 template <int CT, int DIM>
 constexpr uint32_t prompt_lds()
 {
-    return 4 * kKeys * DIM * 2 + (CT == PT_I8 ? 4 * kKeys * 4 : DIM * 8);
+    return 4 * kKeys * DIM * 2 + (CT == PT_I8 ? 4 * kKeys * 4 + 2 * 8 + 2 * 4 : DIM * 8 + 4 * 4);
 }
 
 template <int ACT, int CT, int DIM>
@@ -188,9 +202,12 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     constexpr uint32_t kTileBytes = kKeys * DIM * 2, kRowBytes = DIM * (CT == PT_I8 ? 1 : 2), kPieces = DIM / 8;
     constexpr int kSteps = DIM / 16, kOut = DIM / 32, kLoads = kTileBytes / 16 / 256;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    uint8_t *const sK = smem, *const sV = smem + 2 * kTileBytes;                     // two buffers each
+    // two buffers, each a tile of keys and one of values
     float *const sStep = (float *)(smem + 4 * kTileBytes);                           // int8: [2][keys' 64, values' 64]
-    unsigned long long *const sBad = (unsigned long long *)(smem + 4 * kTileBytes);  // else: [DIM] keys whose value is not finite
+    unsigned long long *const sBad = (unsigned long long *)(smem + 4 * kTileBytes + (CT == PT_I8 ? 4 * kKeys * 4 : 0));
+    // ^ keys whose value is not finite: 16-bit caches [DIM]; int8 [2]
+    float *const sTop = (float *)(sBad + 2);                                         // int8: [2] the largest step of a tile
+    uint32_t *const sHit = (uint32_t *)(sBad + DIM);                                 // else: [4] whether a wave found such a value
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t c = lane & 31, h = lane >> 5;
@@ -267,53 +284,66 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     }
     float m = kLow, l = 0.0f, unit = CT == PT_I8 ? kFirstUnit : 1.0f;
 
-    // page of key k0 + lane; none: -1
-    auto page_of = [&](uint32_t k0) -> int32_t {
-        const uint32_t key = k0 + lane;
-        if (key >= all.hi) {
-            return -1;
+    // Page of key k0 + lane, none: -1. In two halves: the list is read a tile ahead of its use.
+    auto look_up = [&](uint32_t k0) -> int32_t { return table[min(k0 + lane, all.hi - 1) >> a.pool.shift]; };
+    auto page_of = [&](uint32_t k0, int32_t found) -> int32_t { return k0 + lane < all.hi && (uint32_t)found < a.pool.pages ? found : -1; };
+    // A wave's load n covers the rows from 64 (4n + wave) / kPieces on: kRowsAt of them. In pages of at least that many keys
+    // (and of eight at least, so that both head sizes go the same way) they lie side by side, and their address is the wave's.
+    // A key without a page is read from page 0: what it brings is masked, and taken out of the tile where it is not finite.
+    constexpr uint32_t kRowsAt = 64 / kPieces;
+    const bool scalar_pages = a.pool.shift >= 3;
+    const uint32_t in_row = lane / kPieces, piece = lane % kPieces;
+    auto offsets_of = [&](int32_t pages, uint32_t k0, size_t (&off)[kLoads]) {  // of this lane's rows, in bytes
+        const uint32_t mask = (1u << a.pool.shift) - 1;
+        if (scalar_pages) {
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) {
+                const uint32_t rowk = (n * 4 + wave) * kRowsAt;
+                const uint32_t page = (uint32_t)max(__builtin_amdgcn_readlane(pages, rowk), 0);
+                off[n] = ((((size_t)page * a.pool.kv_heads + kvh) << a.pool.shift) | ((k0 + rowk) & mask)) * kRowBytes + in_row * kRowBytes;
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) {
+                const uint32_t rowk = (n * 4 + wave) * kRowsAt + in_row;
+                const uint32_t page = (uint32_t)max(__shfl(pages, rowk, 64), 0);
+                off[n] = ((((size_t)page * a.pool.kv_heads + kvh) << a.pool.shift) | ((k0 + rowk) & mask)) * kRowBytes;
+            }
         }
-        const uint32_t p = (uint32_t)table[key >> a.pool.shift];
-        return p < a.pool.pages ? (int32_t)p : -1;
     };
-    auto slot_of = [&](int32_t page, uint32_t key) -> size_t {
-        return (((size_t)(uint32_t)page * a.pool.kv_heads + kvh) << a.pool.shift) | (key & ((1u << a.pool.shift) - 1));
-    };
-    // 16-bit caches: straight into buffer `buf`
-    auto fetch = [&](uint32_t k0, int32_t pages, uint32_t buf) {
+    // 16-bit caches: straight into a buffer
+    auto fetch = [&](uint32_t k0, int32_t pages, uint8_t *to) {
+        size_t off[kLoads];
+        offsets_of(pages, k0, off);
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const uint32_t at = (n * 4 + wave) * 64, rowk = (at + lane) / kPieces, piece = (at + lane) % kPieces;
-            const int32_t page = __shfl(pages, rowk, 64);
-            const size_t off = slot_of(page, k0 + rowk) * kRowBytes;
-            const uint8_t *kp = (const uint8_t *)a.pool.k + off + 16 * (piece ^ swizzle_k<DIM>(rowk));
-            const uint8_t *vp = (const uint8_t *)a.pool.v + off + 16 * (piece ^ swizzle_v<DIM>(rowk));
-            kp = page < 0 ? (const uint8_t *)g_zeros : kp;
-            vp = page < 0 ? (const uint8_t *)g_zeros : vp;
-            __builtin_amdgcn_global_load_lds((gptr_t)kp, (lptr_t)(sK + buf * kTileBytes + at * 16), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gptr_t)vp, (lptr_t)(sV + buf * kTileBytes + at * 16), 16, 0, 0);
+            const uint32_t at = (n * 4 + wave) * 64, rowk = (n * 4 + wave) * kRowsAt + in_row;
+            const uint8_t *kp = (const uint8_t *)a.pool.k + off[n] + 16 * (piece ^ swizzle_k<DIM>(rowk));
+            const uint8_t *vp = (const uint8_t *)a.pool.v + off[n] + 16 * (piece ^ swizzle_v<DIM>(rowk));
+            __builtin_amdgcn_global_load_lds((gptr_t)kp, (lptr_t)(to + at * 16), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr_t)vp, (lptr_t)(to + kTileBytes + at * 16), 16, 0, 0);
         }
     };
     // int8: eight values of a row per piece into registers, then as fp16 into the buffer
     v2u rk[CT == PT_I8 ? kLoads : 1], rv[CT == PT_I8 ? kLoads : 1];
     float rs = 0.0f;
     auto fetch8 = [&](uint32_t k0, int32_t pages) {
+        size_t off[kLoads];
+        offsets_of(pages, k0, off);
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const uint32_t at = (n * 4 + wave) * 64, rowk = (at + lane) / kPieces, piece = (at + lane) % kPieces;
-            const int32_t page = __shfl(pages, rowk, 64);
-            const size_t off = page < 0 ? 0 : slot_of(page, k0 + rowk) * kRowBytes;
-            rk[n] = *(const v2u *)((const uint8_t *)a.pool.k + off + 8 * piece);
-            rv[n] = *(const v2u *)((const uint8_t *)a.pool.v + off + 8 * piece);
+            rk[n] = *(const v2u *)((const uint8_t *)a.pool.k + off[n] + 8 * piece);
+            rv[n] = *(const v2u *)((const uint8_t *)a.pool.v + off[n] + 8 * piece);
         }
         if (wave < 2) {
-            rs = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[slot_of(pages, k0 + lane)];
+            const size_t slot = (((size_t)(uint32_t)max(pages, 0) * a.pool.kv_heads + kvh) << a.pool.shift) | ((k0 + lane) & ((1u << a.pool.shift) - 1));
+            rs = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[slot];
         }
     };
-    auto put8 = [&](uint32_t buf) {
+    auto put8 = [&](uint32_t buf, uint8_t *to) {
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const uint32_t at = (n * 4 + wave) * 64, rowk = (at + lane) / kPieces, piece = (at + lane) % kPieces;
+            const uint32_t rowk = (n * 4 + wave) * kRowsAt + in_row;
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
                 const v2u w = kv ? rv[n] : rk[n];
@@ -323,53 +353,100 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                     f[i] = bytes_to_f16(__builtin_amdgcn_perm(0, w[i / 2], i & 1 ? 0x0c030c02 : 0x0c010c00));
                 }
                 const uint32_t place = rowk * kPieces + (piece ^ (kv ? swizzle_v<DIM>(rowk) : swizzle_k<DIM>(rowk)));
-                *(v4u *)((kv ? sV : sK) + buf * kTileBytes + place * 16) = f;
+                *(v4u *)(to + kv * kTileBytes + place * 16) = f;
             }
         }
         if (wave < 2) {
-            sStep[buf * 2 * kKeys + wave * kKeys + lane] = __builtin_amdgcn_rcpf(rs);
+            float step = __builtin_amdgcn_rcpf(rs);
+            if (wave == 1) {
+                const bool fine = step - step == 0.0f;  // neither infinite nor NaN
+                const unsigned long long not_fine = __ballot(!fine);
+                step = fine ? step : 0.0f;
+                float most = step;
+#pragma unroll
+                for (int off = 32; off; off >>= 1) {
+                    most = fmaxf(most, __shfl_xor(most, off, 64));
+                }
+                if (lane == 0) {
+                    sBad[buf] = not_fine;
+                    sTop[buf] = most;
+                }
+            }
+            sStep[buf * 2 * kKeys + wave * kKeys + lane] = step;
         }
     };
 
-    int32_t pages = t0 < t1 ? page_of(all.lo + t0 * kKeys) : -1, next = t0 + 1 < t1 ? page_of(all.lo + (t0 + 1) * kKeys) : -1;
-    if (t0 < t1) {
-        if (CT == PT_I8) {
-            fetch8(all.lo + t0 * kKeys, pages);
-        } else {
-            fetch(all.lo + t0 * kKeys, pages, 0);
+    // where this lane reads in a tile: K pieces of row c, and for V (16 lanes read four keys of 16 d, lane e of them the d
+    // 4 (e % 4) .. + 3 of key e / 4, and get d e of all four)
+    uint32_t at_k[kSteps], at_v[kOut][2];
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+        at_k[st] = (c * kPieces + ((2 * st + h) ^ swizzle_k<DIM>(c))) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+        const uint32_t e = lane & 15, sub = (lane >> 4) & 1, from = 4 * i + 2 * sub + e % 4 / 2;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const uint32_t rowk = 4 * h + e / 4 + 8 * w;
+            at_v[i][w] = (rowk * kPieces + (from ^ swizzle_v<DIM>(rowk))) * 16 + 8 * (e % 2);
         }
     }
-    for (uint32_t t = t0; t < t1; ++t) {
-        const uint32_t k0 = all.lo + t * kKeys, buf = (t - t0) & 1;
+
+    int32_t pages = -1, next = -1;
+    if (t0 < t1) {
+        const uint32_t k0 = all.lo + t0 * kKeys;
+        pages = page_of(k0, look_up(k0));
+        next = look_up(k0 + kKeys);
+        if (CT == PT_I8) {
+            fetch8(k0, pages);
+        } else {
+            fetch(k0, pages, smem);
+        }
+    }
+    // One tile: `now` holds it, `ahead` is where the next one goes. (The compiler has to know that the two are apart, else it waits
+    // for the next tile's arrival before it reads this one.)
+    auto step_over = [&](uint32_t t, uint32_t buf, uint8_t *__restrict now, uint8_t *__restrict ahead) {
+        const uint32_t k0 = all.lo + t * kKeys;
         const unsigned long long stored = __ballot(pages >= 0);
         if (CT == PT_I8) {
-            put8(buf);
+            put8(buf, now);
         }
-        __syncthreads();  // the tile is there; everyone is done with the other buffer
-        pages = next;
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile is there
+        __syncthreads();                     // everyone's; and everyone is done with the other buffer
+        pages = page_of(k0 + kKeys, next);
+        next = look_up(k0 + 2 * kKeys);
         if (t + 1 < t1) {
             if (CT == PT_I8) {
                 fetch8(k0 + kKeys, pages);
             } else {
-                fetch(k0 + kKeys, pages, buf ^ 1);
+                fetch(k0 + kKeys, pages, ahead);
             }
-            next = t + 2 < t1 ? page_of(k0 + 2 * kKeys) : -1;
         }
         // does every row of the workgroup see every key of the tile?
         const uint32_t last_lo = paged_span(all.last, a.window, all.hi).lo;
         const bool whole = stored == ~0ull && (int64_t)k0 + kKeys - 1 <= all.first && k0 >= last_lo;
+        // A value that is infinite or NaN must not reach the rows that do not see its key (0 * inf): it is taken out of the tile, and
+        // makes the rows that do see it NaN. An int8 cache has it in the slot's step, put8 has taken that out.
+        unsigned long long bad_keys = 0;
         bool bad = false;
-        if (CT != PT_I8 && !whole) {
-            // a value that is infinite or NaN must not reach the rows that do not see its key (0 * inf): it is taken out of the tile
-            // and put into the rows that do
+        if (CT == PT_I8) {
+            bad_keys = sBad[buf];
+            bad = bad_keys != 0;
+        } else if (!whole) {
             constexpr uint32_t kExp = CT == PT_BF16 ? 0x7f80u : 0x7c00u;
-            uint8_t *const base = sV + buf * kTileBytes;
+            uint8_t *const base = now + kTileBytes;
             bool hit = false;
             for (uint32_t at = tid; at < kTileBytes / 4; at += 256) {
                 const uint32_t w = *(const uint32_t *)(base + at * 4);
                 hit |= (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
             }
-            bad = __syncthreads_or(hit);
+            hit = __any(hit);
+            if (lane == 0) {
+                sHit[wave] = hit;
+            }
+            __syncthreads();
+            bad = (sHit[0] | sHit[1] | sHit[2] | sHit[3]) != 0;
             if (bad) {
                 for (uint32_t d = tid; d < DIM; d += 256) {
                     sBad[d] = 0;
@@ -387,71 +464,97 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             }
         }
         if (!__any(span.hi > k0 && span.lo < k0 + kKeys)) {
-            continue;  // nothing for this wave
+            return;  // nothing for this wave
         }
-        // scores
+        // Scores. The order is written out (the compiler would wait for every read right behind it): eight reads ahead of the
+        // products that use them.
         v16f s[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int j = 0; j < 16; ++j) {
+            s[0][j] = s[1][j] = 0.0f;
+        }
+        V kf[4][2];
+        auto keys = [&](int st) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                s[i][j] = 0.0f;
+            for (int i = 0; i < 2; ++i) {
+                kf[st & 3][i] = *(const V *)(now + i * 32 * DIM * 2 + at_k[st]);
             }
+        };
 #pragma unroll
-            for (int st = 0; st < kSteps; ++st) {
-                const uint32_t rowk = 32 * i + c, place = rowk * kPieces + ((2 * st + h) ^ swizzle_k<DIM>(rowk));
-                const V kv = *(const V *)(sK + buf * kTileBytes + place * 16);
-                s[i] = Op::mfma(kv, qh[st], s[i]);
+        for (int st = 0; st < 4; ++st) {
+            keys(st);
+        }
+        in_order();
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                s[i] = Op::mfma(kf[st & 3][i], qh[st], s[i]);
                 if (kWide) {
-                    s[i] = Op::mfma(kv, ql[st], s[i]);
+                    s[i] = Op::mfma(kf[st & 3][i], ql[st], s[i]);
                 }
             }
+            in_order();
+            if (st + 4 < kSteps) {
+                keys(st + 4);
+                in_order();
+            }
         }
-        float step[2][16], wide = 0.0f;
+        V vv[2][kOut], ph[2], pl[2];
+        Words<4> pw[2];
+        auto value = [&](int u, int i) {
+            const uint8_t *const base = now + kTileBytes + u * 16 * DIM * 2;
+            struct {
+                v4s a, b;
+            } w;
+            w.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(base + at_v[i][0]));
+            w.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(base + at_v[i][1]));
+            vv[u & 1][i] = __builtin_bit_cast(V, w);
+        };
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) {
+            value(0, i);
+        }
+        in_order();
         if (CT == PT_I8) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                    const uint32_t key = 32 * i + 2 * j + 4 * h;
-                    const v4f ks = *(const v4f *)(sStep + buf * 2 * kKeys + key), vs = *(const v4f *)(sStep + buf * 2 * kKeys + kKeys + key);
+                    const v4f ks = *(const v4f *)(sStep + buf * 2 * kKeys + 32 * i + 2 * j + 4 * h);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         s[i][j + e] *= ks[e];
-                        step[i][j + e] = vs[e];
                     }
                 }
             }
         }
         unsigned long long seen = ~0ull;
+        float wide = CT == PT_I8 ? sTop[buf] : 0.0f;  // int8: the largest step among the keys that this row sees
         if (!whole) {
             const uint32_t from = span.lo > k0 ? span.lo - k0 : 0, upto = span.hi > k0 ? span.hi - k0 : 0;  // keys of the tile this row sees
             seen = from >= kKeys || upto <= from ? 0 : (upto >= kKeys ? ~0ull : (1ull << upto) - 1) & (~0ull << from);
             seen &= stored;
+            if (CT == PT_I8) {
+                wide = 0.0f;
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t half = (uint32_t)(seen >> (32 * i)) >> (4 * h);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    if (!(half >> (8 * (j / 4) + j % 4) & 1)) {
-                        s[i][j] = -INFINITY;
-                        if (CT == PT_I8) {
-                            step[i][j] = 0.0f;
-                        }
+                    const bool sees = half >> (8 * (j / 4) + j % 4) & 1;
+                    s[i][j] = sees ? s[i][j] : -INFINITY;
+                    if (CT == PT_I8) {
+                        wide = fmaxf(wide, sees ? sStep[buf * 2 * kKeys + kKeys + 32 * i + 8 * (j / 4) + 4 * h + j % 4] : 0.0f);
                     }
                 }
             }
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                top = fmaxf(top, s[i][j]);
-                if (CT == PT_I8) {
-                    wide = fmaxf(wide, step[i][j]);
-                }
-            }
+        for (int j = 0; j < 16; ++j) {
+            top = fmaxf(top, fmaxf(s[0][j], s[1][j]));
         }
         top *= xscale;
         if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {
@@ -462,12 +565,8 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             m = up;
             if (CT == PT_I8) {
                 const float was = unit;
-                wide = fmaxf(wide, unit);
-#pragma unroll
-                for (int off = 32; off; off >>= 1) {
-                    wide = fmaxf(wide, __shfl_xor(wide, off, 64));
-                }
-                unit = power_above(wide);
+                wide = fmaxf(wide, __shfl_xor(wide, 32, 64));
+                unit = power_above(fmaxf(wide, unit));
                 corr *= was * __builtin_amdgcn_rcpf(unit);
             }
 #pragma unroll
@@ -475,69 +574,83 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 o[i] = o[i] * corr;
             }
         }
+        // Weights times values, 16 keys a step: behind every product stand the next step's reads and a share of its weights
         const float shift = kLift - m, per_unit = __builtin_amdgcn_rcpf(unit);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], xscale, shift));
-                l += p;
-                if (CT == PT_I8) {
-                    p *= step[i][j] * per_unit;
-                }
-                s[i][j] = p;
+        float p[8];
+        auto weight = [&](int u, int j) {  // j and j + 1
+            v2f vs;
+            if (CT == PT_I8) {
+                vs = *(const v2f *)(sStep + buf * 2 * kKeys + kKeys + 16 * u + 8 * (j / 4) + 4 * h + j % 4);
             }
+#pragma unroll
+            for (int e = j; e < j + 2; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u % 2) + e], xscale, shift));
+                if (kWide || CT == PT_I8) {
+                    l += p[e];
+                }
+                if (CT == PT_I8) {
+                    p[e] *= vs[e - j] * per_unit;
+                }
+            }
+            if (!kWide) {
+                const uint32_t w = Op::pack(p[j], p[j + 1]);
+                pw[u & 1].w[j / 2] = w;
+                if (CT != PT_I8) {
+                    l = Op::add_pair(w, l);
+                }
+            }
+        };
+        auto ready = [&](int u) {
+            if (kWide) {
+                Operand<CT>::split(p, 1.0f, &ph[u & 1], &pl[u & 1]);
+            } else {
+                ph[u & 1] = __builtin_bit_cast(V, pw[u & 1]);
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            weight(0, j);
         }
-        // weights times values, 16 keys a step
+        ready(0);
+        in_order();
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            V ph, pl;
-            float p[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                p[j] = s[u / 2][8 * (u % 2) + j];
-            }
-            if (kWide) {
-                Operand<CT>::split(p, 1.0f, &ph, &pl);
-            } else {
-                Words<4> w;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    w.w[j] = Op::pack(p[2 * j], p[2 * j + 1]);
-                }
-                ph = __builtin_bit_cast(V, w);
-            }
 #pragma unroll
             for (int i = 0; i < kOut; ++i) {
-                // 16 lanes read four keys of 16 d: lane e of them the d 4 (e % 4) .. + 3 of key e / 4, and get d e of all four
-                const uint32_t e = lane & 15, sub = (lane >> 4) & 1;
-                const uint32_t piece = 4 * i + 2 * sub + e % 4 / 2;
-                const uint32_t ra = 16 * u + 4 * h + e / 4, rb = ra + 8;
-                const uint8_t *const base = sV + buf * kTileBytes + 8 * (e % 2);
-                const uint8_t *const pa = base + (ra * kPieces + (piece ^ swizzle_v<DIM>(ra))) * 16;
-                const uint8_t *const pb = base + (rb * kPieces + (piece ^ swizzle_v<DIM>(rb))) * 16;
-                struct {
-                    v4s a, b;
-                } w;
-                w.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)pa);
-                w.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)pb);
-                const V vv = __builtin_bit_cast(V, w);
-                o[i] = Op::mfma(vv, ph, o[i]);
+                o[i] = Op::mfma(vv[u & 1][i], ph[u & 1], o[i]);
                 if (kWide) {
-                    o[i] = Op::mfma(vv, pl, o[i]);
+                    o[i] = Op::mfma(vv[u & 1][i], pl[u & 1], o[i]);
+                }
+                in_order();
+                if (u < 3) {
+                    value(u + 1, i);
+#pragma unroll
+                    for (int j = i * (8 / kOut); j < (i + 1) * (8 / kOut); j += 2) {
+                        weight(u + 1, j);
+                    }
+                    if (i == kOut - 1) {
+                        ready(u + 1);
+                    }
+                    in_order();
                 }
             }
         }
-        if (CT != PT_I8 && bad) {
+        if (bad) {
 #pragma unroll
             for (int i = 0; i < kOut; ++i) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    if (sBad[32 * i + 8 * (j / 4) + 4 * h + j % 4] & seen) {
+                    if ((CT == PT_I8 ? bad_keys : sBad[32 * i + 8 * (j / 4) + 4 * h + j % 4]) & seen) {
                         o[i][j] = NAN;
                     }
                 }
             }
+        }
+    };
+    for (uint32_t t = t0; t < t1; t += 2) {
+        step_over(t, 0, smem, smem + 2 * kTileBytes);
+        if (t + 1 < t1) {
+            step_over(t + 1, 1, smem + 2 * kTileBytes, smem);
         }
     }
 
