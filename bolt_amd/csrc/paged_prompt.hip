@@ -192,7 +192,8 @@ constexpr uint32_t prompt_lds()
     return 4 * kKeys * DIM * 2 + (CT == PT_I8 ? 4 * kKeys * 4 + 2 * 8 + 2 * 4 : DIM * 8 + 4 * 4);
 }
 
-template <int ACT, int CT, int DIM>
+// PAGE8: pages of eight keys and more
+template <int ACT, int CT, int DIM, bool PAGE8>
 __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs a, uint32_t shares)
 {
     typedef Product<CT> Op;
@@ -234,6 +235,8 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     const bool mine = r < seq.count * group && row >= 0 && row < (int64_t)a.batch.rows;
     const uint32_t head = kvh * group + (uint32_t)(r % group);
     const PagedSpan span = paged_span(mine ? pos : -1, a.window, all.hi);
+
+    const uint32_t all_hi = paged_span(all.first, 0, all.hi).hi, all_lo = paged_span(all.last, a.window, all.hi).lo;  // seen by every row
 
     V qh[kSteps], ql[kWide ? kSteps : 1];
     float xscale = a.scale2;
@@ -287,57 +290,56 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     // Page of key k0 + lane, none: -1. In two halves: the list is read a tile ahead of its use.
     auto look_up = [&](uint32_t k0) -> int32_t { return table[min(k0 + lane, all.hi - 1) >> a.pool.shift]; };
     auto page_of = [&](uint32_t k0, int32_t found) -> int32_t { return k0 + lane < all.hi && (uint32_t)found < a.pool.pages ? found : -1; };
-    // A wave's load n covers the rows from 64 (4n + wave) / kPieces on: kRowsAt of them. In pages of at least that many keys
-    // (and of eight at least, so that both head sizes go the same way) they lie side by side, and their address is the wave's.
-    // A key without a page is read from page 0: what it brings is masked, and taken out of the tile where it is not finite.
+    // A wave's load n covers kRowsAt rows of the tile, from row (4n + wave) kRowsAt on. In pages of eight keys and more they lie side
+    // by side, so that their address is the wave's and what a lane adds to it is the same for every load. A key without a page
+    // is read from page 0: what it brings is masked, and taken out of the tile where it is not finite.
     constexpr uint32_t kRowsAt = 64 / kPieces;
-    const bool scalar_pages = a.pool.shift >= 3;
     const uint32_t in_row = lane / kPieces, piece = lane % kPieces;
-    auto offsets_of = [&](int32_t pages, uint32_t k0, size_t (&off)[kLoads]) {  // of this lane's rows, in bytes
-        const uint32_t mask = (1u << a.pool.shift) - 1;
-        if (scalar_pages) {
-#pragma unroll
-            for (int n = 0; n < kLoads; ++n) {
-                const uint32_t rowk = (n * 4 + wave) * kRowsAt;
-                const uint32_t page = (uint32_t)max(__builtin_amdgcn_readlane(pages, rowk), 0);
-                off[n] = ((((size_t)page * a.pool.kv_heads + kvh) << a.pool.shift) | ((k0 + rowk) & mask)) * kRowBytes + in_row * kRowBytes;
-            }
-        } else {
-#pragma unroll
-            for (int n = 0; n < kLoads; ++n) {
-                const uint32_t rowk = (n * 4 + wave) * kRowsAt + in_row;
-                const uint32_t page = (uint32_t)max(__shfl(pages, rowk, 64), 0);
-                off[n] = ((((size_t)page * a.pool.kv_heads + kvh) << a.pool.shift) | ((k0 + rowk) & mask)) * kRowBytes;
-            }
+    // byte offset of key k0 + lane in the pool
+    auto offset_of = [&](uint32_t k0, int32_t page) -> size_t {
+        const size_t first = (size_t)(uint32_t)max(page, 0) * a.pool.kv_heads + kvh;
+        return ((first << a.pool.shift) | ((k0 + lane) & ((1u << a.pool.shift) - 1))) * kRowBytes;
+    };
+    // of load n: the wave's part in *base, the lane's as the answer
+    auto row_at = [&](size_t offset, int n, size_t *base) -> uint32_t {
+        if (PAGE8) {
+            const uint32_t from = n * 4 * kRowsAt + wave * kRowsAt;
+            *base = (size_t)__builtin_amdgcn_readlane((uint32_t)(offset >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)offset, from);
+            return in_row * kRowBytes;
         }
+        const uint32_t from = n * 4 * kRowsAt + wave * kRowsAt + in_row;
+        *base = (size_t)(uint32_t)__shfl((uint32_t)(offset >> 32), from, 64) << 32 | (uint32_t)__shfl((uint32_t)offset, from, 64);
+        return 0;
     };
     // 16-bit caches: straight into a buffer
+    const uint32_t first_row = wave * kRowsAt + in_row;  // of load 0; the others' rows are 4 kRowsAt apart, which changes no permutation
     auto fetch = [&](uint32_t k0, int32_t pages, uint8_t *to) {
-        size_t off[kLoads];
-        offsets_of(pages, k0, off);
+        const size_t offset = offset_of(k0, pages);
+        const uint32_t pk = 16 * (piece ^ swizzle_k<DIM>(first_row)), pv = 16 * (piece ^ swizzle_v<DIM>(first_row));
+        uint8_t *const mine_to = to + wave * 1024;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const uint32_t at = (n * 4 + wave) * 64, rowk = (n * 4 + wave) * kRowsAt + in_row;
-            const uint8_t *kp = (const uint8_t *)a.pool.k + off[n] + 16 * (piece ^ swizzle_k<DIM>(rowk));
-            const uint8_t *vp = (const uint8_t *)a.pool.v + off[n] + 16 * (piece ^ swizzle_v<DIM>(rowk));
-            __builtin_amdgcn_global_load_lds((gptr_t)kp, (lptr_t)(to + at * 16), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gptr_t)vp, (lptr_t)(to + kTileBytes + at * 16), 16, 0, 0);
+            size_t base;
+            const uint32_t add = row_at(offset, n, &base);
+            const uint8_t *const kp = (const uint8_t *)a.pool.k + base, *const vp = (const uint8_t *)a.pool.v + base;
+            __builtin_amdgcn_global_load_lds((gptr_t)(kp + (add + pk)), (lptr_t)(mine_to + n * 4096), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr_t)(vp + (add + pv)), (lptr_t)(mine_to + kTileBytes + n * 4096), 16, 0, 0);
         }
     };
     // int8: eight values of a row per piece into registers, then as fp16 into the buffer
     v2u rk[CT == PT_I8 ? kLoads : 1], rv[CT == PT_I8 ? kLoads : 1];
     float rs = 0.0f;
     auto fetch8 = [&](uint32_t k0, int32_t pages) {
-        size_t off[kLoads];
-        offsets_of(pages, k0, off);
+        const size_t offset = offset_of(k0, pages);
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            rk[n] = *(const v2u *)((const uint8_t *)a.pool.k + off[n] + 8 * piece);
-            rv[n] = *(const v2u *)((const uint8_t *)a.pool.v + off[n] + 8 * piece);
+            size_t base;
+            const uint32_t add = row_at(offset, n, &base) + 8 * piece;
+            rk[n] = *(const v2u *)((const uint8_t *)a.pool.k + base + add);
+            rv[n] = *(const v2u *)((const uint8_t *)a.pool.v + base + add);
         }
         if (wave < 2) {
-            const size_t slot = (((size_t)(uint32_t)max(pages, 0) * a.pool.kv_heads + kvh) << a.pool.shift) | ((k0 + lane) & ((1u << a.pool.shift) - 1));
-            rs = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[slot];
+            rs = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[offset / kRowBytes];
         }
     };
     auto put8 = [&](uint32_t buf, uint8_t *to) {
@@ -424,8 +426,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             }
         }
         // does every row of the workgroup see every key of the tile?
-        const uint32_t last_lo = paged_span(all.last, a.window, all.hi).lo;
-        const bool whole = stored == ~0ull && (int64_t)k0 + kKeys - 1 <= all.first && k0 >= last_lo;
+        const bool whole = stored == ~0ull && k0 + kKeys <= all_hi && k0 >= all_lo;
         // A value that is infinite or NaN must not reach the rows that do not see its key (0 * inf): it is taken out of the tile, and
         // makes the rows that do see it NaN. An int8 cache has it in the slot's step, put8 has taken that out.
         unsigned long long bad_keys = 0;
@@ -743,12 +744,19 @@ struct Prompt {
         const uint32_t shares = shares_of(a.pool, a.batch, a.heads);
         const uint64_t tiles = most_tiles(a.batch, a.heads / a.pool.kv_heads);
         constexpr uint32_t lds = prompt_lds<CT, DIM>();
-        static const hipError_t ready = hipFuncSetAttribute((const void *)paged_prompt_kernel<ACT, CT, DIM>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        static const hipError_t ready = [] {
+            const hipError_t e = hipFuncSetAttribute((const void *)paged_prompt_kernel<ACT, CT, DIM, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            return e != hipSuccess ? e : hipFuncSetAttribute((const void *)paged_prompt_kernel<ACT, CT, DIM, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        }();
         if (ready != hipSuccess) {
             return ready;
         }
         const uint64_t blocks = tiles * a.pool.kv_heads;
-        hipLaunchKernelGGL((paged_prompt_kernel<ACT, CT, DIM>), dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
+        if (a.pool.shift >= 3) {
+            hipLaunchKernelGGL((paged_prompt_kernel<ACT, CT, DIM, true>), dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
+        } else {
+            hipLaunchKernelGGL((paged_prompt_kernel<ACT, CT, DIM, false>), dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
+        }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || shares == 1) {
             return e;
