@@ -166,7 +166,13 @@ struct OperandF16 {
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
-    // x * up as the sum of two fp16 parts (what is left is below 2^-21 of it); fp16 and bf16 values are all in the first
+    // a and b as sums of two fp16 parts (what is left is below 2^-21 of them); fp16 and bf16 values are all in the first
+    static __device__ __forceinline__ void split2(float a, float b, uint32_t *hi, uint32_t *lo)
+    {
+        const auto r = __builtin_amdgcn_cvt_pkrtz(a, b);
+        *hi = __builtin_bit_cast(uint32_t, r);
+        *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)r[0], b - (float)r[1]));
+    }
     static __device__ __forceinline__ void split(const float *x, float up, V *hi, V *lo)
     {
         union {
@@ -175,10 +181,7 @@ struct OperandF16 {
         } h, l;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
-            const auto r = __builtin_amdgcn_cvt_pkrtz(a, b);
-            h.w[i] = __builtin_bit_cast(uint32_t, r);
-            l.w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)r[0], b - (float)r[1]));
+            split2(x[2 * i] * up, x[2 * i + 1] * up, &h.w[i], &l.w[i]);
         }
         *hi = h.v;
         *lo = l.v;
@@ -191,6 +194,13 @@ struct OperandBf16 {
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ void split2(float x, float y, uint32_t *hi, uint32_t *lo)  // the upper halves are the truncated values
+    {
+        const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+        *hi = __builtin_amdgcn_perm(b, a, 0x07060302);
+        const float ra = x - __uint_as_float(a & 0xffff0000u), rb = y - __uint_as_float(b & 0xffff0000u);
+        *lo = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302);
+    }
     static __device__ __forceinline__ void split(const float *x, float up, V *hi, V *lo)
     {
         union {
@@ -199,11 +209,8 @@ struct OperandBf16 {
         } h, l;
         (void)up;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // the upper halves are the truncated values
-            const uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
-            h.w[i] = __builtin_amdgcn_perm(b, a, 0x07060302);
-            const float ra = x[2 * i] - __uint_as_float(a & 0xffff0000u), rb = x[2 * i + 1] - __uint_as_float(b & 0xffff0000u);
-            l.w[i] = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302);
+        for (int i = 0; i < 4; ++i) {
+            split2(x[2 * i], x[2 * i + 1], &h.w[i], &l.w[i]);
         }
         *hi = h.v;
         *lo = l.v;

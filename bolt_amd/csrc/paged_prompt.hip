@@ -24,6 +24,7 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(1))) void *gptr_t;
 typedef __attribute__((address_space(3))) void *lptr_t;
+typedef __attribute__((address_space(3))) uint8_t *lds_t;
 
 constexpr uint32_t kRows = 128, kKeys = 64;
 constexpr uint32_t kSpread = 512;  // workgroups below which a tile's keys are shared out
@@ -135,6 +136,12 @@ __device__ __forceinline__ void in_order()
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// One instruction; a NaN wins, and makes its row's weights NaN anyway (fmaxf has the operands quieted first, one more each)
+__device__ __forceinline__ float max_of(float a, float b, float c)
+{
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 template <int CT>
 struct Product {
     typedef v8h V;
@@ -189,7 +196,7 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float a, float 
 template <int CT, int DIM>
 constexpr uint32_t prompt_lds()
 {
-    return 4 * kKeys * DIM * 2 + (CT == PT_I8 ? 4 * kKeys * 4 + 2 * 8 + 2 * 4 : DIM * 8 + 4 * 4);
+    return 4 * kKeys * DIM * 2 + (CT == PT_I8 ? 4 * kKeys * 4 + 2 * 8 + 2 * 4 : DIM * 16 + 4 * 4 + 4);
 }
 
 // PAGE8: pages of eight keys and more
@@ -202,13 +209,15 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     constexpr bool kShiftQ = kWide || (ACT == PT_BF16 && CT == PT_I8);
     constexpr uint32_t kTileBytes = kKeys * DIM * 2, kRowBytes = DIM * (CT == PT_I8 ? 1 : 2), kPieces = DIM / 8;
     constexpr int kSteps = DIM / 16, kOut = DIM / 32, kLoads = kTileBytes / 16 / 256;
+    // LDS: two buffers, each a tile of keys and one of values; behind them
+    //   int8:  [2][keys' 64, values' 64] steps, [2] keys whose step is not finite, [2] the largest step of a tile
+    //   else:  [DIM][128 rows as bits] rows that see a value which is not finite, [4] whether a wave found one, whether there is any
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    // two buffers, each a tile of keys and one of values
-    float *const sStep = (float *)(smem + 4 * kTileBytes);                           // int8: [2][keys' 64, values' 64]
-    unsigned long long *const sBad = (unsigned long long *)(smem + 4 * kTileBytes + (CT == PT_I8 ? 4 * kKeys * 4 : 0));
-    // ^ keys whose value is not finite: 16-bit caches [DIM]; int8 [2]
-    float *const sTop = (float *)(sBad + 2);                                         // int8: [2] the largest step of a tile
-    uint32_t *const sHit = (uint32_t *)(sBad + DIM);                                 // else: [4] whether a wave found such a value
+    lds_t const sTiles = (lds_t)0;  // smem's own address: the kernel has no other LDS. As a constant it goes into the reads' offsets.
+    float *const sStep = (float *)(smem + 4 * kTileBytes);
+    unsigned long long *const sBad = (unsigned long long *)(sStep + 4 * kKeys);
+    float *const sTop = (float *)(sBad + 2);
+    uint32_t *const sPoison = (uint32_t *)(smem + 4 * kTileBytes), *const sHit = sPoison + 4 * DIM, *const sAny = sHit + 4;
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t c = lane & 31, h = lane >> 5;
@@ -220,7 +229,8 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     }
     const uint32_t b = __builtin_amdgcn_readfirstlane(tile.b);
     const PagedSeq seq = paged_seq(a.batch, b);
-    const Reach all = reach_of(a, seq, __builtin_amdgcn_readfirstlane(tile.index), group);
+    const uint32_t tile_index = __builtin_amdgcn_readfirstlane(tile.index);
+    const Reach all = reach_of(a, seq, tile_index, group);
     const uint32_t per = tiles_per_share(all.tiles, shares);
     const uint32_t t0 = share * per, t1 = min(t0 + per, all.tiles);
     if (share && t0 >= all.tiles) {
@@ -230,7 +240,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
 
     // this lane's row
-    const int64_t r = (int64_t)tile.index * kRows + 32 * wave + c, token = r / group;
+    const int64_t r = (int64_t)tile_index * kRows + 32 * wave + c, token = r / group;
     const int64_t row = seq.first + token, pos = seq.pos + token;
     const bool mine = r < seq.count * group && row >= 0 && row < (int64_t)a.batch.rows;
     const uint32_t head = kvh * group + (uint32_t)(r % group);
@@ -285,6 +295,12 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             o[t][i] = 0.0f;
         }
     }
+    if (CT != PT_I8) {  // (visible to all behind the first tile's barrier)
+        for (uint32_t at = tid; at < 4 * DIM + 5; at += 256) {
+            sPoison[at] = 0;
+        }
+    }
+    bool poisoned = false;  // int8: this row sees a slot whose step is not finite
     float m = kLow, l = 0.0f, unit = CT == PT_I8 ? kFirstUnit : 1.0f;
 
     // Page of key k0 + lane, none: -1. In two halves: the list is read a tile ahead of its use.
@@ -313,10 +329,10 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     };
     // 16-bit caches: straight into a buffer
     const uint32_t first_row = wave * kRowsAt + in_row;  // of load 0; the others' rows are 4 kRowsAt apart, which changes no permutation
-    auto fetch = [&](uint32_t k0, int32_t pages, uint8_t *to) {
+    auto fetch = [&](uint32_t k0, int32_t pages, lds_t to) {
         const size_t offset = offset_of(k0, pages);
         const uint32_t pk = 16 * (piece ^ swizzle_k<DIM>(first_row)), pv = 16 * (piece ^ swizzle_v<DIM>(first_row));
-        uint8_t *const mine_to = to + wave * 1024;
+        lds_t const mine_to = to + wave * 1024;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
             size_t base;
@@ -342,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             rs = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[offset / kRowBytes];
         }
     };
-    auto put8 = [&](uint32_t buf, uint8_t *to) {
+    auto put8 = [&](uint32_t buf, lds_t to) {
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
             const uint32_t rowk = (n * 4 + wave) * kRowsAt + in_row;
@@ -355,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                     f[i] = bytes_to_f16(__builtin_amdgcn_perm(0, w[i / 2], i & 1 ? 0x0c030c02 : 0x0c010c00));
                 }
                 const uint32_t place = rowk * kPieces + (piece ^ (kv ? swizzle_v<DIM>(rowk) : swizzle_k<DIM>(rowk)));
-                *(v4u *)(to + kv * kTileBytes + place * 16) = f;
+                *(__attribute__((address_space(3))) v4u *)(to + kv * kTileBytes + place * 16) = f;
             }
         }
         if (wave < 2) {
@@ -403,12 +419,13 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         if (CT == PT_I8) {
             fetch8(k0, pages);
         } else {
-            fetch(k0, pages, smem);
+            fetch(k0, pages, sTiles);
         }
     }
     // One tile: `now` holds it, `ahead` is where the next one goes. (The compiler has to know that the two are apart, else it waits
     // for the next tile's arrival before it reads this one.)
-    auto step_over = [&](uint32_t t, uint32_t buf, uint8_t *__restrict now, uint8_t *__restrict ahead) {
+    auto step_over = [&](uint32_t t, uint32_t buf, __attribute__((address_space(3))) uint8_t *__restrict now,
+                         __attribute__((address_space(3))) uint8_t *__restrict ahead) {
         const uint32_t k0 = all.lo + t * kKeys;
         const unsigned long long stored = __ballot(pages >= 0);
         if (CT == PT_I8) {
@@ -428,18 +445,13 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         // does every row of the workgroup see every key of the tile?
         const bool whole = stored == ~0ull && k0 + kKeys <= all_hi && k0 >= all_lo;
         // A value that is infinite or NaN must not reach the rows that do not see its key (0 * inf): it is taken out of the tile, and
-        // makes the rows that do see it NaN. An int8 cache has it in the slot's step, put8 has taken that out.
-        unsigned long long bad_keys = 0;
-        bool bad = false;
-        if (CT == PT_I8) {
-            bad_keys = sBad[buf];
-            bad = bad_keys != 0;
-        } else if (!whole) {
+        // the rows that do see it become NaN in the end. An int8 cache has it in the slot's step, which put8 has taken out.
+        if (CT != PT_I8 && !whole) {
             constexpr uint32_t kExp = CT == PT_BF16 ? 0x7f80u : 0x7c00u;
-            uint8_t *const base = now + kTileBytes;
+            lds_t const base = now + kTileBytes;
             bool hit = false;
             for (uint32_t at = tid; at < kTileBytes / 4; at += 256) {
-                const uint32_t w = *(const uint32_t *)(base + at * 4);
+                const uint32_t w = *(const __attribute__((address_space(3))) uint32_t *)(base + at * 4);
                 hit |= (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
             }
             hit = __any(hit);
@@ -447,18 +459,25 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 sHit[wave] = hit;
             }
             __syncthreads();
-            bad = (sHit[0] | sHit[1] | sHit[2] | sHit[3]) != 0;
-            if (bad) {
-                for (uint32_t d = tid; d < DIM; d += 256) {
-                    sBad[d] = 0;
-                }
-                __syncthreads();
+            if (sHit[0] | sHit[1] | sHit[2] | sHit[3]) {
                 for (uint32_t at = tid; at < kKeys * DIM; at += 256) {
                     const uint32_t rowk = at / DIM, d = at % DIM;
-                    uint16_t *const p = (uint16_t *)(base + (rowk * kPieces + (d / 8 ^ swizzle_v<DIM>(rowk))) * 16) + d % 8;
+                    auto *const p = (__attribute__((address_space(3))) uint16_t *)(base + (rowk * kPieces + (d / 8 ^ swizzle_v<DIM>(rowk))) * 16) + d % 8;
                     if ((*p & kExp) == kExp) {
-                        atomicOr(&sBad[d], 1ull << rowk);
                         *p = 0;
+                        if (stored >> rowk & 1) {
+                            // rows from the key's own position on, as far as the window reaches
+                            const int64_t key = k0 + rowk, r0 = (int64_t)tile_index * kRows;
+                            const int64_t from = (key - seq.pos) * group - r0, upto = a.window ? (key + a.window - seq.pos) * group - r0 : kRows;
+                            for (uint32_t w = 0; w < 4; ++w) {
+                                const int64_t x = from - 32 * w, y = upto - 32 * w;
+                                const uint32_t bits = (y >= 32 ? ~0u : y <= 0 ? 0u : (1u << y) - 1) & (x <= 0 ? ~0u : x >= 32 ? 0u : ~0u << x);
+                                if (bits) {
+                                    atomicOr(&sPoison[4 * d + w], bits);
+                                    *sAny = 1;
+                                }
+                            }
+                        }
                     }
                 }
                 __syncthreads();
@@ -478,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         auto keys = [&](int st) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                kf[st & 3][i] = *(const V *)(now + i * 32 * DIM * 2 + at_k[st]);
+                kf[st & 3][i] = *(const __attribute__((address_space(3))) V *)(now + i * 32 * DIM * 2 + at_k[st]);
             }
         };
 #pragma unroll
@@ -504,7 +523,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         V vv[2][kOut], ph[2], pl[2];
         Words<4> pw[2];
         auto value = [&](int u, int i) {
-            const uint8_t *const base = now + kTileBytes + u * 16 * DIM * 2;
+            lds_t const base = now + kTileBytes + u * 16 * DIM * 2;
             struct {
                 v4s a, b;
             } w;
@@ -555,7 +574,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            top = fmaxf(top, fmaxf(s[0][j], s[1][j]));
+            top = max_of(top, s[0][j], s[1][j]);
         }
         top *= xscale;
         if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {
@@ -636,26 +655,32 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 }
             }
         }
-        if (bad) {
-#pragma unroll
-            for (int i = 0; i < kOut; ++i) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if ((CT == PT_I8 ? bad_keys : sBad[32 * i + 8 * (j / 4) + 4 * h + j % 4]) & seen) {
-                        o[i][j] = NAN;
-                    }
-                }
-            }
+        if (CT == PT_I8) {
+            poisoned |= (sBad[buf] & seen) != 0;
         }
     };
     for (uint32_t t = t0; t < t1; t += 2) {
-        step_over(t, 0, smem, smem + 2 * kTileBytes);
+        step_over(t, 0, sTiles, sTiles + 2 * kTileBytes);
         if (t + 1 < t1) {
-            step_over(t + 1, 1, smem + 2 * kTileBytes, smem);
+            step_over(t + 1, 1, sTiles + 2 * kTileBytes, sTiles);
         }
     }
 
     l += __shfl_xor(l, 32, 64);
+    if (CT == PT_I8) {
+        l = poisoned ? NAN : l;
+    } else {
+        __syncthreads();
+        if (*sAny) {
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    o[i][j] = sPoison[4 * (32 * i + 8 * (j / 4) + 4 * h + j % 4) + wave] >> c & 1 ? NAN : o[i][j];
+                }
+            }
+        }
+    }
     if (alone) {
         if (!mine) {
             return;
