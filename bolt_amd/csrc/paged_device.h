@@ -257,13 +257,18 @@ struct CacheOperand : Operand<CT> {
     }
 };
 
-// two bytes in the low halves of a word's two 16-bit places, of two's complement -> two fp16: flipping the sign bit and
-// setting 0x64 in front makes 1024 + 128 + value, exactly
-__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w)
+// Two bytes in the low halves of a word's two 16-bit places, of two's complement -> two fp16: with the sign bit flipped and
+// 0x64 in front (biased) they read 1024 + 128 + value, exactly
+__device__ __forceinline__ uint32_t biased_to_f16(uint32_t w)
 {
     typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-    const v2h x = __builtin_bit_cast(v2h, w ^ 0x64806480u);
+    const v2h x = __builtin_bit_cast(v2h, w);
     return __builtin_bit_cast(uint32_t, x - (v2h){(_Float16)1152.0f, (_Float16)1152.0f});
+}
+
+__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w)
+{
+    return biased_to_f16(w ^ 0x64806480u);
 }
 
 template <>

@@ -196,11 +196,17 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float a, float 
 template <int CT, int DIM>
 constexpr uint32_t prompt_lds()
 {
-    return 4 * kKeys * DIM * 2 + (CT == PT_I8 ? 4 * kKeys * 4 + 2 * 8 + 2 * 4 : DIM * 16 + 4 * 4 + 4);
+    return CT == PT_I8 ? 2 * kKeys * DIM * 2 + 2 * kKeys * DIM + 2 * kKeys * 4 + 8 + 4 : 4 * kKeys * DIM * 2 + DIM * 16 + 4 * 4 + 4;
 }
 
-// PAGE8: pages of eight keys and more
-template <int ACT, int CT, int DIM, bool PAGE8>
+// rows of a tile that one load of a wave brings
+template <int CT, int DIM>
+constexpr uint32_t rows_at()
+{
+    return 64 / (DIM * (CT == PT_I8 ? 1 : 2) / 16);
+}
+
+template <int ACT, int CT, int DIM, bool PAGED>
 __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs a, uint32_t shares)
 {
     typedef Product<CT> Op;
@@ -208,16 +214,18 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     constexpr bool kWide = ACT == PT_F32;                                            // two parts per operand
     constexpr bool kShiftQ = kWide || (ACT == PT_BF16 && CT == PT_I8);
     constexpr uint32_t kTileBytes = kKeys * DIM * 2, kRowBytes = DIM * (CT == PT_I8 ? 1 : 2), kPieces = DIM / 8;
-    constexpr int kSteps = DIM / 16, kOut = DIM / 32, kLoads = kTileBytes / 16 / 256;
-    // LDS: two buffers, each a tile of keys and one of values; behind them
-    //   int8:  [2][keys' 64, values' 64] steps, [2] keys whose step is not finite, [2] the largest step of a tile
-    //   else:  [DIM][128 rows as bits] rows that see a value which is not finite, [4] whether a wave found one, whether there is any
+    constexpr int kSteps = DIM / 16, kOut = DIM / 32, kLoads = kKeys * kRowBytes / 16 / 256;
+    // LDS, 16-bit caches: two buffers, each a tile of keys and one of values; [DIM][128 rows as bits] rows that see a value which is
+    //        not finite, [4] whether a wave found one, whether there is any
+    //      int8: a tile of keys and one of values in fp16, the next ones as they are stored; steps of 64 keys and 64 values, keys
+    //        whose step is not finite (64 bits), the power of two above the largest step
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     lds_t const sTiles = (lds_t)0;  // smem's own address: the kernel has no other LDS. As a constant it goes into the reads' offsets.
-    float *const sStep = (float *)(smem + 4 * kTileBytes);
-    unsigned long long *const sBad = (unsigned long long *)(sStep + 4 * kKeys);
-    float *const sTop = (float *)(sBad + 2);
-    uint32_t *const sPoison = (uint32_t *)(smem + 4 * kTileBytes), *const sHit = sPoison + 4 * DIM, *const sAny = sHit + 4;
+    constexpr uint32_t kRawBytes = kKeys * DIM, kBehind = CT == PT_I8 ? 2 * kTileBytes + 2 * kRawBytes : 4 * kTileBytes;
+    float *const sStep = (float *)(smem + kBehind);
+    unsigned long long *const sBad = (unsigned long long *)(sStep + 2 * kKeys);
+    float *const sUnit = (float *)(sBad + 1);
+    uint32_t *const sPoison = (uint32_t *)(smem + kBehind), *const sHit = sPoison + 4 * DIM, *const sAny = sHit + 4;
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t c = lane & 31, h = lane >> 5;
@@ -249,10 +257,10 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     const uint32_t all_hi = paged_span(all.first, 0, all.hi).hi, all_lo = paged_span(all.last, a.window, all.hi).lo;  // seen by every row
 
     V qh[kSteps], ql[kWide ? kSteps : 1];
-    float xscale = a.scale2;
+    const float score_scale = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);  // (int8: part of the keys' steps)
+    float xscale = CT == PT_I8 ? 1.0f : score_scale;                      // the factor of the scores, positive
     {
-        const float sign = a.scale2 == 0.0f ? 0.0f : a.scale2 < 0.0f ? -1.0f : 1.0f;  // the factor of the scores is positive
-        xscale = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);
+        const float sign = a.scale2 == 0.0f ? 0.0f : a.scale2 < 0.0f ? -1.0f : 1.0f;
         const size_t at = (size_t)(mine ? row : 0) * a.qstride + (size_t)(mine ? head : 0) * DIM + 8 * h;
         float top = 0.0f, up = 1.0f;
         if (kShiftQ) {
@@ -306,11 +314,11 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     // Page of key k0 + lane, none: -1. In two halves: the list is read a tile ahead of its use.
     auto look_up = [&](uint32_t k0) -> int32_t { return table[min(k0 + lane, all.hi - 1) >> a.pool.shift]; };
     auto page_of = [&](uint32_t k0, int32_t found) -> int32_t { return k0 + lane < all.hi && (uint32_t)found < a.pool.pages ? found : -1; };
-    // A wave's load n covers kRowsAt rows of the tile, from row (4n + wave) kRowsAt on. In pages of eight keys and more they lie side
-    // by side, so that their address is the wave's and what a lane adds to it is the same for every load. A key without a page
-    // is read from page 0: what it brings is masked, and taken out of the tile where it is not finite.
-    constexpr uint32_t kRowsAt = 64 / kPieces;
-    const uint32_t in_row = lane / kPieces, piece = lane % kPieces;
+    // A wave's load n covers kRowsAt rows of the tile, from row (4n + wave) kRowsAt on. In pages of so many keys and more (PAGED) they
+    // lie side by side, so that their address is the wave's and what a lane adds to it is the same for every load. A key without
+    // a page is read from page 0: what it brings is masked, and taken out of the tile where it is not finite.
+    constexpr uint32_t kRowsAt = rows_at<CT, DIM>(), kChunks = kRowBytes / 16;
+    const uint32_t in_row = lane / kChunks, chunk = lane % kChunks;
     // byte offset of key k0 + lane in the pool
     auto offset_of = [&](uint32_t k0, int32_t page) -> size_t {
         const size_t first = (size_t)(uint32_t)max(page, 0) * a.pool.kv_heads + kvh;
@@ -318,7 +326,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     };
     // of load n: the wave's part in *base, the lane's as the answer
     auto row_at = [&](size_t offset, int n, size_t *base) -> uint32_t {
-        if (PAGE8) {
+        if (PAGED) {
             const uint32_t from = n * 4 * kRowsAt + wave * kRowsAt;
             *base = (size_t)__builtin_amdgcn_readlane((uint32_t)(offset >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)offset, from);
             return in_row * kRowBytes;
@@ -327,11 +335,13 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         *base = (size_t)(uint32_t)__shfl((uint32_t)(offset >> 32), from, 64) << 32 | (uint32_t)__shfl((uint32_t)offset, from, 64);
         return 0;
     };
-    // 16-bit caches: straight into a buffer
+    // Straight into LDS: a 16-bit cache's rows with their pieces permuted, an int8 cache's as they are
     const uint32_t first_row = wave * kRowsAt + in_row;  // of load 0; the others' rows are 4 kRowsAt apart, which changes no permutation
+    float scale = 0.0f;                                  // int8: of key lane (wave 0: key, wave 1: value)
     auto fetch = [&](uint32_t k0, int32_t pages, lds_t to) {
+        constexpr uint32_t kApart = CT == PT_I8 ? kRawBytes : kTileBytes;
         const size_t offset = offset_of(k0, pages);
-        const uint32_t pk = 16 * (piece ^ swizzle_k<DIM>(first_row)), pv = 16 * (piece ^ swizzle_v<DIM>(first_row));
+        const uint32_t pk = 16 * (CT == PT_I8 ? chunk : chunk ^ swizzle_k<DIM>(first_row)), pv = 16 * (CT == PT_I8 ? chunk : chunk ^ swizzle_v<DIM>(first_row));
         lds_t const mine_to = to + wave * 1024;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
@@ -339,43 +349,35 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             const uint32_t add = row_at(offset, n, &base);
             const uint8_t *const kp = (const uint8_t *)a.pool.k + base, *const vp = (const uint8_t *)a.pool.v + base;
             __builtin_amdgcn_global_load_lds((gptr_t)(kp + (add + pk)), (lptr_t)(mine_to + n * 4096), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gptr_t)(vp + (add + pv)), (lptr_t)(mine_to + kTileBytes + n * 4096), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr_t)(vp + (add + pv)), (lptr_t)(mine_to + kApart + n * 4096), 16, 0, 0);
+        }
+        if (CT == PT_I8 && wave < 2) {
+            scale = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[offset / kRowBytes];
         }
     };
-    // int8: eight values of a row per piece into registers, then as fp16 into the buffer
-    v2u rk[CT == PT_I8 ? kLoads : 1], rv[CT == PT_I8 ? kLoads : 1];
-    float rs = 0.0f;
-    auto fetch8 = [&](uint32_t k0, int32_t pages) {
-        const size_t offset = offset_of(k0, pages);
+    // int8: what this wave fetched, from where it lies to fp16 tiles; and the steps. Those of values are multiples of a power of two
+    // that none exceeds; one that is not finite is taken out.
+    auto convert = [&](lds_t from, lds_t to) {
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            size_t base;
-            const uint32_t add = row_at(offset, n, &base) + 8 * piece;
-            rk[n] = *(const v2u *)((const uint8_t *)a.pool.k + base + add);
-            rv[n] = *(const v2u *)((const uint8_t *)a.pool.v + base + add);
-        }
-        if (wave < 2) {
-            rs = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[offset / kRowBytes];
-        }
-    };
-    auto put8 = [&](uint32_t buf, lds_t to) {
-#pragma unroll
-        for (int n = 0; n < kLoads; ++n) {
-            const uint32_t rowk = (n * 4 + wave) * kRowsAt + in_row;
+            const uint32_t rowk = n * 4 * kRowsAt + first_row;
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
-                const v2u w = kv ? rv[n] : rk[n];
-                v4u f;
+                const v4u w = *(const __attribute__((address_space(3))) v4u *)(from + kv * kRawBytes + wave * 1024 + n * 4096 + lane * 16);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    f[i] = bytes_to_f16(__builtin_amdgcn_perm(0, w[i / 2], i & 1 ? 0x0c030c02 : 0x0c010c00));
+                for (int half = 0; half < 2; ++half) {
+                    v4u f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        f[i] = biased_to_f16(__builtin_amdgcn_perm(0x64646464u, w[2 * half + i / 2] ^ 0x80808080u, i & 1 ? 0x04030402 : 0x04010400));
+                    }
+                    const uint32_t piece = (2 * chunk + half) ^ (kv ? swizzle_v<DIM>(rowk) : swizzle_k<DIM>(rowk));
+                    *(__attribute__((address_space(3))) v4u *)(to + kv * kTileBytes + (rowk * kPieces + piece) * 16) = f;
                 }
-                const uint32_t place = rowk * kPieces + (piece ^ (kv ? swizzle_v<DIM>(rowk) : swizzle_k<DIM>(rowk)));
-                *(__attribute__((address_space(3))) v4u *)(to + kv * kTileBytes + place * 16) = f;
             }
         }
         if (wave < 2) {
-            float step = __builtin_amdgcn_rcpf(rs);
+            float step = __builtin_amdgcn_rcpf(scale);
             if (wave == 1) {
                 const bool fine = step - step == 0.0f;  // neither infinite nor NaN
                 const unsigned long long not_fine = __ballot(!fine);
@@ -385,12 +387,16 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 for (int off = 32; off; off >>= 1) {
                     most = fmaxf(most, __shfl_xor(most, off, 64));
                 }
+                const float unit_of_tile = power_above(most);
                 if (lane == 0) {
-                    sBad[buf] = not_fine;
-                    sTop[buf] = most;
+                    *sBad = not_fine;
+                    *sUnit = unit_of_tile;
                 }
+                step *= __builtin_amdgcn_rcpf(unit_of_tile);
+            } else {
+                step *= score_scale;
             }
-            sStep[buf * 2 * kKeys + wave * kKeys + lane] = step;
+            sStep[wave * kKeys + lane] = step;
         }
     };
 
@@ -416,31 +422,24 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         const uint32_t k0 = all.lo + t0 * kKeys;
         pages = page_of(k0, look_up(k0));
         next = look_up(k0 + kKeys);
-        if (CT == PT_I8) {
-            fetch8(k0, pages);
-        } else {
-            fetch(k0, pages, sTiles);
-        }
+        fetch(k0, pages, CT == PT_I8 ? sTiles + 2 * kTileBytes : sTiles);
     }
-    // One tile: `now` holds it, `ahead` is where the next one goes. (The compiler has to know that the two are apart, else it waits
+    // One tile: `now` holds it, `ahead` is where the next one goes (int8: where this one lies as it is stored, too). (The compiler has to know that the two are apart, else it waits
     // for the next tile's arrival before it reads this one.)
-    auto step_over = [&](uint32_t t, uint32_t buf, __attribute__((address_space(3))) uint8_t *__restrict now,
+    auto step_over = [&](uint32_t t, __attribute__((address_space(3))) uint8_t *__restrict now,
                          __attribute__((address_space(3))) uint8_t *__restrict ahead) {
         const uint32_t k0 = all.lo + t * kKeys;
         const unsigned long long stored = __ballot(pages >= 0);
-        if (CT == PT_I8) {
-            put8(buf, now);
-        }
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile is there
-        __syncthreads();                     // everyone's; and everyone is done with the other buffer
+        __syncthreads();                     // everyone's; and everyone is done with the tile before
+        if (CT == PT_I8) {
+            convert(ahead, now);
+            __syncthreads();
+        }
         pages = page_of(k0 + kKeys, next);
         next = look_up(k0 + 2 * kKeys);
         if (t + 1 < t1) {
-            if (CT == PT_I8) {
-                fetch8(k0 + kKeys, pages);
-            } else {
-                fetch(k0 + kKeys, pages, ahead);
-            }
+            fetch(k0 + kKeys, pages, ahead);
         }
         // does every row of the workgroup see every key of the tile?
         const bool whole = stored == ~0ull && k0 + kKeys <= all_hi && k0 >= all_lo;
@@ -486,22 +485,23 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         if (!__any(span.hi > k0 && span.lo < k0 + kKeys)) {
             return;  // nothing for this wave
         }
-        // Scores. The order is written out (the compiler would wait for every read right behind it): eight reads ahead of the
+        // Scores. The order is written out (the compiler would wait for every read right behind it): six or eight reads ahead of the
         // products that use them.
         v16f s[2];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             s[0][j] = s[1][j] = 0.0f;
         }
-        V kf[4][2];
+        constexpr int kRing = CT == PT_I8 || kWide ? 3 : 4;  // pairs of reads under way
+        V kf[kRing][2];
         auto keys = [&](int st) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                kf[st & 3][i] = *(const __attribute__((address_space(3))) V *)(now + i * 32 * DIM * 2 + at_k[st]);
+                kf[st % kRing][i] = *(const __attribute__((address_space(3))) V *)(now + i * 32 * DIM * 2 + at_k[st]);
             }
         };
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
+        for (int st = 0; st < kRing; ++st) {
             keys(st);
         }
         in_order();
@@ -509,14 +509,14 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         for (int st = 0; st < kSteps; ++st) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                s[i] = Op::mfma(kf[st & 3][i], qh[st], s[i]);
+                s[i] = Op::mfma(kf[st % kRing][i], qh[st], s[i]);
                 if (kWide) {
-                    s[i] = Op::mfma(kf[st & 3][i], ql[st], s[i]);
+                    s[i] = Op::mfma(kf[st % kRing][i], ql[st], s[i]);
                 }
             }
             in_order();
-            if (st + 4 < kSteps) {
-                keys(st + 4);
+            if (st + kRing < kSteps) {
+                keys(st + kRing);
                 in_order();
             }
         }
@@ -541,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                    const v4f ks = *(const v4f *)(sStep + buf * 2 * kKeys + 32 * i + 2 * j + 4 * h);
+                    const v4f ks = *(const v4f *)(sStep + 32 * i + 2 * j + 4 * h);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         s[i][j + e] *= ks[e];
@@ -550,14 +550,10 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             }
         }
         unsigned long long seen = ~0ull;
-        float wide = CT == PT_I8 ? sTop[buf] : 0.0f;  // int8: the largest step among the keys that this row sees
         if (!whole) {
             const uint32_t from = span.lo > k0 ? span.lo - k0 : 0, upto = span.hi > k0 ? span.hi - k0 : 0;  // keys of the tile this row sees
             seen = from >= kKeys || upto <= from ? 0 : (upto >= kKeys ? ~0ull : (1ull << upto) - 1) & (~0ull << from);
             seen &= stored;
-            if (CT == PT_I8) {
-                wide = 0.0f;
-            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t half = (uint32_t)(seen >> (32 * i)) >> (4 * h);
@@ -565,9 +561,6 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 for (int j = 0; j < 16; ++j) {
                     const bool sees = half >> (8 * (j / 4) + j % 4) & 1;
                     s[i][j] = sees ? s[i][j] : -INFINITY;
-                    if (CT == PT_I8) {
-                        wide = fmaxf(wide, sees ? sStep[buf * 2 * kKeys + kKeys + 32 * i + 8 * (j / 4) + 4 * h + j % 4] : 0.0f);
-                    }
                 }
             }
         }
@@ -577,7 +570,8 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             top = max_of(top, s[0][j], s[1][j]);
         }
         top *= xscale;
-        if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {
+        const float tile_unit = CT == PT_I8 ? *sUnit : 1.0f;
+        if (__any(top > m + kSlack || (CT == PT_I8 && tile_unit > unit))) {
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const float up = fmaxf(top, m);
             float corr = __builtin_amdgcn_exp2f(m - up);
@@ -585,8 +579,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             m = up;
             if (CT == PT_I8) {
                 const float was = unit;
-                wide = fmaxf(wide, __shfl_xor(wide, 32, 64));
-                unit = power_above(fmaxf(wide, unit));
+                unit = fmaxf(tile_unit, unit);
                 corr *= was * __builtin_amdgcn_rcpf(unit);
             }
 #pragma unroll
@@ -595,21 +588,25 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             }
         }
         // Weights times values, 16 keys a step: behind every product stand the next step's reads and a share of its weights
-        const float shift = kLift - m, per_unit = __builtin_amdgcn_rcpf(unit);
+        // (int8: the tile's steps are multiples of its own power of two; what that is of the output's goes into the exponent, and
+        // out of the sum again. It ends at 2^-64, where a tile's values are far below what the output can hold of others.)
+        const float part = CT == PT_I8 ? fmaxf(tile_unit * __builtin_amdgcn_rcpf(unit), 5.42101086e-20f) : 1.0f;
+        const float shift = (CT == PT_I8 ? kLift + __builtin_amdgcn_logf(part) : kLift) - m;
+        float sum = 0.0f;
         float p[8];
         auto weight = [&](int u, int j) {  // j and j + 1
             v2f vs;
             if (CT == PT_I8) {
-                vs = *(const v2f *)(sStep + buf * 2 * kKeys + kKeys + 16 * u + 8 * (j / 4) + 4 * h + j % 4);
+                vs = *(const v2f *)(sStep + kKeys + 16 * u + 8 * (j / 4) + 4 * h + j % 4);
             }
 #pragma unroll
             for (int e = j; e < j + 2; ++e) {
                 p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u % 2) + e], xscale, shift));
-                if (kWide || CT == PT_I8) {
-                    l += p[e];
-                }
                 if (CT == PT_I8) {
-                    p[e] *= vs[e - j] * per_unit;
+                    sum += p[e];
+                    p[e] *= vs[e - j];
+                } else if (kWide) {
+                    l += p[e];
                 }
             }
             if (!kWide) {
@@ -656,13 +653,18 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             }
         }
         if (CT == PT_I8) {
-            poisoned |= (sBad[buf] & seen) != 0;
+            l += sum * __builtin_amdgcn_rcpf(part);
+            poisoned |= (*sBad & seen) != 0;
         }
     };
     for (uint32_t t = t0; t < t1; t += 2) {
-        step_over(t, 0, sTiles, sTiles + 2 * kTileBytes);
+        step_over(t, sTiles, sTiles + 2 * kTileBytes);
         if (t + 1 < t1) {
-            step_over(t + 1, 1, sTiles + 2 * kTileBytes, sTiles);
+            if (CT == PT_I8) {
+                step_over(t + 1, sTiles, sTiles + 2 * kTileBytes);
+            } else {
+                step_over(t + 1, sTiles + 2 * kTileBytes, sTiles);
+            }
         }
     }
 
@@ -758,7 +760,7 @@ uint32_t shares_of(const PagedPool &pool, const PagedBatch &b, uint32_t heads)
 {
     const uint64_t grid = most_tiles(b, heads / pool.kv_heads) * pool.kv_heads;
     const uint64_t keys = (((uint64_t)b.max_pages << pool.shift) + kKeys * kLeast - 1) / (kKeys * kLeast);
-    const uint64_t n = grid >= kSpread ? 1 : kSpread / grid;
+    const uint64_t n = grid >= kSpread ? 1 : (kSpread + grid / 2) / grid;
     return (uint32_t)(n < keys ? n : keys);
 }
 
@@ -777,7 +779,7 @@ struct Prompt {
             return ready;
         }
         const uint64_t blocks = tiles * a.pool.kv_heads;
-        if (a.pool.shift >= 3) {
+        if (1u << a.pool.shift >= rows_at<CT, DIM>()) {
             hipLaunchKernelGGL((paged_prompt_kernel<ACT, CT, DIM, true>), dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
         } else {
             hipLaunchKernelGGL((paged_prompt_kernel<ACT, CT, DIM, false>), dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
