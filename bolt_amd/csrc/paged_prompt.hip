@@ -358,12 +358,15 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     // int8: what this wave fetched, from where it lies to fp16 tiles; and the steps. Those of values are multiples of a power of two
     // that none exceeds; one that is not finite is taken out.
     auto convert = [&](lds_t from, lds_t to) {
+        uint32_t me = lane;
+        asm volatile("" : "+v"(me));  // addresses are made anew: kept from tile to tile they would cost registers that the tile needs
+        const uint32_t chunk = me % kChunks;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const uint32_t rowk = n * 4 * kRowsAt + first_row;
+            const uint32_t rowk = (n * 4 + wave) * kRowsAt + me / kChunks;
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
-                const v4u w = *(const __attribute__((address_space(3))) v4u *)(from + kv * kRawBytes + wave * 1024 + n * 4096 + lane * 16);
+                const v4u w = *(const __attribute__((address_space(3))) v4u *)(from + kv * kRawBytes + wave * 1024 + n * 4096 + me * 16);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     v4u f;
@@ -482,8 +485,8 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 __syncthreads();
             }
         }
-        if (!__any(span.hi > k0 && span.lo < k0 + kKeys)) {
-            return;  // nothing for this wave
+        if (CT != PT_I8 && !__any(span.hi > k0 && span.lo < k0 + kKeys)) {
+            return;  // nothing for this wave (int8: gone through all the same, the way round it cost a copy of every output register)
         }
         // Scores. The order is written out (the compiler would wait for every read right behind it): six or eight reads ahead of the
         // products that use them.
