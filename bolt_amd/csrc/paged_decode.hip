@@ -14,24 +14,29 @@
 // 2^15, inside fp16; a weight of less than 2^-37 of the row's largest is lost. An int8 cache's steps (1 / scale) are part of
 // the weights, divided by a power of two that no step exceeds, so that they add nothing to that range.
 //
-// The keys of all sequences are cut into chunks of equal length, chosen on the device from the lengths themselves (a
-// captured launch serves any lengths): about kTarget workgroups in all. A sequence with one chunk writes its output;
-// several leave (maximum, sum, output) parts, which a second launch joins.
+// The tiles (of 128 keys) of all sequences stand in one row that is cut into equal shares, as many as workgroups fit the chip:
+// every workgroup reads the same number of bytes, whatever the lengths are. They are read on the device, so a captured launch
+// serves any. A share may hold the end of one sequence, whole ones, and the beginning of another; a sequence that lies in one
+// share is written out, one that several hold leaves (maximum, sum, output) parts, which a second launch joins.
 #include "paged_device.h"
 
 namespace bg {
 
 namespace {
 
-constexpr uint32_t kTarget = 1024;   // workgroups that a launch aims at
-constexpr uint32_t kTile = 128;      // keys of one round of a workgroup's four waves
-constexpr uint32_t kMinTiles = 2;    // shortest chunk, in tiles
+constexpr uint32_t kCus = 256;
+constexpr uint32_t kTileShift = 7;   // keys of one round of a workgroup's four waves: 128
+constexpr uint32_t kLeast = 1;       // fewest tiles in a share
+
+// workgroups of this kernel that a CU holds (registers)
+template <int DIM>
+constexpr uint32_t per_cu()
+{
+    return DIM == 128 ? 3 : 4;
+}
+
 constexpr float kLow = -1.7e38f;     // running maximum before the first key
 constexpr float kSlack = 2.0f, kLift = 13.0f;  // see above: 2^(kSlack + kLift) fits fp16
-
-struct Chunk {
-    uint32_t b, index, count, part;  // sequence; which of its chunks, of how many; its first part's number
-};
 
 __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v)
 {
@@ -47,73 +52,55 @@ __device__ __forceinline__ PagedSpan span_of(const PagedAttentionArgs &a, uint32
     return paged_span((int64_t)a.batch.lens[b] - 1, a.window, a.batch.max_pages << a.pool.shift);
 }
 
-// tiles of a sequence, counted from its first key rounded down to a step of 32
-__device__ __forceinline__ uint32_t tiles_of(const PagedAttentionArgs &a, uint32_t b)
+// Tiles of a sequence, counted from its first key rounded down to a step of 32; one where there is nothing to see (somebody
+// has to write the zeros). shift: kTileShift, more where the launch could have 2^31 of them.
+__device__ __forceinline__ uint32_t tiles_of(const PagedAttentionArgs &a, uint32_t b, uint32_t shift)
 {
     const PagedSpan s = span_of(a, b);
-    return (s.hi - (s.lo & ~31u) + kTile - 1) / kTile;
+    const uint32_t n = (s.hi - (s.lo & ~31u) + (1u << shift) - 1) >> shift;
+    return n ? n : 1;
 }
 
-__device__ __forceinline__ uint32_t chunks_of(uint32_t tiles, uint32_t per)
+// tiles per share, with `shares` of them to a key head's column
+__device__ __forceinline__ uint32_t tiles_per_share(const PagedAttentionArgs &a, uint32_t shares, uint32_t shift, uint32_t lane)
 {
-    return tiles ? (tiles - 1) / per + 1 : 1;
-}
-
-// Tiles per chunk. per_head: chunks that a key head's share of the launch has room for beside one per sequence.
-__device__ __forceinline__ uint32_t tiles_per_chunk(const PagedAttentionArgs &a, uint32_t per_head, uint32_t lane)
-{
-    // a launch has at most 65535 sequences of 2^24 tiles: summed in units that fit 32 bits
     uint32_t sum = 0;
     for (uint32_t b = lane; b < a.batch.batch; b += 64) {
-        sum += (tiles_of(a, b) + 511) / 512;
+        sum += tiles_of(a, b, shift);
     }
-    const uint32_t coarse = wave_sum_u32(sum);
-    uint32_t per;
-    if (coarse < (1u << 22)) {
-        sum = 0;
-        for (uint32_t b = lane; b < a.batch.batch; b += 64) {
-            sum += tiles_of(a, b);
-        }
-        per = (wave_sum_u32(sum) + per_head - 1) / per_head;
-    } else {
-        per = (coarse / per_head + 1) * 512;
-    }
-    return per < kMinTiles ? kMinTiles : per;
+    const uint32_t per = (wave_sum_u32(sum) + shares - 1) / shares;
+    return per < kLeast ? kLeast : per;
 }
 
-// Chunk number x of the launch's list (false: behind the last); every wave finds out by itself.
-__device__ __forceinline__ bool find_chunk(const PagedAttentionArgs &a, uint32_t per, uint32_t x, uint32_t lane, Chunk *out)
+// The sequence that tile number `tile` belongs to, and the tiles before it (false: behind the last). Every wave finds out by itself.
+__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t tile, uint32_t shift, uint32_t lane, uint32_t *b_out, uint32_t *before)
 {
-    uint32_t base = 0, part = 0;
+    uint32_t base = 0;
     for (uint32_t b0 = 0; b0 < a.batch.batch; b0 += 64) {
-        const uint32_t b = b0 + lane;
-        const uint32_t n = b < a.batch.batch ? chunks_of(tiles_of(a, b), per) : 0;
+        const uint32_t n = b0 + lane < a.batch.batch ? tiles_of(a, b0 + lane, shift) : 0;
         uint32_t upto = n;
 #pragma unroll
         for (uint32_t off = 1; off < 64; off <<= 1) {
             const uint32_t v = __shfl_up(upto, off, 64);
             upto += lane >= off ? v : 0;
         }
-        const uint32_t all = __shfl(upto, 63, 64), parts = n > 1 ? n : 0;
-        if (x < base + all) {
-            const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(base + upto > x));
-            out->b = b0 + at;
-            out->count = __builtin_amdgcn_readlane(n, at);
-            out->index = x - base - (__builtin_amdgcn_readlane(upto, at) - out->count);
-            out->part = part + wave_sum_u32(lane < at ? parts : 0);
+        const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
+        if (tile < base + all) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(base + upto > tile));
+            *b_out = b0 + at;
+            *before = base + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at);
             return true;
         }
         base += all;
-        part += wave_sum_u32(parts);
     }
     return false;
 }
 
-// Parts of split sequences: room for 2 * per_head of them per key head and query tile (a sequence with n > 1 chunks has more
-// than (n - 1) * per tiles, so n <= 2 (n - 1) < 2 tiles / per in the sum). A part: 16 rows of DIM values, 16 maxima, 16 sums.
-__device__ __forceinline__ float *part_at(const PagedAttentionArgs &a, uint32_t per_head, uint32_t column, uint32_t part, uint32_t dim)
+// A part: 16 rows of DIM values, 16 maxima, 16 sums. A share leaves two at most: of the sequence that its first tile belongs to
+// (slot 0), and of one that begins inside it and goes on behind it (slot 1).
+__device__ __forceinline__ float *part_at(const PagedAttentionArgs &a, uint32_t shares, uint32_t column, uint32_t share, uint32_t slot, uint32_t dim)
 {
-    return (float *)a.ws + ((size_t)column * 2 * per_head + part) * 16 * (dim + 2);
+    return (float *)a.ws + (((size_t)column * shares + share) * 2 + slot) * 16 * (dim + 2);
 }
 
 template <int ACT>
@@ -131,7 +118,7 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, v4f v)
 
 // PAGE16: pages of 16 keys and more, so that each 16-key half of a step lies in one page and its address is the wave's.
 template <int ACT, int CT, int DIM, bool PAGE16>
-__global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttentionArgs a, uint32_t per_head)
+__global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedAttentionArgs a, uint32_t shares, uint32_t shift)
 {
     typedef CacheOperand<CT> Op;
     constexpr int kSteps = DIM / 32, kVec = DIM / 16;
@@ -142,285 +129,296 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttentionArgs
 
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 15, g = lane >> 4;
-    Chunk ch;
-    const uint32_t per = tiles_per_chunk(a, per_head, lane);
-    if (!find_chunk(a, per, blockIdx.x, lane, &ch)) {
-        return;
-    }
-    const uint32_t group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
+    const uint32_t per = tiles_per_share(a, shares, shift, lane);
+    const uint32_t share = blockIdx.x, group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
     const uint32_t kvh = blockIdx.y / qtiles, q0 = blockIdx.y % qtiles * 16;
     const uint32_t nq = group - q0 < 16 ? group - q0 : 16;
-    const uint32_t b = __builtin_amdgcn_readfirstlane(ch.b);
-    const PagedSpan span = span_of(a, b);
-    const uint32_t first = span.lo & ~31u, tiles = (span.hi - first + kTile - 1) / kTile;
-    const uint32_t mine = (tiles + ch.count - 1) / ch.count;  // tiles per chunk, evenly
-    const uint32_t from = first + ch.index * mine * kTile;
-    const uint32_t to = min(from + mine * kTile, span.hi);
-    const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
+    uint32_t b, before;
+    if ((uint64_t)share * per > 0xffffffffu || !find_tile(a, share * per, shift, lane, &b, &before)) {
+        return;
+    }
+    uint32_t tile = share * per;  // next tile of the row
+    const uint32_t end = tile + per;
+    for (;;) {
+        b = __builtin_amdgcn_readfirstlane(b);
+        const PagedSpan span = span_of(a, b);
+        const uint32_t first = span.lo & ~31u, behind = before + tiles_of(a, b, shift);
+        const uint32_t stop = min(behind, end);
+        const uint32_t from = first + ((tile - before) << shift);
+        const uint32_t to = min(first + ((stop - before) << shift), span.hi);
+        const bool whole_sequence = tile == before && stop == behind;
+        const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
 
-    // queries
-    typename Op::V qh[kSteps], ql[kSteps];
-    float xscale = a.scale2;
-    {
-        float x[kSteps][8];
-        const size_t at = (size_t)b * a.qstride + (size_t)(kvh * group + q0 + c) * DIM;
-        float top = 0.0f;
+        // queries
+        typename Op::V qh[kSteps], ql[kSteps];
+        float xscale = a.scale2;
+        {
+            float x[kSteps][8];
+            const size_t at = (size_t)b * a.qstride + (size_t)(kvh * group + q0 + c) * DIM;
+            float top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            if (c < nq) {
-                load8<ACT>(a.q, at + Op::d_of(s, g), x[s]);
+            for (int s = 0; s < kSteps; ++s) {
+                if (c < nq) {
+                    load8<ACT>(a.q, at + Op::d_of(s, g), x[s]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        x[s][j] = 0.0f;
+                    }
+                }
+                if (kShiftQ) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        top = fmaxf(top, fabsf(x[s][j]));
+                    }
+                }
+            }
+            float up = 1.0f;
+            if (kShiftQ) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                int e = 0;
+                up = shift_into_f16(top, &e);
+                xscale = ldexpf(a.scale2, e);
+            }
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                Op::split(x[s], up, &qh[s], &ql[s]);
+            }
+        }
+
+        v4f o[kVec];
+#pragma unroll
+        for (int t = 0; t < kVec; ++t) {
+            o[t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float m = kLow, l = 0.0f, unit = CT == PT_I8 ? kFirstUnit : 1.0f;  // unit: the power of two that o's int8 steps are divided by
+
+        for (uint32_t k0 = from + 32 * wave; k0 < to; k0 += 128) {
+            typename Op::Raw kr[2][Op::kRawK(DIM)];
+            typename Op::template RawV<DIM> vr[8];
+            v4f ksc[2], vsc[2];
+            uint32_t seen = 0xff;  // bit j: key 16 (j / 4) + 4g + j % 4 of the step takes part
+            if (PAGE16) {
+                const uint8_t *kb[2], *vb[2];
+                bool whole = k0 >= span.lo && k0 + 32 <= to;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t key = k0 + 16 * h;
+                    int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
+                    if (slot < 0) {
+                        seen &= h ? 0x0f : 0xf0;
+                        whole = false;
+                        slot = 0;
+                    }
+                    kb[h] = (const uint8_t *)a.pool.k + slot * kRowBytes;
+                    vb[h] = (const uint8_t *)a.pool.v + slot * kRowBytes;
+                    if (CT == PT_I8) {
+                        ksc[h] = load_scales(a.pool.ks + slot + 4 * g);
+                        vsc[h] = load_scales(a.pool.vs + slot + 4 * g);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    Op::load_k(kb[h] + c * kRowBytes, g, kr[h]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    vr[j] = Op::template load_v<DIM>(vb[j >> 2] + (4 * g + (j & 3)) * kRowBytes, c);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                        if (key < span.lo || key >= to) {
+                            seen &= ~(1u << j);
+                        }
+                    }
+                }
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[s][j] = 0.0f;
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t key = k0 + 16 * h + c;
+                    int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
+                    Op::load_k((const uint8_t *)a.pool.k + (slot < 0 ? 0 : slot) * kRowBytes, g, kr[h]);
                 }
-            }
-            if (kShiftQ) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    top = fmaxf(top, fabsf(x[s][j]));
-                }
-            }
-        }
-        float up = 1.0f;
-        if (kShiftQ) {
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            int e = 0;
-            up = shift_into_f16(top, &e);
-            xscale = ldexpf(a.scale2, e);
-        }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            Op::split(x[s], up, &qh[s], &ql[s]);
-        }
-    }
-
-    v4f o[kVec];
-#pragma unroll
-    for (int t = 0; t < kVec; ++t) {
-        o[t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    float m = kLow, l = 0.0f, unit = CT == PT_I8 ? kFirstUnit : 1.0f;  // unit: the power of two that o's int8 steps are divided by
-
-    for (uint32_t k0 = from + 32 * wave; k0 < to; k0 += kTile) {
-        typename Op::Raw kr[2][Op::kRawK(DIM)];
-        typename Op::template RawV<DIM> vr[8];
-        v4f ksc[2], vsc[2];
-        uint32_t seen = 0xff;  // bit j: key 16 (j / 4) + 4g + j % 4 of the step takes part
-        if (PAGE16) {
-            const uint8_t *kb[2], *vb[2];
-            bool whole = k0 >= span.lo && k0 + 32 <= to;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t key = k0 + 16 * h;
-                int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
-                if (slot < 0) {
-                    seen &= h ? 0x0f : 0xf0;
-                    whole = false;
-                    slot = 0;
-                }
-                kb[h] = (const uint8_t *)a.pool.k + slot * kRowBytes;
-                vb[h] = (const uint8_t *)a.pool.v + slot * kRowBytes;
-                if (CT == PT_I8) {
-                    ksc[h] = load_scales(a.pool.ks + slot + 4 * g);
-                    vsc[h] = load_scales(a.pool.vs + slot + 4 * g);
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                Op::load_k(kb[h] + c * kRowBytes, g, kr[h]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                vr[j] = Op::template load_v<DIM>(vb[j >> 2] + (4 * g + (j & 3)) * kRowBytes, c);
-            }
-            if (!whole) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                    if (key < span.lo || key >= to) {
+                    int64_t slot = key >= span.lo && key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
+                    if (slot < 0) {
                         seen &= ~(1u << j);
+                        slot = 0;
+                    }
+                    vr[j] = Op::template load_v<DIM>((const uint8_t *)a.pool.v + slot * kRowBytes, c);
+                    if (CT == PT_I8) {
+                        ksc[j >> 2][j & 3] = a.pool.ks[slot];
+                        vsc[j >> 2][j & 3] = a.pool.vs[slot];
                     }
                 }
             }
-        } else {
+            v4f s[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t key = k0 + 16 * h + c;
-                int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
-                Op::load_k((const uint8_t *)a.pool.k + (slot < 0 ? 0 : slot) * kRowBytes, g, kr[h]);
-            }
+                s[h] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                int64_t slot = key >= span.lo && key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
-                if (slot < 0) {
-                    seen &= ~(1u << j);
-                    slot = 0;
-                }
-                vr[j] = Op::template load_v<DIM>((const uint8_t *)a.pool.v + slot * kRowBytes, c);
-                if (CT == PT_I8) {
-                    ksc[j >> 2][j & 3] = a.pool.ks[slot];
-                    vsc[j >> 2][j & 3] = a.pool.vs[slot];
-                }
-            }
-        }
-        v4f s[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            s[h] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int t = 0; t < kSteps; ++t) {
-                const typename Op::V kv = Op::k_operand(kr[h], t);
-                s[h] = Op::mfma(kv, qh[t], s[h]);
-                if (kSplitQ) {
-                    s[h] = Op::mfma(kv, ql[t], s[h]);
-                }
-            }
-        }
-        float x[8], step[8], top = -INFINITY, wide = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float f = xscale;
-            if (CT == PT_I8) {
-                f *= __builtin_amdgcn_rcpf(ksc[j >> 2][j & 3]);
-                step[j] = __builtin_amdgcn_rcpf(vsc[j >> 2][j & 3]);
-            }
-            x[j] = s[j >> 2][j & 3] * f;
-        }
-        if (seen != 0xff) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (!(seen >> j & 1)) {
-                    x[j] = -INFINITY;
-                    if (CT == PT_I8) {
-                        step[j] = 0.0f;
-                    } else {
-                        vr[j] = Op::template zero_v<DIM>();
+                for (int t = 0; t < kSteps; ++t) {
+                    const typename Op::V kv = Op::k_operand(kr[h], t);
+                    s[h] = Op::mfma(kv, qh[t], s[h]);
+                    if (kSplitQ) {
+                        s[h] = Op::mfma(kv, ql[t], s[h]);
                     }
                 }
             }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            top = fmaxf(top, x[j]);
-            if (CT == PT_I8) {
-                wide = fmaxf(wide, step[j]);
-            }
-        }
-        if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float up = fmaxf(top, m);
-            float corr = __builtin_amdgcn_exp2f(m - up);
-            l *= corr;
-            m = up;
-            if (CT == PT_I8) {
-                const float was = unit;
-                wide = fmaxf(wide, unit);
-#pragma unroll
-                for (int off = 32; off; off >>= 1) {
-                    wide = fmaxf(wide, __shfl_xor(wide, off, 64));
-                }
-                unit = power_above(wide);
-                corr *= was * __builtin_amdgcn_rcpf(unit);
-            }
-#pragma unroll
-            for (int t = 0; t < kVec; ++t) {
-                o[t] = o[t] * corr;
-            }
-        }
-        float p[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(x[j] - m + kLift);
-            l += p[j];
-        }
-        if (CT == PT_I8) {
-            const float per_unit = __builtin_amdgcn_rcpf(unit);
+            float x[8], step[8], top = -INFINITY, wide = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[j] *= step[j] * per_unit;
+                float f = xscale;
+                if (CT == PT_I8) {
+                    f *= __builtin_amdgcn_rcpf(ksc[j >> 2][j & 3]);
+                    step[j] = __builtin_amdgcn_rcpf(vsc[j >> 2][j & 3]);
+                }
+                x[j] = s[j >> 2][j & 3] * f;
+            }
+            if (seen != 0xff) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (!(seen >> j & 1)) {
+                        x[j] = -INFINITY;
+                        if (CT == PT_I8) {
+                            step[j] = 0.0f;
+                        } else {
+                            vr[j] = Op::template zero_v<DIM>();
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                top = fmaxf(top, x[j]);
+                if (CT == PT_I8) {
+                    wide = fmaxf(wide, step[j]);
+                }
+            }
+            if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float up = fmaxf(top, m);
+                float corr = __builtin_amdgcn_exp2f(m - up);
+                l *= corr;
+                m = up;
+                if (CT == PT_I8) {
+                    const float was = unit;
+                    wide = fmaxf(wide, unit);
+#pragma unroll
+                    for (int off = 32; off; off >>= 1) {
+                        wide = fmaxf(wide, __shfl_xor(wide, off, 64));
+                    }
+                    unit = power_above(wide);
+                    corr *= was * __builtin_amdgcn_rcpf(unit);
+                }
+#pragma unroll
+                for (int t = 0; t < kVec; ++t) {
+                    o[t] = o[t] * corr;
+                }
+            }
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] = __builtin_amdgcn_exp2f(x[j] - m + kLift);
+                l += p[j];
+            }
+            if (CT == PT_I8) {
+                const float per_unit = __builtin_amdgcn_rcpf(unit);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    p[j] *= step[j] * per_unit;
+                }
+            }
+            typename Op::V ph, pl;
+            Op::split(p, 1.0f, &ph, &pl);
+#pragma unroll
+            for (int t = 0; t < kVec; ++t) {
+                const typename Op::V vt = Op::template v_operand<DIM>(vr, t);
+                o[t] = Op::mfma(vt, ph, o[t]);
+                o[t] = Op::mfma(vt, pl, o[t]);
             }
         }
-        typename Op::V ph, pl;
-        Op::split(p, 1.0f, &ph, &pl);
-#pragma unroll
-        for (int t = 0; t < kVec; ++t) {
-            const typename Op::V vt = Op::template v_operand<DIM>(vr, t);
-            o[t] = Op::mfma(vt, ph, o[t]);
-            o[t] = Op::mfma(vt, pl, o[t]);
-        }
-    }
 
-    // the four waves' parts
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (g == 0) {
-        sM[wave][c] = m;
-        sL[wave][c] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int t = 0; t < kVec; t += 4) {
-            *(v4f *)(&sO[wave][c * kRow + kVec * (4 * g + i) + t]) = (v4f){o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]} * unit;
+        // the four waves' parts
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (g == 0) {
+            sM[wave][c] = m;
+            sL[wave][c] = l;
         }
-    }
-    __syncthreads();
-    float *part = part_at(a, per_head, blockIdx.y, ch.part + ch.index, DIM);
-    for (uint32_t at = threadIdx.x; at < nq * (DIM / 4); at += 256) {
-        const uint32_t r = at / (DIM / 4), d = at % (DIM / 4) * 4;
-        const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
-        float sum = 0.0f;
-        v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sM[w][r] - top);
-            sum += sL[w][r] * f;
-            v += *(const v4f *)(&sO[w][r * kRow + d]) * f;
-        }
-        if (ch.count == 1) {
-            v = sum == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
-            store_out4<ACT>(a.out, (size_t)b * a.ostride + (size_t)(kvh * group + q0 + r) * DIM + d, v);
-        } else {
-            *(v4f *)(part + r * DIM + d) = v;
-            if (d == 0) {
-                part[16 * DIM + r] = top;
-                part[16 * DIM + 16 + r] = sum;
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int t = 0; t < kVec; t += 4) {
+                *(v4f *)(&sO[wave][c * kRow + kVec * (4 * g + i) + t]) = (v4f){o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]} * unit;
             }
         }
+        __syncthreads();
+        float *part = part_at(a, shares, blockIdx.y, share, tile != share * per, DIM);
+        for (uint32_t at = threadIdx.x; at < nq * (DIM / 4); at += 256) {
+            const uint32_t r = at / (DIM / 4), d = at % (DIM / 4) * 4;
+            const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
+            float sum = 0.0f;
+            v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sM[w][r] - top);
+                sum += sL[w][r] * f;
+                v += *(const v4f *)(&sO[w][r * kRow + d]) * f;
+            }
+            if (whole_sequence) {
+                v = sum == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
+                store_out4<ACT>(a.out, (size_t)b * a.ostride + (size_t)(kvh * group + q0 + r) * DIM + d, v);
+            } else {
+                *(v4f *)(part + r * DIM + d) = v;
+                if (d == 0) {
+                    part[16 * DIM + r] = top;
+                    part[16 * DIM + 16 + r] = sum;
+                }
+            }
+        }
+        tile = stop;
+        if (tile >= end || ++b >= a.batch.batch) {
+            return;
+        }
+        before = behind;
+        __syncthreads();  // the next sequence's parts go where these were
     }
 }
 
 // Joins the parts of split sequences: a workgroup per query head and sequence, DIM / 4 lanes to a part.
 template <int ACT, int DIM>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionArgs a, uint32_t per_head)
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionArgs a, uint32_t shares, uint32_t shift)
 {
     constexpr uint32_t kLanes = DIM / 4, kWays = 256 / kLanes;
     __shared__ __attribute__((aligned(16))) float sO[kWays][DIM];
     __shared__ float sL[kWays], sM[kWays];
     const uint32_t lane = threadIdx.x & 63, h = blockIdx.x, b = blockIdx.y;
-    const uint32_t per = tiles_per_chunk(a, per_head, lane);
-    const uint32_t count = chunks_of(tiles_of(a, b), per);
+    const uint32_t per = tiles_per_share(a, shares, shift, lane);
+    uint32_t before = 0;
+    for (uint32_t i = lane; i < b; i += 64) {
+        before += tiles_of(a, i, shift);
+    }
+    before = wave_sum_u32(before);
+    const uint32_t first = before / per, count = (before + tiles_of(a, b, shift) - 1) / per - first + 1;
     if (count == 1) {
         return;
     }
-    uint32_t before = 0;
-    for (uint32_t i = lane; i < b; i += 64) {
-        const uint32_t n = chunks_of(tiles_of(a, i), per);
-        before += n > 1 ? n : 0;
-    }
-    before = wave_sum_u32(before);
     const uint32_t group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
     const uint32_t kvh = h / group, in = h % group, r = in % 16;
-    const float *part = part_at(a, per_head, kvh * qtiles + in / 16, before, DIM);
+    const float *part = part_at(a, shares, kvh * qtiles + in / 16, first, 0, DIM);
+    const uint32_t slot = before % per != 0;  // of the first part; the others are the first of their share
     const uint32_t way = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
     float top = kLow, sum = 0.0f;
     v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t i = way; i < count; i += kWays) {
-        const float *p = part + (size_t)i * 16 * (DIM + 2);
+        const float *p = part + ((size_t)2 * i + (i ? 0 : slot)) * 16 * (DIM + 2);
         const float m = p[16 * DIM + r], up = fmaxf(top, m);
         const float f = __builtin_amdgcn_exp2f(top - up), e = __builtin_amdgcn_exp2f(m - up);
         sum = sum * f + p[16 * DIM + 16 + r] * e;
@@ -457,28 +455,49 @@ uint32_t columns(uint32_t heads, uint32_t kv_heads)
     return kv_heads * ((heads / kv_heads + 15) / 16);
 }
 
-uint32_t chunks_per_head(uint32_t heads, uint32_t kv_heads)
+// Shares of a column: of the numbers that fill the chip once to four times, the first that leaves no more than a tenth idle,
+// or else the one that leaves least.
+uint32_t shares_of(uint32_t heads, uint32_t kv_heads, uint32_t dim)
 {
-    const uint32_t n = columns(heads, kv_heads);
-    return n >= kTarget ? 1 : (kTarget + n - 1) / n;
+    const uint32_t n = columns(heads, kv_heads), fit = kCus * (dim == 128 ? per_cu<128>() : per_cu<64>());
+    uint32_t best = 1;
+    double used = 0.0;
+    for (uint32_t r = 1; r <= 4 && used < 0.9; ++r) {
+        const uint32_t s = fit * r / n;
+        if (s && (double)s * n / (fit * r) > used) {
+            used = (double)s * n / (fit * r);
+            best = s;
+        }
+    }
+    return best;
+}
+
+uint32_t tile_shift(const PagedPool &pool, const PagedBatch &b)
+{
+    uint32_t shift = kTileShift;
+    while ((uint64_t)b.batch * ((((uint64_t)b.max_pages << pool.shift) >> shift) + 2) > 0x7fffffffull) {
+        ++shift;
+    }
+    return shift;
 }
 
 template <int ACT, int CT, int DIM>
 struct Decode {
     static hipError_t run(const PagedAttentionArgs &a, hipStream_t st)
     {
-        const uint32_t per_head = chunks_per_head(a.heads, a.pool.kv_heads);
-        const dim3 grid(per_head + a.batch.batch, columns(a.heads, a.pool.kv_heads));
+        const uint32_t shares = shares_of(a.heads, a.pool.kv_heads, DIM), shift = tile_shift(a.pool, a.batch);
+        const dim3 grid(shares, columns(a.heads, a.pool.kv_heads));
         if (a.pool.shift >= 4) {
-            hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, true>), grid, dim3(256), 0, st, a, per_head);
+            hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, true>), grid, dim3(256), 0, st, a, shares, shift);
         } else {
-            hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, false>), grid, dim3(256), 0, st, a, per_head);
+            hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, false>), grid, dim3(256), 0, st, a, shares, shift);
         }
         const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) {
+        // a sequence that fits the smallest share and stands alone is never cut
+        if (e != hipSuccess || (a.batch.batch == 1 && a.batch.max_pages << a.pool.shift <= kLeast << shift)) {
             return e;
         }
-        hipLaunchKernelGGL((paged_join_kernel<ACT, DIM>), dim3(a.heads, a.batch.batch), dim3(256), 0, st, a, per_head);
+        hipLaunchKernelGGL((paged_join_kernel<ACT, DIM>), dim3(a.heads, a.batch.batch), dim3(256), 0, st, a, shares, shift);
         return hipGetLastError();
     }
 };
@@ -487,7 +506,7 @@ struct Decode {
 
 size_t paged_decode_workspace(const PagedPool &pool, uint32_t heads)
 {
-    return (size_t)columns(heads, pool.kv_heads) * 2 * chunks_per_head(heads, pool.kv_heads) * 16 * (pool.dim + 2) * sizeof(float);
+    return (size_t)columns(heads, pool.kv_heads) * shares_of(heads, pool.kv_heads, pool.dim) * 2 * 16 * (pool.dim + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_decode(const PagedAttentionArgs &a, hipStream_t st)

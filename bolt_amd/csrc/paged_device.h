@@ -126,24 +126,25 @@ struct Words<4> {
     uint32_t w[4];
 };
 
+// (read once: past the caches. A 2 GiB read goes at 7.0 TB/s so, at 6.2 through them.)
 template <int W>
 __device__ __forceinline__ Words<W> load_words(const void *p)
 {
     Words<W> r;
     if (W == 4) {
-        const v4u v = *(const v4u *)p;
+        const v4u v = __builtin_nontemporal_load((const v4u *)p);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             r.w[i] = v[i];
         }
     } else if (W == 2) {
-        const v2u v = *(const v2u *)p;
+        const v2u v = __builtin_nontemporal_load((const v2u *)p);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             r.w[i] = v[i];
         }
     } else {
-        r.w[0] = *(const uint32_t *)p;
+        r.w[0] = __builtin_nontemporal_load((const uint32_t *)p);
     }
     return r;
 }

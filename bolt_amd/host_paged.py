@@ -41,6 +41,7 @@ class PagedKvCache:
         self.keep = (k, v, k_scale, v_scale)
         self.device = _one_device(*self.keep)
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.scale = 1.0 / math.sqrt(self.head_dim)
         self.struct = BoltPagedKvCache(DT_OF[k.dtype], self.pages, self.page_size, self.kv_heads, self.head_dim, k.data_ptr(), v.data_ptr(),
                                        None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr())
         self.ref = C.byref(self.struct)
@@ -85,38 +86,48 @@ def _one_device(*tensors):
     return next(iter(found))
 
 
-def _rows(t, name, batch, heads, dim, dtype, device):
-    """Checks rows of heads, [rows, heads, dim] with dense heads; returns the elements between rows."""
-    _want(t.shape == (batch.rows, heads, dim), "%s: [%d, %d, %d]" % (name, batch.rows, heads, dim))
-    _want(t.dtype == dtype and t.device == device, "%s: %s on %s" % (name, dtype, device))
+def _rows(t, name, shape, dtype, device):
+    """Checks rows of heads, [rows, heads, dim] with dense heads; returns the elements between rows. (On the path of every call:
+    no message is made before it is needed.)"""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise BoltError("%s: %s %s on %s, not %s %s on %s" % (name, list(shape), dtype, device, list(t.shape), t.dtype, t.device))
     s = t.stride()
-    _want(s[2] == 1 and (s[1] == dim or heads == 1), "%s: the heads of a row are dense" % name)
-    return s[0] if batch.rows > 1 else max(s[0], heads * dim)
+    if s[2] != 1 or (s[1] != shape[2] and shape[1] != 1):
+        raise BoltError("%s: the heads of a row are dense" % name)
+    return s[0] if shape[0] > 1 else max(s[0], shape[1] * shape[2])
 
 
 def _here(cache, batch):
-    _want(cache.device == batch.device and cache.device.index == torch.cuda.current_device(),
-          "cache and batch belong to the current GPU")
+    if cache.device != batch.device or cache.device.index != torch.cuda.current_device():
+        raise BoltError("cache and batch belong to the current GPU")
 
 
 def kv_cache_append(cache, batch, k, v, q=None, rotary=None, q_out=None):
     """k, v: [rows, kv_heads, head_dim], q: [rows, heads, head_dim], rows any number of elements apart. Returns q_out, the
     rotated queries (None without q). Rows that belong to no sequence are left as they are in q_out."""
     _here(cache, batch)
-    _want(rotary is None or rotary.device == cache.device, "the angles are on the cache's GPU")
-    ks = _rows(k, "k", batch, cache.kv_heads, cache.head_dim, k.dtype, cache.device)
-    vs = _rows(v, "v", batch, cache.kv_heads, cache.head_dim, k.dtype, cache.device)
+    device, dtype, shape = cache.device, k.dtype, (batch.rows, cache.kv_heads, cache.head_dim)
+    if rotary is not None and rotary.device != device:
+        raise BoltError("the angles are on the cache's GPU")
+    dt = DT_OF.get(dtype)
+    if dt is None:
+        raise BoltError("float32, float16 or bfloat16 rows")
+    ks, vs = _rows(k, "k", shape, dtype, device), _rows(v, "v", shape, dtype, device)
     heads, qs, qo, qp, qop = 0, 0, 0, None, None
     if q is not None:
         heads = q.shape[1]
+        shape = (shape[0], heads, shape[2])
+        qs = _rows(q, "q", shape, dtype, device)
         if q_out is None:
-            q_out = torch.empty((batch.rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
-        qs = _rows(q, "q", batch, heads, cache.head_dim, k.dtype, cache.device)
-        qo = _rows(q_out, "q_out", batch, heads, cache.head_dim, k.dtype, cache.device)
+            q_out = torch.empty(shape, dtype=dtype, device=device)
+            qo = heads * shape[2]
+        else:
+            qo = _rows(q_out, "q_out", shape, dtype, device)
         qp, qop = q.data_ptr(), q_out.data_ptr()
-    _want(k.dtype in DT_OF, "float32, float16 or bfloat16 rows")
-    check(lib().bolt_gfx950_kv_cache_append(cache.ref, batch.ref, DT_OF[k.dtype], k.data_ptr(), ks, v.data_ptr(), vs, heads, qp, qs, qop, qo,
-                                            None if rotary is None else rotary.ref), "kv_cache_append")
+    code = lib().bolt_gfx950_kv_cache_append(cache.ref, batch.ref, dt, k.data_ptr(), ks, v.data_ptr(), vs, heads, qp, qs, qop, qo,
+                                             None if rotary is None else rotary.ref)
+    if code:
+        check(code, "kv_cache_append")
     return q_out
 
 
@@ -129,17 +140,25 @@ def paged_attention_workspace(cache, batch, heads):
 
 def _attention(fn, what, cache, batch, q, out, scale, window, workspace):
     _here(cache, batch)
-    _want(q.dim() == 3 and q.dtype in DT_OF, "q: [rows, heads, head_dim] of float32, float16 or bfloat16")
+    device, dtype = cache.device, q.dtype
+    dt = DT_OF.get(dtype)
+    if dt is None or q.dim() != 3:
+        raise BoltError("q: [rows, heads, head_dim] of float32, float16 or bfloat16")
     heads = q.shape[1]
+    shape = (batch.rows, heads, cache.head_dim)
+    qs = _rows(q, "q", shape, dtype, device)
     if workspace is None:
         workspace = paged_attention_workspace(cache, batch, heads)
+    elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+        raise BoltError("workspace: contiguous uint8 on the cache's GPU")
     if out is None:
-        out = torch.empty((batch.rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
-    qs = _rows(q, "q", batch, heads, cache.head_dim, q.dtype, cache.device)
-    os = _rows(out, "out", batch, heads, cache.head_dim, q.dtype, cache.device)
-    _want(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == cache.device, "workspace: contiguous uint8 on the cache's GPU")
-    check(fn(cache.ref, batch.ref, DT_OF[q.dtype], heads, q.data_ptr(), qs, out.data_ptr(), os,
-             1.0 / math.sqrt(cache.head_dim) if scale is None else scale, window, workspace.data_ptr(), workspace.numel()), what)
+        out, os = torch.empty(shape, dtype=dtype, device=device), heads * shape[2]
+    else:
+        os = _rows(out, "out", shape, dtype, device)
+    code = fn(cache.ref, batch.ref, dt, heads, q.data_ptr(), qs, out.data_ptr(), os, cache.scale if scale is None else scale, window,
+              workspace.data_ptr(), workspace.numel())
+    if code:
+        check(code, what)
     return out
 
 
