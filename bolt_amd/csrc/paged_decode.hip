@@ -38,15 +38,6 @@ constexpr uint32_t per_cu()
 constexpr float kLow = -1.7e38f;     // running maximum before the first key
 constexpr float kSlack = 2.0f, kLift = 13.0f;  // see above: 2^(kSlack + kLift) fits fp16
 
-__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v)
-{
-#pragma unroll
-    for (int off = 32; off; off >>= 1) {
-        v += __shfl_xor(v, off, 64);
-    }
-    return v;
-}
-
 __device__ __forceinline__ PagedSpan span_of(const PagedAttentionArgs &a, uint32_t b)
 {
     return paged_span((int64_t)a.batch.lens[b] - 1, a.window, a.batch.max_pages << a.pool.shift);
@@ -62,38 +53,10 @@ __device__ __forceinline__ uint32_t tiles_of(const PagedAttentionArgs &a, uint32
 }
 
 // tiles per share, with `shares` of them to a key head's column
-__device__ __forceinline__ uint32_t tiles_per_share(const PagedAttentionArgs &a, uint32_t shares, uint32_t shift, uint32_t lane)
+__device__ __forceinline__ uint32_t tiles_per_share(uint32_t tiles, uint32_t shares)
 {
-    uint32_t sum = 0;
-    for (uint32_t b = lane; b < a.batch.batch; b += 64) {
-        sum += tiles_of(a, b, shift);
-    }
-    const uint32_t per = (wave_sum_u32(sum) + shares - 1) / shares;
+    const uint32_t per = (tiles + shares - 1) / shares;
     return per < kLeast ? kLeast : per;
-}
-
-// The sequence that tile number `tile` belongs to, and the tiles before it (false: behind the last). Every wave finds out by itself.
-__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t tile, uint32_t shift, uint32_t lane, uint32_t *b_out, uint32_t *before)
-{
-    uint32_t base = 0;
-    for (uint32_t b0 = 0; b0 < a.batch.batch; b0 += 64) {
-        const uint32_t n = b0 + lane < a.batch.batch ? tiles_of(a, b0 + lane, shift) : 0;
-        uint32_t upto = n;
-#pragma unroll
-        for (uint32_t off = 1; off < 64; off <<= 1) {
-            const uint32_t v = __shfl_up(upto, off, 64);
-            upto += lane >= off ? v : 0;
-        }
-        const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
-        if (tile < base + all) {
-            const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(base + upto > tile));
-            *b_out = b0 + at;
-            *before = base + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at);
-            return true;
-        }
-        base += all;
-    }
-    return false;
 }
 
 // A part: 16 rows of DIM values, 16 maxima, 16 sums. A share leaves two at most: of the sequence that its first tile belongs to
@@ -129,15 +92,17 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
 
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 15, g = lane >> 4;
-    const uint32_t per = tiles_per_share(a, shares, shift, lane);
+    auto tiles = [&](uint32_t i) { return tiles_of(a, i, shift); };
+    const Places all = places_of(a.batch.batch, lane, tiles);
+    const uint32_t per = tiles_per_share(all.sum, shares);
     const uint32_t share = blockIdx.x, group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
     const uint32_t kvh = blockIdx.y / qtiles, q0 = blockIdx.y % qtiles * 16;
     const uint32_t nq = group - q0 < 16 ? group - q0 : 16;
-    uint32_t b, before;
-    if ((uint64_t)share * per > 0xffffffffu || !find_tile(a, share * per, shift, lane, &b, &before)) {
+    if ((uint64_t)share * per >= all.sum) {
         return;
     }
-    uint32_t tile = share * per;  // next tile of the row
+    uint32_t tile = share * per, before;  // next tile of the row; those in front of its sequence
+    uint32_t b = entry_at(all, a.batch.batch, lane, tile, tiles, &before);
     const uint32_t end = tile + per;
     for (;;) {
         b = __builtin_amdgcn_readfirstlane(b);
@@ -400,13 +365,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionArgs a, u
     __shared__ __attribute__((aligned(16))) float sO[kWays][DIM];
     __shared__ float sL[kWays], sM[kWays];
     const uint32_t lane = threadIdx.x & 63, h = blockIdx.x, b = blockIdx.y;
-    const uint32_t per = tiles_per_share(a, shares, shift, lane);
-    uint32_t before = 0;
-    for (uint32_t i = lane; i < b; i += 64) {
-        before += tiles_of(a, i, shift);
+    auto tiles = [&](uint32_t i) { return tiles_of(a, i, shift); };
+    const Places all = places_of(a.batch.batch, lane, tiles);
+    const uint32_t per = tiles_per_share(all.sum, shares);
+    uint32_t before = 0, mine = 0;  // tiles in front of sequence b, its own
+    if (b < 64) {
+        mine = __builtin_amdgcn_readlane(all.first, b);
+        before = __builtin_amdgcn_readlane(all.upto, b) - mine;
+    } else {
+        mine = tiles(b);
+        before = places_of(b, lane, tiles).sum;
     }
-    before = wave_sum_u32(before);
-    const uint32_t first = before / per, count = (before + tiles_of(a, b, shift) - 1) / per - first + 1;
+    const uint32_t first = before / per, count = (before + mine - 1) / per - first + 1;
     if (count == 1) {
         return;
     }

@@ -75,6 +75,60 @@ __device__ __forceinline__ void store8(void *p, size_t at, const float *x)
     }
 }
 
+// ---- sums over a wave ---------------------------------------------------------------------------------
+// Inclusive sums over the 64 lanes, on the vector unit alone (rows of 16, then 15 -> 16.., 31 -> 32..)
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v)
+{
+#define BG_SCAN_STEP(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false)
+    BG_SCAN_STEP(0x111, 0xf);  // row_shr:1
+    BG_SCAN_STEP(0x112, 0xf);
+    BG_SCAN_STEP(0x114, 0xf);
+    BG_SCAN_STEP(0x118, 0xf);
+    BG_SCAN_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    BG_SCAN_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef BG_SCAN_STEP
+    return v;
+}
+
+// A list of n counts, count(i), laid end to end: which entry place x falls into. Every wave finds out by itself. The first 64
+// counts are asked for once.
+struct Places {
+    uint32_t first, upto, sum;  // this lane's of the first 64 counts, the sum up to it, the sum of all
+};
+
+template <typename F>
+__device__ __forceinline__ Places places_of(uint32_t n, uint32_t lane, F count)
+{
+    Places p;
+    p.first = lane < n ? count(lane) : 0;
+    p.upto = wave_scan_u32(p.first);
+    p.sum = __builtin_amdgcn_readlane(p.upto, 63);
+    for (uint32_t i0 = 64; i0 < n; i0 += 64) {
+        p.sum += __builtin_amdgcn_readlane(wave_scan_u32(i0 + lane < n ? count(i0 + lane) : 0), 63);
+    }
+    return p;
+}
+
+// x < p.sum; *before: the places in front of the entry
+template <typename F>
+__device__ __forceinline__ uint32_t entry_at(const Places &p, uint32_t n, uint32_t lane, uint32_t x, F count, uint32_t *before)
+{
+    uint32_t base = 0, c = p.first, upto = p.upto;
+    for (uint32_t i0 = 0;;) {
+        const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
+        if (x < base + all || i0 + 64 >= n) {
+            const unsigned long long behind = __ballot(base + upto > x);
+            const uint32_t at = behind ? (uint32_t)__builtin_ctzll(behind) : 63;
+            *before = base + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(c, at);
+            return min(i0 + at, n - 1);
+        }
+        base += all;
+        i0 += 64;
+        c = i0 + lane < n ? count(i0 + lane) : 0;
+        upto = wave_scan_u32(c);
+    }
+}
+
 // ---- operands of the matrix instructions ------------------------------------------------------------
 // A 32-deep 16-bit operand: lane (i = lane % 16, g = lane / 16) holds eight contraction elements of row (column) i. Which
 // eight of a head's DIM values step s of lane group g means is free as long as both operands agree (d_of): an int8 lane

@@ -32,58 +32,25 @@ constexpr uint32_t kLeast = 4;     // fewest key tiles per share
 constexpr float kLow = -1.7e38f;
 constexpr float kSlack = 2.0f, kLift = 13.0f;
 
-struct Tile {
-    uint32_t b, index;
-};
-
-__device__ __forceinline__ uint32_t row_tiles(const PagedAttentionArgs &a, uint32_t b, uint32_t group)
+// rows (token, head) of a sequence in tiles of kRows; no more tokens than the buffers have rows, so that it all fits 31 bits
+__device__ __forceinline__ uint32_t rows_of(const PagedAttentionArgs &a, const PagedSeq &s, uint32_t group)
 {
-    const PagedSeq s = paged_seq(a.batch, b);
-    const uint64_t n = s.count < (int64_t)a.batch.rows ? (uint64_t)s.count : a.batch.rows;
-    return (uint32_t)((n * group + kRows - 1) / kRows);
+    return (s.count < (int64_t)a.batch.rows ? (uint32_t)s.count : a.batch.rows) * group;
 }
 
-__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v)
+// Row tile number x of the launch: its sequence and its number there. Counted from the last one: the later tiles of a sequence
+// see the most keys and start first.
+__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t group, uint32_t x, uint32_t lane, uint32_t *b, uint32_t *tile)
 {
-#pragma unroll
-    for (int off = 32; off; off >>= 1) {
-        v += __shfl_xor(v, off, 64);
-    }
-    return v;
-}
-
-// Row tile number x of the launch, counted from the last one: the later tiles of a sequence see the most keys and start
-// first. Every wave finds out by itself.
-__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t group, uint32_t x, uint32_t lane, Tile *out)
-{
-    uint32_t all = 0;
-    for (uint32_t b = lane; b < a.batch.batch; b += 64) {
-        all += row_tiles(a, b, group);
-    }
-    all = wave_sum_u32(all);
-    if (x >= all) {
+    auto count = [&](uint32_t i) { return (rows_of(a, paged_seq(a.batch, i), group) + kRows - 1) / kRows; };
+    const Places all = places_of(a.batch.batch, lane, count);
+    if (x >= all.sum) {
         return false;
     }
-    x = all - 1 - x;
-    uint32_t base = 0;
-    for (uint32_t b0 = 0; b0 < a.batch.batch; b0 += 64) {
-        const uint32_t n = b0 + lane < a.batch.batch ? row_tiles(a, b0 + lane, group) : 0;
-        uint32_t upto = n;
-#pragma unroll
-        for (uint32_t off = 1; off < 64; off <<= 1) {
-            const uint32_t v = __shfl_up(upto, off, 64);
-            upto += lane >= off ? v : 0;
-        }
-        const uint32_t sum = __builtin_amdgcn_readlane(upto, 63);
-        if (x < base + sum) {
-            const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(base + upto > x));
-            out->b = b0 + at;
-            out->index = x - base - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
-            return true;
-        }
-        base += sum;
-    }
-    return false;
+    uint32_t before;
+    *b = entry_at(all, a.batch.batch, lane, all.sum - 1 - x, count, &before);
+    *tile = all.sum - 1 - x - before;
+    return true;
 }
 
 // What a tile's rows see: positions of the first and last row, keys [lo, hi) with lo rounded down to a tile
@@ -92,10 +59,10 @@ struct Reach {
     uint32_t lo, hi, tiles;
 };
 
-__device__ __forceinline__ Reach reach_of(const PagedAttentionArgs &a, const PagedSeq &s, uint32_t tile, uint32_t group)
+__device__ __forceinline__ Reach reach_of(const PagedAttentionArgs &a, const PagedSeq &s, uint32_t rows, uint32_t tile, uint32_t group)
 {
     Reach r;
-    const int64_t rows = s.count * group, r0 = (int64_t)tile * kRows, r1 = r0 + kRows < rows ? r0 + kRows : rows;
+    const uint32_t r0 = tile * kRows, r1 = min(r0 + kRows, rows);
     r.first = s.pos + r0 / group;
     r.last = s.pos + (r1 - 1) / group;
     const uint32_t capacity = a.batch.max_pages << a.pool.shift;
@@ -231,14 +198,15 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     const uint32_t c = lane & 31, h = lane >> 5;
     const uint32_t kvh = blockIdx.x % a.pool.kv_heads, share = blockIdx.x / a.pool.kv_heads % shares, x = blockIdx.x / a.pool.kv_heads / shares;
     const uint32_t group = a.heads / a.pool.kv_heads;
-    Tile tile;
-    if (!find_tile(a, group, x, lane, &tile)) {
+    uint32_t b, tile_index;
+    if (!find_tile(a, group, x, lane, &b, &tile_index)) {
         return;
     }
-    const uint32_t b = __builtin_amdgcn_readfirstlane(tile.b);
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile_index = __builtin_amdgcn_readfirstlane(tile_index);
     const PagedSeq seq = paged_seq(a.batch, b);
-    const uint32_t tile_index = __builtin_amdgcn_readfirstlane(tile.index);
-    const Reach all = reach_of(a, seq, tile_index, group);
+    const uint32_t rows = rows_of(a, seq, group);
+    const Reach all = reach_of(a, seq, rows, tile_index, group);
     const uint32_t per = tiles_per_share(all.tiles, shares);
     const uint32_t t0 = share * per, t1 = min(t0 + per, all.tiles);
     if (share && t0 >= all.tiles) {
@@ -248,10 +216,10 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
 
     // this lane's row
-    const int64_t r = (int64_t)tile_index * kRows + 32 * wave + c, token = r / group;
+    const uint32_t r = tile_index * kRows + 32 * wave + c, token = r / group;
     const int64_t row = seq.first + token, pos = seq.pos + token;
-    const bool mine = r < seq.count * group && row >= 0 && row < (int64_t)a.batch.rows;
-    const uint32_t head = kvh * group + (uint32_t)(r % group);
+    const bool mine = r < rows && row >= 0 && row < (int64_t)a.batch.rows;
+    const uint32_t head = kvh * group + (r - token * group);
     const PagedSpan span = paged_span(mine ? pos : -1, a.window, all.hi);
 
     const uint32_t all_hi = paged_span(all.first, 0, all.hi).hi, all_lo = paged_span(all.last, a.window, all.hi).lo;  // seen by every row
@@ -259,41 +227,6 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     V qh[kSteps], ql[kWide ? kSteps : 1];
     const float score_scale = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);  // (int8: part of the keys' steps)
     float xscale = CT == PT_I8 ? 1.0f : score_scale;                      // the factor of the scores, positive
-    {
-        const float sign = a.scale2 == 0.0f ? 0.0f : a.scale2 < 0.0f ? -1.0f : 1.0f;
-        const size_t at = (size_t)(mine ? row : 0) * a.qstride + (size_t)(mine ? head : 0) * DIM + 8 * h;
-        float top = 0.0f, up = 1.0f;
-        if (kShiftQ) {
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                float v[8];
-                load8<ACT>(a.q, at + 16 * s, v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    top = fmaxf(top, fabsf(v[j]));
-                }
-            }
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            int e = 0;
-            up = shift_into_f16(top, &e);
-            xscale = ldexpf(xscale, e);
-            xscale = xscale < 1.17549435e-38f ? 1.17549435e-38f : xscale;  // not zero: it meets scores of -inf
-        }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            float v[8];
-            load8<ACT>(a.q, at + 16 * s, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] *= sign;
-            }
-            V lo;
-            Operand<CT>::split(v, up, &qh[s], &lo);
-            if (kWide) {
-                ql[s] = lo;
-            }
-        }
-    }
 
     v16f o[kOut];
 #pragma unroll
@@ -427,6 +360,43 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         next = look_up(k0 + kKeys);
         fetch(k0, pages, CT == PT_I8 ? sTiles + 2 * kTileBytes : sTiles);
     }
+    // queries (while the first tile is on its way)
+    {
+        const float sign = a.scale2 == 0.0f ? 0.0f : a.scale2 < 0.0f ? -1.0f : 1.0f;
+        const size_t at = (size_t)(mine ? row : 0) * a.qstride + (size_t)(mine ? head : 0) * DIM + 8 * h;
+        float top = 0.0f, up = 1.0f;
+        if (kShiftQ) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                float v[8];
+                load8<ACT>(a.q, at + 16 * s, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    top = fmaxf(top, fabsf(v[j]));
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            int e = 0;
+            up = shift_into_f16(top, &e);
+            xscale = ldexpf(xscale, e);
+            xscale = xscale < 1.17549435e-38f ? 1.17549435e-38f : xscale;  // not zero: it meets scores of -inf
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            float v[8];
+            load8<ACT>(a.q, at + 16 * s, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] *= sign;
+            }
+            V lo;
+            Operand<CT>::split(v, up, &qh[s], &lo);
+            if (kWide) {
+                ql[s] = lo;
+            }
+        }
+    }
+
     // One tile: `now` holds it, `ahead` is where the next one goes (int8: where this one lies as it is stored, too). (The compiler has to know that the two are apart, else it waits
     // for the next tile's arrival before it reads this one.)
     auto step_over = [&](uint32_t t, __attribute__((address_space(3))) uint8_t *__restrict now,
@@ -723,20 +693,22 @@ __global__ __launch_bounds__(8 * DIM / 4) void paged_prompt_join_kernel(PagedAtt
 {
     const uint32_t lane = threadIdx.x & 63, kvh = blockIdx.x % a.pool.kv_heads, x = blockIdx.x / a.pool.kv_heads;
     const uint32_t group = a.heads / a.pool.kv_heads;
-    Tile tile;
-    if (!find_tile(a, group, x, lane, &tile)) {
+    uint32_t b, tile_index;
+    if (!find_tile(a, group, x, lane, &b, &tile_index)) {
         return;
     }
-    const PagedSeq seq = paged_seq(a.batch, tile.b);
-    const Reach all = reach_of(a, seq, tile.index, group);
+    const PagedSeq seq = paged_seq(a.batch, b);
+    const uint32_t rows = rows_of(a, seq, group);
+    const Reach all = reach_of(a, seq, rows, tile_index, group);
     const uint32_t per = tiles_per_share(all.tiles, shares);
     if (per >= all.tiles) {
         return;
     }
     const uint32_t count = (all.tiles + per - 1) / per;
     const uint32_t pr = blockIdx.y * 8 + threadIdx.x / (DIM / 4), d = threadIdx.x % (DIM / 4) * 4;
-    const int64_t r = (int64_t)tile.index * kRows + pr, row = seq.first + r / group;
-    if (r >= seq.count * group || row < 0 || row >= (int64_t)a.batch.rows) {
+    const uint32_t r = tile_index * kRows + pr;
+    const int64_t row = seq.first + r / group;
+    if (r >= rows || row < 0 || row >= (int64_t)a.batch.rows) {
         return;
     }
     float top = kLow, sum = 0.0f;
