@@ -38,17 +38,31 @@ __device__ __forceinline__ uint32_t rows_of(const PagedAttentionArgs &a, const P
     return (s.count < (int64_t)a.batch.rows ? (uint32_t)s.count : a.batch.rows) * group;
 }
 
-// Row tile number x of the launch: its sequence and its number there. Counted from the last one: the later tiles of a sequence
-// see the most keys and start first.
+// Row tile number x of the launch: its sequence and its number there. What takes longest starts first: the longest sequence
+// (of up to 64, of more the last one), and of a sequence the last tile, which sees the most keys.
 __device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t group, uint32_t x, uint32_t lane, uint32_t *b, uint32_t *tile)
 {
     auto count = [&](uint32_t i) { return (rows_of(a, paged_seq(a.batch, i), group) + kRows - 1) / kRows; };
-    const Places all = places_of(a.batch.batch, lane, count);
+    const uint32_t n = a.batch.batch;
+    const Places all = places_of(n, lane, count);
     if (x >= all.sum) {
         return false;
     }
+    if (n <= 64) {
+        const int32_t keys = lane < n ? a.batch.lens[lane] : -0x7fffffff - 1;
+        uint32_t before = 0;  // tiles of longer sequences, and of those in front that are as long
+        for (uint32_t i = 0; i < n; ++i) {
+            const int32_t other = __builtin_amdgcn_readlane(keys, i);
+            before += other > keys || (other == keys && i < lane) ? (uint32_t)__builtin_amdgcn_readlane(all.first, i) : 0;
+        }
+        const unsigned long long here = __ballot(x >= before && x - before < all.first);
+        const uint32_t at = here ? (uint32_t)__builtin_ctzll(here) : 0;
+        *b = at;
+        *tile = __builtin_amdgcn_readlane(all.first, at) - 1 - (x - __builtin_amdgcn_readlane(before, at));
+        return here != 0;
+    }
     uint32_t before;
-    *b = entry_at(all, a.batch.batch, lane, all.sum - 1 - x, count, &before);
+    *b = entry_at(all, n, lane, all.sum - 1 - x, count, &before);
     *tile = all.sum - 1 - x - before;
     return true;
 }
