@@ -22,15 +22,18 @@ struct PagedSeq {
     int64_t first, count, pos;
 };
 
-BG_HD inline PagedSeq paged_seq(const PagedBatch &a, uint32_t b)
+BG_HD inline PagedSeq paged_seq_from(int32_t first, int64_t next, int32_t len)
 {
     PagedSeq s;
-    s.first = a.offsets ? a.offsets[b] : (int64_t)b;
-    const int64_t next = a.offsets ? a.offsets[b + 1] : (int64_t)b + 1;
+    s.first = first;
     s.count = next > s.first ? next - s.first : 0;
-    const int64_t len = a.lens[b];
     s.pos = (len > 0 ? len : 0) - s.count;
     return s;
+}
+
+BG_HD inline PagedSeq paged_seq(const PagedBatch &a, uint32_t b)
+{
+    return a.offsets ? paged_seq_from(a.offsets[b], a.offsets[b + 1], a.lens[b]) : paged_seq_from((int32_t)b, (int64_t)b + 1, a.lens[b]);
 }
 
 // The sequence that owns a packed row: the last b with offsets[b] <= row (offsets ascend); the caller checks that the row

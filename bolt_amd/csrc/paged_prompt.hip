@@ -40,30 +40,35 @@ __device__ __forceinline__ uint32_t rows_of(const PagedAttentionArgs &a, const P
 
 // Row tile number x of the launch: its sequence and its number there. What takes longest starts first: the longest sequence
 // (of up to 64, of more the last one), and of a sequence the last tile, which sees the most keys.
-__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t group, uint32_t x, uint32_t lane, uint32_t *b, uint32_t *tile)
+__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t group, uint32_t x, uint32_t lane, uint32_t *b_out, uint32_t *tile, PagedSeq *seq)
 {
-    auto count = [&](uint32_t i) { return (rows_of(a, paged_seq(a.batch, i), group) + kRows - 1) / kRows; };
     const uint32_t n = a.batch.batch;
+    if (n <= 64) {  // everything that is needed is asked for at once
+        const uint32_t mine = lane < n ? lane : n - 1;
+        const int32_t first = a.batch.offsets[mine], next = a.batch.offsets[mine + 1], keys = lane < n ? a.batch.lens[mine] : -0x7fffffff - 1;
+        const uint32_t tiles = lane < n ? (rows_of(a, paged_seq_from(first, next, keys), group) + kRows - 1) / kRows : 0;
+        uint32_t before = 0;  // tiles of longer sequences, and of those in front that are as long
+        for (uint32_t i = 0; i < n; ++i) {
+            const int32_t other = __builtin_amdgcn_readlane(keys, i);
+            before += other > keys || (other == keys && i < lane) ? (uint32_t)__builtin_amdgcn_readlane(tiles, i) : 0;
+        }
+        const unsigned long long here = __ballot(x >= before && x - before < tiles);
+        const uint32_t at = here ? (uint32_t)__builtin_ctzll(here) : 0;
+        *b_out = at;
+        *tile = __builtin_amdgcn_readlane(tiles, at) - 1 - (x - __builtin_amdgcn_readlane(before, at));
+        *seq = paged_seq_from(__builtin_amdgcn_readlane(first, at), __builtin_amdgcn_readlane(next, at), __builtin_amdgcn_readlane(keys, at));
+        return here != 0;
+    }
+    auto count = [&](uint32_t i) { return (rows_of(a, paged_seq(a.batch, i), group) + kRows - 1) / kRows; };
     const Places all = places_of(n, lane, count);
     if (x >= all.sum) {
         return false;
     }
-    if (n <= 64) {
-        const int32_t keys = lane < n ? a.batch.lens[lane] : -0x7fffffff - 1;
-        uint32_t before = 0;  // tiles of longer sequences, and of those in front that are as long
-        for (uint32_t i = 0; i < n; ++i) {
-            const int32_t other = __builtin_amdgcn_readlane(keys, i);
-            before += other > keys || (other == keys && i < lane) ? (uint32_t)__builtin_amdgcn_readlane(all.first, i) : 0;
-        }
-        const unsigned long long here = __ballot(x >= before && x - before < all.first);
-        const uint32_t at = here ? (uint32_t)__builtin_ctzll(here) : 0;
-        *b = at;
-        *tile = __builtin_amdgcn_readlane(all.first, at) - 1 - (x - __builtin_amdgcn_readlane(before, at));
-        return here != 0;
-    }
     uint32_t before;
-    *b = entry_at(all, n, lane, all.sum - 1 - x, count, &before);
-    *tile = all.sum - 1 - x - before;
+    const uint32_t b = __builtin_amdgcn_readfirstlane(entry_at(all, n, lane, all.sum - 1 - x, count, &before));
+    *b_out = b;
+    *tile = __builtin_amdgcn_readfirstlane(all.sum - 1 - x - before);
+    *seq = paged_seq(a.batch, b);
     return true;
 }
 
@@ -213,12 +218,10 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     const uint32_t kvh = blockIdx.x % a.pool.kv_heads, share = blockIdx.x / a.pool.kv_heads % shares, x = blockIdx.x / a.pool.kv_heads / shares;
     const uint32_t group = a.heads / a.pool.kv_heads;
     uint32_t b, tile_index;
-    if (!find_tile(a, group, x, lane, &b, &tile_index)) {
+    PagedSeq seq;
+    if (!find_tile(a, group, x, lane, &b, &tile_index, &seq)) {
         return;
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    tile_index = __builtin_amdgcn_readfirstlane(tile_index);
-    const PagedSeq seq = paged_seq(a.batch, b);
     const uint32_t rows = rows_of(a, seq, group);
     const Reach all = reach_of(a, seq, rows, tile_index, group);
     const uint32_t per = tiles_per_share(all.tiles, shares);
@@ -435,10 +438,18 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         if (CT != PT_I8 && !whole) {
             constexpr uint32_t kExp = CT == PT_BF16 ? 0x7f80u : 0x7c00u;
             lds_t const base = now + kTileBytes;
+            v4u w[kTileBytes / 16 / 256];
+#pragma unroll
+            for (uint32_t n = 0; n < kTileBytes / 16 / 256; ++n) {
+                w[n] = *(const __attribute__((address_space(3))) v4u *)(base + (n * 256 + tid) * 16);
+            }
             bool hit = false;
-            for (uint32_t at = tid; at < kTileBytes / 4; at += 256) {
-                const uint32_t w = *(const __attribute__((address_space(3))) uint32_t *)(base + at * 4);
-                hit |= (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
+#pragma unroll
+            for (uint32_t n = 0; n < kTileBytes / 16 / 256; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    hit |= (w[n][i] & kExp) == kExp || (w[n][i] >> 16 & kExp) == kExp;
+                }
             }
             hit = __any(hit);
             if (lane == 0) {
@@ -468,9 +479,6 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 }
                 __syncthreads();
             }
-        }
-        if (CT != PT_I8 && !__any(span.hi > k0 && span.lo < k0 + kKeys)) {
-            return;  // nothing for this wave (int8: gone through all the same, the way round it cost a copy of every output register)
         }
         // Scores. The order is written out (the compiler would wait for every read right behind it): six or eight reads ahead of the
         // products that use them.
@@ -708,10 +716,10 @@ __global__ __launch_bounds__(8 * DIM / 4) void paged_prompt_join_kernel(PagedAtt
     const uint32_t lane = threadIdx.x & 63, kvh = blockIdx.x % a.pool.kv_heads, x = blockIdx.x / a.pool.kv_heads;
     const uint32_t group = a.heads / a.pool.kv_heads;
     uint32_t b, tile_index;
-    if (!find_tile(a, group, x, lane, &b, &tile_index)) {
+    PagedSeq seq;
+    if (!find_tile(a, group, x, lane, &b, &tile_index, &seq)) {
         return;
     }
-    const PagedSeq seq = paged_seq(a.batch, b);
     const uint32_t rows = rows_of(a, seq, group);
     const Reach all = reach_of(a, seq, rows, tile_index, group);
     const uint32_t per = tiles_per_share(all.tiles, shares);
