@@ -32,7 +32,7 @@ constexpr uint32_t kLeast = 1;       // fewest tiles in a share
 template <int DIM>
 constexpr uint32_t per_cu()
 {
-    return DIM == 128 ? 3 : 4;
+    return DIM == 128 ? 2 : 3;
 }
 
 constexpr float kLow = -1.7e38f;     // running maximum before the first key
@@ -79,6 +79,15 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, v4f v)
     }
 }
 
+// What a lane holds of a step's keys and values, as they are stored. Bit j of seen: key 16 (j / 4) + 4 g + j % 4 takes part.
+template <int CT, int DIM>
+struct Step {
+    typename CacheOperand<CT>::Raw kr[2][CacheOperand<CT>::kRawK(DIM)];
+    typename CacheOperand<CT>::template RawV<DIM> vr[8];
+    v4f ksc[2], vsc[2];
+    uint32_t seen;
+};
+
 // PAGE16: pages of 16 keys and more, so that each 16-key half of a step lies in one page and its address is the wave's.
 template <int ACT, int CT, int DIM, bool PAGE16>
 __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedAttentionArgs a, uint32_t shares, uint32_t shift)
@@ -119,21 +128,18 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
         float xscale = a.scale2;
         {
             float x[kSteps][8];
-            const size_t at = (size_t)b * a.qstride + (size_t)(kvh * group + q0 + c) * DIM;
+            const size_t at = (size_t)b * a.qstride + (size_t)(kvh * group + q0 + min(c, nq - 1)) * DIM;  // (columns behind the group: zeros)
             float top = 0.0f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                if (c < nq) {
-                    load8<ACT>(a.q, at + Op::d_of(s, g), x[s]);
-                } else {
+                load8<ACT>(a.q, at + Op::d_of(s, g), x[s]);
+            }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        x[s][j] = 0.0f;
-                    }
-                }
-                if (kShiftQ) {
+            for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < 8; ++j) {
+                    x[s][j] = c < nq ? x[s][j] : 0.0f;
+                    if (kShiftQ) {
                         top = fmaxf(top, fabsf(x[s][j]));
                     }
                 }
@@ -159,44 +165,55 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
         }
         float m = kLow, l = 0.0f, unit = CT == PT_I8 ? kFirstUnit : 1.0f;  // unit: the power of two that o's int8 steps are divided by
 
-        for (uint32_t k0 = from + 32 * wave; k0 < to; k0 += 128) {
-            typename Op::Raw kr[2][Op::kRawK(DIM)];
-            typename Op::template RawV<DIM> vr[8];
-            v4f ksc[2], vsc[2];
-            uint32_t seen = 0xff;  // bit j: key 16 (j / 4) + 4g + j % 4 of the step takes part
+        // One step's 32 keys: list entries of its two halves a step ahead of its loads, those ahead of the arithmetic of the step before
+        struct Pages {
+            uint32_t p[2];
+        };
+        const uniform_list list = (uniform_list)table;
+        auto look_up = [&](uint32_t k0) -> Pages {
+            Pages r = {{0, 0}};
+            if (PAGE16) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    r.p[h] = (uint32_t)list[min(k0 + 16 * h, to - 1) >> a.pool.shift];
+                }
+            }
+            return r;
+        };
+        auto fetch = [&](uint32_t k0, const Pages &pages, Step<CT, DIM> &n) {
+            n.seen = 0xff;
             if (PAGE16) {
                 const uint8_t *kb[2], *vb[2];
                 bool whole = k0 >= span.lo && k0 + 32 <= to;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t key = k0 + 16 * h;
-                    int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
-                    if (slot < 0) {
-                        seen &= h ? 0x0f : 0xf0;
-                        whole = false;
-                        slot = 0;
-                    }
+                    const bool there = pages.p[h] < a.pool.pages && key < to;
+                    const uint32_t page = there ? pages.p[h] : 0, in = there ? key & ((1u << a.pool.shift) - 1) : 0;
+                    n.seen &= there ? 0xff : h ? 0x0f : 0xf0;
+                    whole &= there;
+                    const size_t slot = ((((size_t)page * a.pool.kv_heads + kvh) << a.pool.shift) | in);
                     kb[h] = (const uint8_t *)a.pool.k + slot * kRowBytes;
                     vb[h] = (const uint8_t *)a.pool.v + slot * kRowBytes;
                     if (CT == PT_I8) {
-                        ksc[h] = load_scales(a.pool.ks + slot + 4 * g);
-                        vsc[h] = load_scales(a.pool.vs + slot + 4 * g);
+                        n.ksc[h] = load_scales(a.pool.ks + slot + 4 * g);
+                        n.vsc[h] = load_scales(a.pool.vs + slot + 4 * g);
                     }
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    Op::load_k(kb[h] + c * kRowBytes, g, kr[h]);
+                    Op::load_k(kb[h] + c * kRowBytes, g, n.kr[h]);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    vr[j] = Op::template load_v<DIM>(vb[j >> 2] + (4 * g + (j & 3)) * kRowBytes, c);
+                    n.vr[j] = Op::template load_v<DIM>(vb[j >> 2] + (4 * g + (j & 3)) * kRowBytes, c);
                 }
                 if (!whole) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint32_t key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
                         if (key < span.lo || key >= to) {
-                            seen &= ~(1u << j);
+                            n.seen &= ~(1u << j);
                         }
                     }
                 }
@@ -205,30 +222,32 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t key = k0 + 16 * h + c;
                     int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
-                    Op::load_k((const uint8_t *)a.pool.k + (slot < 0 ? 0 : slot) * kRowBytes, g, kr[h]);
+                    Op::load_k((const uint8_t *)a.pool.k + (slot < 0 ? 0 : slot) * kRowBytes, g, n.kr[h]);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
                     int64_t slot = key >= span.lo && key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
                     if (slot < 0) {
-                        seen &= ~(1u << j);
+                        n.seen &= ~(1u << j);
                         slot = 0;
                     }
-                    vr[j] = Op::template load_v<DIM>((const uint8_t *)a.pool.v + slot * kRowBytes, c);
+                    n.vr[j] = Op::template load_v<DIM>((const uint8_t *)a.pool.v + slot * kRowBytes, c);
                     if (CT == PT_I8) {
-                        ksc[j >> 2][j & 3] = a.pool.ks[slot];
-                        vsc[j >> 2][j & 3] = a.pool.vs[slot];
+                        n.ksc[j >> 2][j & 3] = a.pool.ks[slot];
+                        n.vsc[j >> 2][j & 3] = a.pool.vs[slot];
                     }
                 }
             }
+        };
+        auto attend = [&](Step<CT, DIM> &n) {
             v4f s[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 s[h] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int t = 0; t < kSteps; ++t) {
-                    const typename Op::V kv = Op::k_operand(kr[h], t);
+                    const typename Op::V kv = Op::k_operand(n.kr[h], t);
                     s[h] = Op::mfma(kv, qh[t], s[h]);
                     if (kSplitQ) {
                         s[h] = Op::mfma(kv, ql[t], s[h]);
@@ -240,20 +259,20 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
             for (int j = 0; j < 8; ++j) {
                 float f = xscale;
                 if (CT == PT_I8) {
-                    f *= __builtin_amdgcn_rcpf(ksc[j >> 2][j & 3]);
-                    step[j] = __builtin_amdgcn_rcpf(vsc[j >> 2][j & 3]);
+                    f *= __builtin_amdgcn_rcpf(n.ksc[j >> 2][j & 3]);
+                    step[j] = __builtin_amdgcn_rcpf(n.vsc[j >> 2][j & 3]);
                 }
                 x[j] = s[j >> 2][j & 3] * f;
             }
-            if (seen != 0xff) {
+            if (n.seen != 0xff) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (!(seen >> j & 1)) {
+                    if (!(n.seen >> j & 1)) {
                         x[j] = -INFINITY;
                         if (CT == PT_I8) {
                             step[j] = 0.0f;
                         } else {
-                            vr[j] = Op::template zero_v<DIM>();
+                            n.vr[j] = Op::template zero_v<DIM>();
                         }
                     }
                 }
@@ -304,29 +323,57 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
             Op::split(p, 1.0f, &ph, &pl);
 #pragma unroll
             for (int t = 0; t < kVec; ++t) {
-                const typename Op::V vt = Op::template v_operand<DIM>(vr, t);
+                const typename Op::V vt = Op::template v_operand<DIM>(n.vr, t);
                 o[t] = Op::mfma(vt, ph, o[t]);
                 o[t] = Op::mfma(vt, pl, o[t]);
             }
+        };
+        uint32_t k0 = from + 32 * wave;
+        if (k0 < to) {
+            Step<CT, DIM> one, two;
+            Pages pages = look_up(k0);
+            fetch(k0, pages, one);
+            pages = look_up(k0 + 128);
+            // (behind the last step the first slot of the pool is read: a way round the loads would leave their number open, and what
+            // is waited for with it)
+            for (;;) {
+                fetch(k0 + 128, pages, two);
+                pages = look_up(k0 + 256);
+                attend(one);
+                k0 += 128;
+                if (k0 >= to) {
+                    break;
+                }
+                fetch(k0 + 128, pages, one);
+                pages = look_up(k0 + 256);
+                attend(two);
+                k0 += 128;
+                if (k0 >= to) {
+                    break;
+                }
+            }
         }
 
-        // the four waves' parts
+        // the four waves' parts (addresses made anew: kept over the loop they would cost it registers)
+        uint32_t me = threadIdx.x;
+        asm volatile("" : "+v"(me));
+        const uint32_t ec = me & 15, eg = me >> 4 & 3;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
-        if (g == 0) {
-            sM[wave][c] = m;
-            sL[wave][c] = l;
+        if (eg == 0) {
+            sM[wave][ec] = m;
+            sL[wave][ec] = l;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int t = 0; t < kVec; t += 4) {
-                *(v4f *)(&sO[wave][c * kRow + kVec * (4 * g + i) + t]) = (v4f){o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]} * unit;
+                *(v4f *)(&sO[wave][ec * kRow + kVec * (4 * eg + i) + t]) = (v4f){o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]} * unit;
             }
         }
         __syncthreads();
         float *part = part_at(a, shares, blockIdx.y, share, tile != share * per, DIM);
-        for (uint32_t at = threadIdx.x; at < nq * (DIM / 4); at += 256) {
+        for (uint32_t at = me; at < nq * (DIM / 4); at += 256) {
             const uint32_t r = at / (DIM / 4), d = at % (DIM / 4) * 4;
             const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
             float sum = 0.0f;

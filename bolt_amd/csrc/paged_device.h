@@ -75,6 +75,10 @@ __device__ __forceinline__ void store8(void *p, size_t at, const float *x)
     }
 }
 
+// a list that no kernel running now writes, for reads at the wave's own index: they go through the scalar unit, so that no
+// vector load behind them has to be waited for
+typedef const __attribute__((address_space(4))) int32_t *uniform_list;
+
 // ---- sums over a wave ---------------------------------------------------------------------------------
 // Inclusive sums over the 64 lanes, on the vector unit alone (rows of 16, then 15 -> 16.., 31 -> 32..)
 __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v)
