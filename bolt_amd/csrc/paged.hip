@@ -10,31 +10,58 @@ namespace bg {
 // and the elements behind the rotated part). Every step is one fp32 operation in the order the plain formula has it:
 //   a' = a * cos - b * sin,  b' = b * cos + a * sin
 // rounded once to the stored type. An int8 slot gets s = (1 / max|x|) * 127 (1 for an all-zero row) and q = rne(x * s).
+// What bounds it is memory: every element is read once and written once. The rows' elements are asked for before anything
+// else, and whose row it is by all lanes at once, so that a row waits twice for memory and not once per step of a search.
 template <int ACT, int CT, int DIM>
 __global__ void paged_append_kernel(PagedAppendArgs a)
 {
     constexpr uint32_t kLanes = DIM / 16;
-    const uint32_t row = blockIdx.x;
-    const uint32_t b = paged_owner(a.batch, row);
-    const PagedSeq s = paged_seq(a.batch, b);
+    const uint32_t row = blockIdx.x, lane = threadIdx.x & 63;
+    const uint32_t kvh = a.pool.kv_heads, heads = a.heads + 2 * kvh;
+    struct Item {
+        uint32_t head, l, h, e0, e1;  // head row among all, run of 16 elements in it, head among its kind, where its halves are
+        bool is_q, is_v, turned;
+        float x[16];
+    };
+    auto load = [&](uint32_t item, Item &n) {
+        n.head = item / kLanes;
+        n.l = item % kLanes;
+        n.is_q = n.head < a.heads;
+        n.is_v = n.head >= a.heads + kvh;
+        n.h = n.is_q ? n.head : n.is_v ? n.head - a.heads - kvh : n.head - a.heads;
+        n.turned = !n.is_v && 16 * n.l < a.rot;
+        n.e0 = n.turned && !a.interleaved ? 8 * n.l : 16 * n.l;
+        n.e1 = n.turned && !a.interleaved ? a.rot / 2 + 8 * n.l : 16 * n.l + 8;
+        const void *src = n.is_q ? a.q : n.is_v ? a.v : a.k;
+        const size_t base = (size_t)row * (n.is_q ? a.qstride : n.is_v ? a.vstride : a.kstride) + (size_t)n.h * DIM;
+        load8<ACT>(src, base + n.e0, n.x);
+        load8<ACT>(src, base + n.e1, n.x + 8);
+    };
+    Item n;
+    if (threadIdx.x < heads * kLanes) {
+        load(threadIdx.x, n);
+    }
+    uint32_t b;
+    PagedSeq s;
+    if (!a.batch.offsets || a.batch.batch > 64) {
+        b = paged_owner(a.batch, row);
+        s = paged_seq(a.batch, b);
+    } else {
+        const uint32_t last = a.batch.batch - 1, mine = min(lane, last);
+        const int32_t first = a.batch.offsets[mine], next = a.batch.offsets[mine + 1], len = a.batch.lens[mine];
+        const unsigned long long reached = __ballot(lane <= last && (int64_t)first <= (int64_t)row);
+        b = reached ? 63 - (uint32_t)__builtin_clzll(reached) : 0;
+        s = paged_seq_from(__builtin_amdgcn_readlane(first, b), __builtin_amdgcn_readlane(next, b), __builtin_amdgcn_readlane(len, b));
+    }
     const int64_t i = (int64_t)row - s.first, pos = s.pos + i;
-    if (i < 0 || i >= s.count || pos < 0 || pos >= (int64_t)a.batch.max_pages << a.pool.shift ||
-        (a.rot && pos >= (int64_t)a.angles)) {
+    if (i < 0 || i >= s.count || pos < 0 || pos >= (int64_t)a.batch.max_pages << a.pool.shift || (a.rot && pos >= (int64_t)a.angles)) {
         return;
     }
-    const uint32_t kvh = a.pool.kv_heads, heads = a.heads + 2 * kvh;
-    for (uint32_t item = threadIdx.x; item < heads * kLanes; item += blockDim.x) {
-        const uint32_t head = item / kLanes, l = item % kLanes;
-        const bool is_q = head < a.heads, is_v = head >= a.heads + kvh;
-        const uint32_t h = is_q ? head : is_v ? head - a.heads - kvh : head - a.heads;
-        const bool turned = !is_v && 16 * l < a.rot;
-        const uint32_t e0 = turned && !a.interleaved ? 8 * l : 16 * l;
-        const uint32_t e1 = turned && !a.interleaved ? a.rot / 2 + 8 * l : 16 * l + 8;
-        const void *src = is_q ? a.q : is_v ? a.v : a.k;
-        const size_t base = (size_t)row * (is_q ? a.qstride : is_v ? a.vstride : a.kstride) + (size_t)h * DIM;
-        float x[16];
-        load8<ACT>(src, base + e0, x);
-        load8<ACT>(src, base + e1, x + 8);
+    const int64_t slot0 = paged_slot(a.batch.table + (size_t)b * a.batch.max_pages, (uint32_t)pos, a.pool.shift, a.pool.pages, kvh, 0);
+    for (uint32_t item = threadIdx.x; item < heads * kLanes;) {
+        const uint32_t l = n.l, h = n.h, e0 = n.e0, e1 = n.e1;
+        const bool is_q = n.is_q, is_v = n.is_v, turned = n.turned;
+        float (&x)[16] = n.x;
         if (turned) {
             const size_t at = (size_t)pos * (a.rot / 2) + 8 * l;
             float c[8], sn[8];
@@ -57,9 +84,8 @@ __global__ void paged_append_kernel(PagedAppendArgs a)
             const size_t to = (size_t)row * a.qostride + (size_t)h * DIM;
             store8<ACT>(a.qout, to + e0, x);
             store8<ACT>(a.qout, to + e1, x + 8);
-            continue;
         }
-        const int64_t slot = paged_slot(a.batch.table + (size_t)b * a.batch.max_pages, (uint32_t)pos, a.pool.shift, a.pool.pages, kvh, h);
+        const int64_t slot = slot0 < 0 || is_q ? -1 : slot0 + ((int64_t)h << a.pool.shift);
         void *dst = is_v ? a.pool.v : a.pool.k;
         if (CT == PT_I8) {
             float top = 0.0f;
@@ -98,6 +124,10 @@ __global__ void paged_append_kernel(PagedAppendArgs a)
         } else if (slot >= 0) {
             store8<CT>(dst, (size_t)slot * DIM + e0, x);
             store8<CT>(dst, (size_t)slot * DIM + e1, x + 8);
+        }
+        item += blockDim.x;
+        if (item < heads * kLanes) {
+            load(item, n);
         }
     }
 }

@@ -75,7 +75,7 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, v4f v)
         typedef _Float16 v4h __attribute__((ext_vector_type(4)));
         *(v4h *)((uint16_t *)out + at) = (v4h){(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
     } else {
-        *(v2u *)((uint16_t *)out + at) = (v2u){f32_to_bf16(v[0]) | (f32_to_bf16(v[1]) << 16), f32_to_bf16(v[2]) | (f32_to_bf16(v[3]) << 16)};
+        *(v2u *)((uint16_t *)out + at) = (v2u){pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
     }
 }
 

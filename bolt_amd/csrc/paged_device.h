@@ -9,14 +9,12 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
-// round to nearest even; NaN keeps its sign and becomes quiet
-__device__ __forceinline__ uint32_t f32_to_bf16(float f)
+// two values rounded to nearest, the first in the low half
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b)
 {
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) {
-        return (u >> 16) | 0x40u;
-    }
-    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2b));
 }
 
 // eight consecutive elements (16-byte aligned) <-> fp32
@@ -69,7 +67,7 @@ __device__ __forceinline__ void store8(void *p, size_t at, const float *x)
         v4u a;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            a[i] = f32_to_bf16(x[2 * i]) | (f32_to_bf16(x[2 * i + 1]) << 16);
+            a[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
         }
         *(v4u *)((uint16_t *)p + at) = a;
     }
