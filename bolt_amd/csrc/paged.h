@@ -45,6 +45,6 @@ hipError_t launch_paged_decode(const PagedAttentionArgs &a, hipStream_t st);
 size_t paged_decode_workspace(const PagedPool &pool, uint32_t heads);  // bytes
 hipError_t launch_paged_prompt(const PagedAttentionArgs &a, hipStream_t st);
 size_t paged_prompt_workspace(const PagedPool &pool, const PagedBatch &batch, uint32_t heads);  // bytes
-bool paged_prompt_fits(const PagedPool &pool, const PagedBatch &batch, uint32_t heads);  // the grid in 31 bits
+bool paged_prompt_fits(const PagedPool &pool, const PagedBatch &batch, uint32_t heads);  // a grid of fewer than 2^32 threads, which is what a launch can have
 
 }  // namespace bg

@@ -795,7 +795,7 @@ struct Prompt {
 bool paged_prompt_fits(const PagedPool &pool, const PagedBatch &batch, uint32_t heads)
 {
     const uint32_t group = heads / pool.kv_heads;
-    return (uint64_t)batch.rows * group <= 0x7fffffffull && most_tiles(batch, group) * pool.kv_heads <= 0x7fffffffull;
+    return (uint64_t)batch.rows * group <= 0x7fffffffull && most_tiles(batch, group) * pool.kv_heads < 1u << 24;
 }
 
 size_t paged_prompt_workspace(const PagedPool &pool, const PagedBatch &batch, uint32_t heads)

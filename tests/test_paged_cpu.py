@@ -114,6 +114,19 @@ def test_refusals_of_attention(prompt):
     assert attend(True, b=rows(None)) == NULL_POINTER      # prompt needs them
 
 
+def test_more_row_tiles_than_a_launch_can_have():
+    """128 rows to a workgroup of 256 threads, fewer than 2^32 threads to a launch: fewer than 2^24 (rows * heads / 128 + batch * key
+    heads)"""
+    n = C.c_size_t(0)
+    size = lib().bolt_gfx950_paged_attention_workspace_bytes
+    for batch, tokens, kv, heads, code in ((65535, 65535, 512, 512, NOT_SUPPORTED), (65535, 65535, 254, 254, SUCCESS), (1, 1 << 27, 16, 16, NOT_SUPPORTED),
+                                           (1, (1 << 27) - 4096, 16, 16, SUCCESS)):
+        b = rows(P, batch=batch, numTokens=tokens)
+        assert size(pool(kvHeads=kv), b, heads, C.byref(n)) == code
+        if code:
+            assert attend(True, c=pool(kvHeads=kv), b=b, heads=heads, qs=heads * 64, os_=heads * 64) == code
+
+
 def test_nothing_to_do_is_success():
     for b in (rows(P, batch=0, numTokens=0), rows(P, numTokens=0), rows(P, batch=0)):
         assert append(b=b) == SUCCESS and attend(True, b=b) == SUCCESS
