@@ -12,11 +12,16 @@ namespace bg {
 // rounded once to the stored type. An int8 slot gets s = (1 / max|x|) * 127 (1 for an all-zero row) and q = rne(x * s).
 // What bounds it is memory: every element is read once and written once. The rows' elements are asked for before anything
 // else, and whose row it is by all lanes at once, so that a row waits twice for memory and not once per step of a search.
+constexpr uint32_t kRowsX = 20;  // log2 of the rows along the grid's x extent: a launch has fewer than 2^32 threads there
+
 template <int ACT, int CT, int DIM>
 __global__ void paged_append_kernel(PagedAppendArgs a)
 {
     constexpr uint32_t kLanes = DIM / 16;
-    const uint32_t row = blockIdx.x, lane = threadIdx.x & 63;
+    const uint32_t row = blockIdx.y << kRowsX | blockIdx.x, lane = threadIdx.x & 63;
+    if (row >= a.batch.rows) {
+        return;
+    }
     const uint32_t kvh = a.pool.kv_heads, heads = a.heads + 2 * kvh;
     struct Item {
         uint32_t head, l, h, e0, e1;  // head row among all, run of 16 elements in it, head among its kind, where its halves are
@@ -140,7 +145,8 @@ struct Append {
     {
         const uint32_t items = (a.heads + 2 * a.pool.kv_heads) * (DIM / 16);
         const uint32_t threads = items >= 512 ? 512 : (items + 63) / 64 * 64;
-        hipLaunchKernelGGL((paged_append_kernel<ACT, CT, DIM>), dim3(a.batch.rows), dim3(threads), 0, st, a);
+        const uint32_t x = a.batch.rows < 1u << kRowsX ? a.batch.rows : 1u << kRowsX;
+        hipLaunchKernelGGL((paged_append_kernel<ACT, CT, DIM>), dim3(x, (a.batch.rows + x - 1) / x), dim3(threads), 0, st, a);
         return hipGetLastError();
     }
 };

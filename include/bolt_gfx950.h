@@ -513,7 +513,7 @@ EE bolt_gfx950_gelu_f32(float *x, size_t n);
  * A batch says where the new tokens of `batch` sequences are: they are packed rows, sequence b owning rows offsets[b] up to
  * offsets[b + 1] (ascending), and they are the LAST ones of the sequence's lengths[b] keys. offsets == NULL: one new token
  * per sequence, row b (numTokens == batch). numTokens is the number of rows the buffers have: rows behind
- * offsets[batch] belong to nobody and are neither read nor written. lengths, offsets and pageTable are read by the
+ * offsets[batch] belong to nobody: what they hold has no influence, and they are not written. lengths, offsets and pageTable are read by the
  * kernels, so that a captured graph can be replayed with other values; nothing in them is trusted: a page number
  * outside the pool, a position in front of the sequence or behind the page table (maxPages pages) is a key that is not
  * stored and not seen, never an address. lengths[b] == 0: a place of a padded batch that nobody uses.

@@ -149,6 +149,24 @@ def test_append_of_infinities_and_nan_shows_them():
     assert torch.isnan(scale[0]) and scale[1] == 0 and scale[2] == 127
 
 
+def test_append_of_more_rows_than_a_grid_is_wide():
+    """2^26 + 2 rows of 64 threads, all but the last three nobody's"""
+    rows, g = (1 << 26) + 2, torch.Generator().manual_seed(7)
+    c = Case("f16", "f16", 1, 1, 64, 8, (3,), (3,), seed=7)
+    pc, _, _ = c.gpu()
+    new = torch.empty(rows, 1, 64, dtype=torch.float16, device="cuda")
+    new[-3:] = last = torch.randn(3, 1, 64, generator=g).half().cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    batch = hp.PagedBatch(c.table.cuda(), torch.tensor([3], **i32), torch.tensor([rows - 3, rows], **i32), rows)
+    torch.cuda.synchronize()
+    hp.kv_cache_append(pc, batch, new, new)
+    sync()
+    for now, was in zip(pc.keep[:2], (c.k, c.v)):
+        want = was.clone()
+        want[c.table[0, 0].long(), 0, :3] = last[:, 0].cpu()
+        assert torch.equal(bits(now), bits(want))
+
+
 # ---- attention --------------------------------------------------------------------------------------
 DECODE = [
     # heads, kv_heads, dim, page, lengths, window
