@@ -13,6 +13,8 @@
 // a row are permuted so that 16 lanes of either read pattern touch all banks. An int8 cache passes registers on the way
 // and lies in LDS as fp16, which holds its values exactly; its steps multiply scores and weights.
 // Where few tiles meet many keys, several workgroups share a tile's keys and a second launch joins their parts.
+#include <atomic>
+
 #include "paged_device.h"
 
 namespace bg {
@@ -761,6 +763,28 @@ uint32_t shares_of(const PagedPool &pool, const PagedBatch &b, uint32_t heads)
     return (uint32_t)(n < keys ? n : keys);
 }
 
+// Before a kernel's first launch on a device (one bit each in `done`; a second time does no harm): it may ask for its LDS, and has
+// none besides, for the tiles are taken to start at LDS address 0
+hipError_t prepare(const void *kernel, uint32_t lds, std::atomic<uint64_t> &done)
+{
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (e != hipSuccess || (device < 64 && done.load(std::memory_order_relaxed) & bit)) {
+        return e;
+    }
+    hipFuncAttributes have;
+    e = hipFuncGetAttributes(&have, kernel);
+    if (e == hipSuccess && have.sharedSizeBytes != 0) {
+        e = hipErrorInvalidImage;
+    }
+    e = e != hipSuccess ? e : hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e == hipSuccess) {
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return e;
+}
+
 template <int ACT, int CT, int DIM>
 struct Prompt {
     static hipError_t run(const PagedAttentionArgs &a, hipStream_t st)
@@ -768,20 +792,16 @@ struct Prompt {
         const uint32_t shares = shares_of(a.pool, a.batch, a.heads);
         const uint64_t tiles = most_tiles(a.batch, a.heads / a.pool.kv_heads);
         constexpr uint32_t lds = prompt_lds<CT, DIM>();
-        static const hipError_t ready = [] {
-            const hipError_t e = hipFuncSetAttribute((const void *)paged_prompt_kernel<ACT, CT, DIM, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-            return e != hipSuccess ? e : hipFuncSetAttribute((const void *)paged_prompt_kernel<ACT, CT, DIM, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        }();
-        if (ready != hipSuccess) {
-            return ready;
+        const bool paged = 1u << a.pool.shift >= rows_at<CT, DIM>();
+        const auto kernel = paged ? paged_prompt_kernel<ACT, CT, DIM, true> : paged_prompt_kernel<ACT, CT, DIM, false>;
+        static std::atomic<uint64_t> ready[2];
+        hipError_t e = prepare((const void *)kernel, lds, ready[paged]);
+        if (e != hipSuccess) {
+            return e;
         }
         const uint64_t blocks = tiles * a.pool.kv_heads;
-        if (1u << a.pool.shift >= rows_at<CT, DIM>()) {
-            hipLaunchKernelGGL((paged_prompt_kernel<ACT, CT, DIM, true>), dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
-        } else {
-            hipLaunchKernelGGL((paged_prompt_kernel<ACT, CT, DIM, false>), dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
-        }
-        const hipError_t e = hipGetLastError();
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
+        e = hipGetLastError();
         if (e != hipSuccess || shares == 1) {
             return e;
         }
