@@ -433,6 +433,15 @@ EE bolt_gfx950_set_stream(void *stream)
     return SUCCESS;
 }
 
+EE bolt_gfx950_get_stream(void **stream)
+{
+    if (!stream) {
+        return NULL_POINTER;
+    }
+    *stream = (void *)ctx().stream;
+    return SUCCESS;
+}
+
 EE bolt_gfx950_synchronize(void)
 {
     EE e = ensure_init();

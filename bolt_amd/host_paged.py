@@ -1,6 +1,6 @@
 """Host-side mirrors of the paged key / value cache entry points on torch CUDA tensors: append with position rotation,
 attention of one new token per sequence, attention of prompts. All arithmetic is in libbolt_gfx950.so; the calls enqueue
-on the library's stream (bolt_gfx950_set_stream) and return.
+on the library's stream (bolt_gfx950_set_stream) and return. What they allocate belongs to that stream.
 
     cache = PagedKvCache(k, v)                                   # [pages, kv_heads, page_size, head_dim]
     batch = PagedBatch(page_table, lengths)                      # lengths include the new tokens
@@ -86,6 +86,19 @@ def _one_device(*tensors):
     return next(iter(found))
 
 
+def _empty(shape, dtype, device):
+    """A new tensor that the library's stream uses. torch hands memory out again in the order of the stream it was allocated on, so
+    it is allocated on that one; and the stream that is current in torch has to be done with it, too, before it is."""
+    ours, current = C.c_void_p(), torch.cuda.current_stream(device)
+    check(lib().bolt_gfx950_get_stream(C.byref(ours)), "get_stream")
+    if (ours.value or 0) == current.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(ours.value, device) if ours.value else torch.cuda.default_stream(device)):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(current)
+    return t
+
+
 def _rows(t, name, shape, dtype, device):
     """Checks rows of heads, [rows, heads, dim] with dense heads; returns the elements between rows. (On the path of every call:
     no message is made before it is needed.)"""
@@ -119,7 +132,7 @@ def kv_cache_append(cache, batch, k, v, q=None, rotary=None, q_out=None):
         shape = (shape[0], heads, shape[2])
         qs = _rows(q, "q", shape, dtype, device)
         if q_out is None:
-            q_out = torch.empty(shape, dtype=dtype, device=device)
+            q_out = _empty(shape, dtype, device)
             qo = heads * shape[2]
         else:
             qo = _rows(q_out, "q_out", shape, dtype, device)
@@ -135,7 +148,7 @@ def paged_attention_workspace(cache, batch, heads):
     """Device memory for the attention calls of this cache and batch shape; calls that may overlap need one each."""
     n = C.c_size_t(0)
     check(lib().bolt_gfx950_paged_attention_workspace_bytes(cache.ref, batch.ref, heads, C.byref(n)), "paged_attention_workspace_bytes")
-    return torch.empty(n.value, dtype=torch.uint8, device=cache.device)
+    return _empty(n.value, torch.uint8, cache.device)
 
 
 def _attention(fn, what, cache, batch, q, out, scale, window, workspace):
@@ -152,7 +165,7 @@ def _attention(fn, what, cache, batch, q, out, scale, window, workspace):
     elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
         raise BoltError("workspace: contiguous uint8 on the cache's GPU")
     if out is None:
-        out, os = torch.empty(shape, dtype=dtype, device=device), heads * shape[2]
+        out, os = _empty(shape, dtype, device), heads * shape[2]
     else:
         os = _rows(out, "out", shape, dtype, device)
     code = fn(cache.ref, batch.ref, dt, heads, q.data_ptr(), qs, out.data_ptr(), os, cache.scale if scale is None else scale, window,

@@ -321,6 +321,30 @@ def test_same_bytes_again_and_on_another_stream(prompt):
         assert torch.equal(bits(o[mine]), bits(first[mine]))
 
 
+@pytest.mark.parametrize("prompt", [False, True])
+def test_what_a_call_allocates_is_not_handed_out_before_its_work_is_done(prompt):
+    """The library's stream is behind; torch's own goes on and asks for memory of the sizes that the call has just let go"""
+    c = Case("f32", "f16", 8, 2, 128, 16, (900, 400), (9, 1) if prompt else (1, 1), seed=24)
+    want = attend(c, prompt)
+    cache, batch, q = c.gpu(offsets=prompt)
+    fn = hp.paged_attention_prompt if prompt else hp.paged_attention_decode
+    size = hp.paged_attention_workspace(cache, batch, 8).numel()
+    side = torch.cuda.Stream()
+    capi.check(capi.lib().bolt_gfx950_set_stream(side.cuda_stream), "set_stream")
+    try:
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        out = fn(cache, batch, q)
+        taken = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]
+        torch.cuda.current_stream().synchronize()
+        sync()
+    finally:
+        capi.check(capi.lib().bolt_gfx950_set_stream(None), "set_stream")
+    mine = slice(0, int(c.offsets[-1]))
+    assert torch.equal(bits(out[mine]), bits(want[mine])) and all((t == 255).all() for t in taken)
+
+
 @pytest.mark.parametrize("cache_type", ["f16", "i8"])
 def test_offsets_beyond_32_bits(cache_type):
     """a pool of more than 2^32 elements, the sequence in its last pages"""
