@@ -107,7 +107,11 @@ def _rows(t, name, shape, dtype, device):
     s = t.stride()
     if s[2] != 1 or (s[1] != shape[2] and shape[1] != 1):
         raise BoltError("%s: the heads of a row are dense" % name)
-    return s[0] if shape[0] > 1 else max(s[0], shape[1] * shape[2])
+    if shape[0] < 2:
+        return shape[1] * shape[2]
+    if s[0] > 0xffffffff:  # (ctypes would pass its low 32 bits)
+        raise BoltError("%s: rows are fewer than 2^32 elements apart" % name)
+    return s[0]
 
 
 def _here(cache, batch):
@@ -128,6 +132,8 @@ def kv_cache_append(cache, batch, k, v, q=None, rotary=None, q_out=None):
     ks, vs = _rows(k, "k", shape, dtype, device), _rows(v, "v", shape, dtype, device)
     heads, qs, qo, qp, qop = 0, 0, 0, None, None
     if q is not None:
+        if q.dim() != 3:
+            raise BoltError("q: [rows, heads, head_dim]")
         heads = q.shape[1]
         shape = (shape[0], heads, shape[2])
         qs = _rows(q, "q", shape, dtype, device)
@@ -157,6 +163,8 @@ def _attention(fn, what, cache, batch, q, out, scale, window, workspace):
     dt = DT_OF.get(dtype)
     if dt is None or q.dim() != 3:
         raise BoltError("q: [rows, heads, head_dim] of float32, float16 or bfloat16")
+    if not 0 <= window <= 0xffffffff:
+        raise BoltError("window: 0 (every key) to 2^32 - 1 keys")
     heads = q.shape[1]
     shape = (batch.rows, heads, cache.head_dim)
     qs = _rows(q, "q", shape, dtype, device)

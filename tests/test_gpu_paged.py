@@ -42,6 +42,17 @@ def attend(case, prompt, **kw):
     return out
 
 
+def test_rows_four_billion_elements_apart_are_refused():
+    """2^32 + 128 elements between rows: 128 in 32 bits"""
+    c = Case("f16", "f16", 2, 2, 64, 16, (9, 5), (1, 1), seed=1)
+    cache, batch, q = c.gpu(offsets=False)
+    far = torch.empty((1 << 32) + 256, dtype=torch.float16, device="cuda").as_strided((2, 2, 64), ((1 << 32) + 128, 64, 1))
+    for call in (lambda: hp.paged_attention_decode(cache, batch, far), lambda: hp.paged_attention_decode(cache, batch, q, out=far),
+                 lambda: hp.kv_cache_append(cache, batch, far, q), lambda: hp.kv_cache_append(cache, batch, q, q, q, None, far)):
+        with pytest.raises(capi.BoltError, match="2\\^32"):
+            call()
+
+
 # ---- append -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("act,cache", COMBOS)
 @pytest.mark.parametrize("dim,page,rot,interleaved,new,past", [
@@ -50,6 +61,9 @@ def attend(case, prompt, **kw):
     (128, 64, 32, False, (70,), (60,)),
     (64, 1, 16, True, (3, 2), (0, 5)),
     (128, 4096, 0, False, (2, 9), (4094, 0)),
+    (128, 16, 80, False, (6,), (11,)),
+    (64, 8, 48, True, (6,), (11,)),
+    (64, 2, 64, False, tuple(i * 7 % 4 for i in range(150)), tuple(i * 5 % 9 for i in range(150))),
 ])
 def test_append(act, cache, dim, page, rot, interleaved, new, past):
     print("append", act, cache, dim, page, rot, interleaved, new, past, flush=True)
@@ -177,11 +191,15 @@ DECODE = [
     (40, 2, 128, 128, (700, 129), 100),
     (3, 3, 64, 4096, (1, 4097, 515), 33),
     (16, 8, 128, 64, (2500, 1, 0, 640), 1),
+    (71, 1, 64, 16, (40, 90), 0),                                              # five tiles of queries, the last of seven
+    (1024, 1024, 64, 16, (5, 140), 0),                                         # more columns than workgroups fit the chip
+    (16, 16, 128, 16, tuple(i * 37 % 400 for i in range(67)), 0),              # shares that hold several sequences and parts of others
+    (2, 1, 64, 8, tuple(i * 53 % 270 for i in range(300)), 0),
 ]
 
 
 @pytest.mark.parametrize("act,cache", COMBOS)
-@pytest.mark.parametrize("shape", DECODE, ids=str)
+@pytest.mark.parametrize("shape", DECODE, ids=lambda s: str(s)[:40])
 def test_decode(act, cache, shape):
     heads, kv, dim, page, lengths, window = shape
     print("decode", act, cache, shape, flush=True)
@@ -201,11 +219,15 @@ PROMPT = [
     (8, 2, 128, 128, (300, 0), (65, 129), 40, 2),
     (3, 3, 64, 4096, (4090, 0), (9, 64), 0, 0),
     (10, 2, 64, 64, (0, 17), (200, 3), 1, 0),
+    (71, 1, 64, 16, (40, 0), (3, 5), 0, 0),
+    (2, 1, 128, 8, tuple(i * 29 % 90 for i in range(130)), tuple(i * 7 % 5 for i in range(130)), 0, 3),
+    (8, 1, 64, 16, (700, 20, 0), (7, 40, 1), 0, 0),                            # keys of a tile shared out, of some and not of others
+    (16, 2, 128, 32, (900, 3), (20, 20), 500, 0),
 ]
 
 
 @pytest.mark.parametrize("act,cache", COMBOS)
-@pytest.mark.parametrize("shape", PROMPT, ids=str)
+@pytest.mark.parametrize("shape", PROMPT, ids=lambda s: str(s)[:40])
 def test_prompt(act, cache, shape):
     heads, kv, dim, page, past, new, window, spare = shape
     print("prompt", act, cache, shape, flush=True)
@@ -226,6 +248,38 @@ def test_attention_with_lists_that_point_outside(prompt, act, cache):
     out = attend(c, prompt)
     assert_attention(out, c)
     assert not out[int(c.offsets[1])].any() and not out[int(c.offsets[3])].any()
+
+
+LOW, HIGH = -(1 << 31), (1 << 31) - 1
+
+
+@pytest.mark.parametrize("cache_type", ["f16", "i8"])
+@pytest.mark.parametrize("offsets,lengths", [
+    ((0, 5, 3, 9, 9), (20, 11, 24, 0)), ((-5, 3, 2, HIGH, 7), (HIGH, LOW, 17, -1)), ((HIGH, LOW, HIGH, 0, LOW), (24, 24, 24, 24)),
+    ((0, HIGH, 0, HIGH, 0), (HIGH, 24, 5, 1)), ((9, 10, 11, 12, 13), (1, 2, 3, 4)), ((-9, -4, 0, 1, 2), (9, 24, 9, 24)),
+] + [(tuple(i * 7919 % 23 - 6 for i in range(81)), tuple(i * 31 % 40 - 4 for i in range(80)))], ids=lambda s: str(s)[:40])
+def test_lists_of_anything_stay_inside_the_buffers(cache_type, offsets, lengths):
+    """Offsets that do not ascend, behind and in front of the rows; lengths of any size: what the calls answer means nothing, but
+    nothing around the rows and the pool's pages changes"""
+    print("lists", cache_type, offsets[:5], lengths[:5], flush=True)
+    rows, n = 9, len(lengths)
+    c = Case("f16", cache_type, 6, 2, 64, 8, (24,) * n, (1,) * n, seed=31)
+    outer = [None if t is None else torch.cat([t[:2], t, t[:2]]).cuda() for t in (c.k, c.v, c.ks, c.vs)]
+    before = [None if t is None else t.clone() for t in outer]
+    cache = hp.PagedKvCache(*(None if t is None else t[2:-2] for t in outer))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    batch = hp.PagedBatch(c.table.cuda(), torch.tensor(lengths, **i32), torch.tensor(offsets, **i32), rows)
+    wide = [torch.full((rows + 4, 6, 64), 5.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+    q, k = (torch.ones(rows, h, 64, dtype=torch.float16, device="cuda") for h in (6, 2))
+    r = hp.Rotary(*(torch.ones(24, 32, device="cuda") for _ in range(2)))
+    hp.kv_cache_append(cache, batch, k, k, q, r, wide[0][2:-2])
+    hp.paged_attention_prompt(cache, batch, q, out=wide[1][2:-2])
+    sync()
+    for t in wide:
+        assert (t[:2] == 5).all() and (t[-2:] == 5).all()
+    for t, was in zip(outer, before):
+        for end in (slice(0, 2), slice(-2, None)):
+            assert t is None or torch.equal(bits(t[end]), bits(was[end]))
 
 
 @pytest.mark.parametrize("act,cache", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "i8")])
@@ -267,6 +321,41 @@ def test_large_and_small_scores(prompt, act, cache):
         if cache != "i8":
             c.k[c.k.isfinite()] *= 0.01 if size == 60.0 else 1.0
         assert_attention(attend(c, prompt), c)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("act,cache", COMBOS)
+def test_scales_below_zero_and_of_zero(prompt, act, cache):
+    c = Case(act, cache, 4, 2, 128, 16, (150, 40, 0), (20, 1, 0) if prompt else (1, 1, 1), seed=25)
+    for scale in (-0.3, 0.0, -1e-3):
+        assert_attention(attend(c, prompt, scale=scale), c, scale)
+
+
+@pytest.mark.parametrize("cache_type", ["f16", "i8"])
+def test_sequences_that_share_pages(cache_type):
+    """a common beginning in the same pages, once in one sequence's own order and once twice in one table"""
+    for prompt in (False, True):
+        c = Case("f16", cache_type, 6, 3, 64, 16, (50, 60, 48), (3, 9, 2) if prompt else (1, 1, 1), seed=26)
+        c.table[1, :2] = c.table[0, :2]
+        c.table[2, 0] = c.table[2, 1] = c.table[0, 1]
+        assert_attention(attend(c, prompt), c)
+
+
+@pytest.mark.parametrize("cache_type", ["f16", "i8"])
+def test_a_table_of_two_billion_positions_for_many(cache_type):
+    """130 rows of 2^31 - 4096 positions each, which are more tiles of 128 keys than 31 bits count; lengths among them are short,
+    but for two whose keys fill several tiles of the larger ones"""
+    lengths = [1 + i * 97 % 300 for i in range(128)] + [5000, 1300]
+    c = Case("f16", cache_type, 2, 1, 64, 4096, lengths, [1] * 130, seed=27)
+    want = attend(c, False)
+    assert_attention(want, c)
+    cache, batch, q = c.gpu(offsets=False)
+    table = torch.full((130, (1 << 31) // 4096 - 1), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.max_pages] = c.table.cuda()
+    torch.cuda.synchronize()
+    out = hp.paged_attention_decode(cache, hp.PagedBatch(table, batch.keep[1]), q)
+    sync()
+    assert_attention(out, c)
 
 
 def test_queries_beyond_the_range_of_fp16():
@@ -432,6 +521,78 @@ def test_captured_step_replayed_with_other_lengths():
         capi.check(capi.lib().bolt_gfx950_set_stream(None), "set_stream")
 
 
+@pytest.mark.parametrize("act,cache_type", [("f16", "f16"), ("bf16", "i8")])
+def test_captured_prompts_replayed_with_other_lengths(act, cache_type):
+    """a chunk of prompts in a graph: offsets, lengths and queries change between the replays, empty places and none at all among
+    them; the library's eager calls run in between and give the same bytes"""
+    c = Case(act, cache_type, 8, 2, 128, 16, (400, 90, 33), (30, 9, 1), seed=28, rows=48)
+    cache, batch, q = c.gpu()
+    _, lengths, offsets = batch.keep
+    ws = hp.paged_attention_workspace(cache, batch, 8)
+    out = torch.full_like(q, 7.0)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    capi.check(capi.lib().bolt_gfx950_set_stream(side.cuda_stream), "set_stream")
+    try:
+        hp.paged_attention_prompt(cache, batch, q, out=out, workspace=ws)
+        sync()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            hp.paged_attention_prompt(cache, batch, q, out=out, workspace=ws)
+        g = torch.Generator().manual_seed(29)
+        for held, new in (((400, 90, 33), (30, 9, 1)), ((17, 0, 0), (17, 0, 0)), ((0, 0, 0), (0, 0, 0)), ((399, 64, 1), (1, 40, 1)), ((200, 80, 20), (7, 0, 41))):
+            c.lengths, c.new = list(held), list(new)
+            c.offsets = torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32)
+            c.q = torch.randn(c.q.shape, generator=g).to(TYPES[act])
+            for to, values in ((lengths, torch.tensor(held, dtype=torch.int32)), (offsets, c.offsets), (q, c.q), (out, torch.full_like(c.q, 7.0))):
+                to.copy_(values)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            mine = assert_attention(out, c)
+            assert (out[torch.from_numpy(~mine).cuda()] == 7).all()
+            eager = torch.full_like(q, 7.0)
+            torch.cuda.synchronize()
+            hp.paged_attention_prompt(cache, batch, q, out=eager)
+            sync()
+            assert torch.equal(bits(eager), bits(out))
+    finally:
+        capi.check(capi.lib().bolt_gfx950_set_stream(None), "set_stream")
+
+
+def test_two_threads_at_once():
+    """every thread has a stream of its own; workspaces are apart, the cache is shared"""
+    import threading
+    c = Case("f16", "f16", 16, 4, 128, 16, (1500, 700, 90), (1, 1, 1), seed=30)
+    p = Case("f16", "f16", 16, 4, 128, 16, (1500, 700, 90), (40, 200, 90), seed=30)
+    want = [attend(c, False), attend(p, True)]
+    sides = [(hp.paged_attention_decode, *c.gpu(offsets=False)), (hp.paged_attention_prompt, *p.gpu())]
+    torch.cuda.synchronize()
+    outs, errors = [[], []], []
+
+    def run(i):
+        try:
+            stream = torch.cuda.Stream()
+            capi.check(capi.lib().bolt_gfx950_set_stream(stream.cuda_stream), "set_stream")
+            fn, cache, batch, q = sides[i]
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    outs[i].append(fn(cache, batch, q))
+            stream.synchronize()
+            capi.check(capi.lib().bolt_gfx950_set_stream(None), "set_stream")
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i, case in enumerate((c, p)):
+        mine = slice(0, int(case.offsets[-1]))
+        assert len(outs[i]) == 20 and all(torch.equal(bits(o[mine]), bits(want[i][mine])) for o in outs[i])
+
+
 @pytest.mark.parametrize("cache_type", ["f16", "i8"])
 def test_generation_over_an_int8_projection(cache_type):
     """What the operators are for: hidden states go through the library's int8 QKV product, prompts are stored and attended, then
@@ -511,7 +672,8 @@ def test_host_mirror_refuses():
                  lambda: hp.paged_attention_prompt(cache, batch, q), lambda: hp.paged_attention_decode(cache, batch, q, out=q),
                  lambda: hp.paged_attention_decode(cache, batch, q, out=torch.empty_like(q).float()), lambda: hp.paged_attention_decode(cache, batch, q[:, :3]),
                  lambda: hp.paged_attention_decode(cache, batch, q, workspace=torch.empty(0, dtype=torch.uint8, device="cuda")),
-                 lambda: hp.kv_cache_append(cache, batch, k[:1], k), lambda: hp.kv_cache_append(cache, batch, k.bfloat16(), k.bfloat16()),
+                 lambda: hp.paged_attention_decode(cache, batch, q, window=-1), lambda: hp.paged_attention_decode(cache, batch, q, window=1 << 32),
+                 lambda: hp.kv_cache_append(cache, batch, k, k, q[0]), lambda: hp.kv_cache_append(cache, batch, k[:1], k), lambda: hp.kv_cache_append(cache, batch, k.bfloat16(), k.bfloat16()),
                  lambda: hp.kv_cache_append(cache, batch, k, k.float()), lambda: hp.kv_cache_append(cache, batch, k, k, q.float()),
                  lambda: hp.kv_cache_append(cache, batch, k, k, q, hp.Rotary(torch.zeros(9, 4, device="cuda"), torch.zeros(9, 4, device="cuda")))):
         with pytest.raises(capi.BoltError):
