@@ -172,7 +172,7 @@ SIGNATURES = {
                                                              C.c_int, C.POINTER(C.c_int), C.c_int, ActivationParamSpec,
                                                              C.c_int]),
     "bolt_gfx950_set_stream": (C.c_int, [_vp]),
-    "bolt_gfx950_get_stream": (C.c_int, [C.POINTER(_vp)]),
+    "bolt_gfx950_get_stream": (_vp, []),
     "bolt_gfx950_synchronize": (C.c_int, []),
     "bolt_gfx950_last_error": (C.c_char_p, []),
     "bolt_gfx950_set_option": (C.c_int, [C.c_char_p, C.c_int]),

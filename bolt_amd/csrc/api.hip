@@ -433,13 +433,9 @@ EE bolt_gfx950_set_stream(void *stream)
     return SUCCESS;
 }
 
-EE bolt_gfx950_get_stream(void **stream)
+void *bolt_gfx950_get_stream(void)
 {
-    if (!stream) {
-        return NULL_POINTER;
-    }
-    *stream = (void *)ctx().stream;
-    return SUCCESS;
+    return (void *)ctx().stream;
 }
 
 EE bolt_gfx950_synchronize(void)

@@ -13,6 +13,7 @@ import math
 import torch
 
 from . import capi
+# (torch._C: what torch.cuda.current_device() and current_stream() wrap; a call on a decoder's path costs the host 8 us)
 from .capi import BoltError, BoltPagedBatch, BoltPagedKvCache, BoltRotary, check, lib
 
 DT_OF = {torch.float32: capi.DT_F32, torch.float16: capi.DT_F16, torch.bfloat16: capi.DT_BF16, torch.int8: capi.DT_I8}
@@ -89,13 +90,12 @@ def _one_device(*tensors):
 def _empty(shape, dtype, device):
     """A new tensor that the library's stream uses. torch hands memory out again in the order of the stream it was allocated on, so
     it is allocated on that one; and the stream that is current in torch has to be done with it, too, before it is."""
-    ours, current = C.c_void_p(), torch.cuda.current_stream(device)
-    check(lib().bolt_gfx950_get_stream(C.byref(ours)), "get_stream")
-    if (ours.value or 0) == current.cuda_stream:
+    ours = lib().bolt_gfx950_get_stream() or 0
+    if ours == torch._C._cuda_getCurrentRawStream(device.index):
         return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(ours.value, device) if ours.value else torch.cuda.default_stream(device)):
+    with torch.cuda.stream(torch.cuda.ExternalStream(ours, device) if ours else torch.cuda.default_stream(device)):
         t = torch.empty(shape, dtype=dtype, device=device)
-    t.record_stream(current)
+    t.record_stream(torch.cuda.current_stream(device))
     return t
 
 
@@ -115,7 +115,7 @@ def _rows(t, name, shape, dtype, device):
 
 
 def _here(cache, batch):
-    if cache.device != batch.device or cache.device.index != torch.cuda.current_device():
+    if cache.device != batch.device or cache.device.index != torch._C._cuda_getDevice():
         raise BoltError("cache and batch belong to the current GPU")
 
 

@@ -43,7 +43,7 @@ EE bolt_gfx950_init(void);
  * scratch words are shared by its calls). */
 EE bolt_gfx950_set_stream(void *stream);
 /* The calling thread's stream, for callers that allocate from a pool that is ordered by streams. Waits for nothing. */
-EE bolt_gfx950_get_stream(void **stream);
+void *bolt_gfx950_get_stream(void);
 EE bolt_gfx950_synchronize(void);
 const char *bolt_gfx950_last_error(void);
 /* Tuning / test knobs. "gemm_tile": -1 shape heuristic (default), 0 general kernel, 2 the
