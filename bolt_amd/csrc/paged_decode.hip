@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
             for (int j = 0; j < 8; ++j) {
                 top = fmaxf(top, x[j]);
                 if (CT == PT_I8) {
-                    wide = fmaxf(wide, step[j]);
+                    wide = fmaxf(wide, fabsf(step[j]));
                 }
             }
             if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {

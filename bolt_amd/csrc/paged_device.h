@@ -92,6 +92,21 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v)
     return v;
 }
 
+// largest magnitude of the 64 lanes' values, none of them NaN
+__device__ __forceinline__ float wave_max_abs(float f)
+{
+    uint32_t v = __float_as_uint(fabsf(f));
+#define BG_MAX_STEP(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false))
+    BG_MAX_STEP(0x111, 0xf);  // (as in wave_scan_u32)
+    BG_MAX_STEP(0x112, 0xf);
+    BG_MAX_STEP(0x114, 0xf);
+    BG_MAX_STEP(0x118, 0xf);
+    BG_MAX_STEP(0x142, 0xa);
+    BG_MAX_STEP(0x143, 0xc);
+#undef BG_MAX_STEP
+    return __uint_as_float(__builtin_amdgcn_readlane(v, 63));
+}
+
 // A list of n counts, count(i), laid end to end: which entry place x falls into. Every wave finds out by itself. The first 64
 // counts are asked for once.
 struct Places {

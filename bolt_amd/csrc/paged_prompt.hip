@@ -9,9 +9,16 @@
 //   out^T = V^T P^T    contraction over the keys in the order the scores lie in: P goes from the accumulators into the
 //                      operand with no exchange between lanes; V^T comes from LDS through the transposing read
 //                      (ds_read_b64_tr_b16: a lane gets four keys' values of one d)
-// Key and value tiles go from memory to LDS without passing registers, one tile ahead, in pieces of 16 bytes; the pieces of
-// a row are permuted so that 16 lanes of either read pattern touch all banks. An int8 cache passes registers on the way
-// and lies in LDS as fp16, which holds its values exactly; its steps multiply scores and weights.
+// Key and value tiles of a 16-bit cache go from memory to LDS without passing registers, one tile ahead, in pieces of 16
+// bytes; the pieces of a row are permuted so that 16 lanes of either read pattern touch all banks. An int8 cache's are read
+// into registers two tiles ahead and put into LDS as fp16, which holds its values exactly, between the products of the tile
+// before theirs (a tile waits for one barrier and no load); its steps multiply scores and weights.
+//
+// What it costs. A wave issues 32 products of 32x32x16 a tile (head size 128; 36.5 cycles each alone, 44 with real data,
+// when the power limit lowers the clock) and some 250 vector instructions and 32 exponentials, and it does not overlap its
+// own products with them: two waves on every SIMD, from two workgroups, do. One prompt of 8192 tokens, 32 heads over 8, runs
+// at 1.0 PFLOP/s, where the library's 8192^3 product of the same type reaches 1.2. Head size 128 takes 220 to 230 registers
+// of the 256 that two waves leave each; more rows to a wave would halve the reads of LDS and do not fit.
 // Where few tiles meet many keys, several workgroups share a tile's keys and a second launch joins their parts.
 #include <atomic>
 
@@ -130,6 +137,23 @@ __device__ __forceinline__ float max_of(float a, float b, float c)
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
+// int8: the steps of a tile's keys (times the score scale) and values (over `unit`), values whose step is not finite, and the
+// power of two above the largest step
+struct StepsOfTile {
+    float step[2][kKeys];
+    unsigned long long bad;
+    float unit, unused;
+};
+
+// the workgroup's barrier behind its LDS accesses, without a wait for loads from memory, which __syncthreads() has
+__device__ __forceinline__ void barrier()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <int CT>
 struct Product {
     typedef v8h V;
@@ -184,7 +208,7 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float a, float 
 template <int CT, int DIM>
 constexpr uint32_t prompt_lds()
 {
-    return CT == PT_I8 ? 2 * kKeys * DIM * 2 + 2 * kKeys * DIM + 2 * kKeys * 4 + 8 + 4 : 4 * kKeys * DIM * 2 + DIM * 16 + 4 * 4 + 4;
+    return 4 * kKeys * DIM * 2 + (CT == PT_I8 ? 2 * sizeof(StepsOfTile) : DIM * 16 + 4 * 4 + 4);
 }
 
 // rows of a tile that one load of a wave brings
@@ -203,16 +227,13 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     constexpr bool kShiftQ = kWide || (ACT == PT_BF16 && CT == PT_I8);
     constexpr uint32_t kTileBytes = kKeys * DIM * 2, kRowBytes = DIM * (CT == PT_I8 ? 1 : 2), kPieces = DIM / 8;
     constexpr int kSteps = DIM / 16, kOut = DIM / 32, kLoads = kKeys * kRowBytes / 16 / 256;
-    // LDS, 16-bit caches: two buffers, each a tile of keys and one of values; [DIM][128 rows as bits] rows that see a value which is
-    //        not finite, [4] whether a wave found one, whether there is any
-    //      int8: a tile of keys and one of values in fp16, the next ones as they are stored; steps of 64 keys and 64 values, keys
-    //        whose step is not finite (64 bits), the power of two above the largest step
+    // LDS: two buffers, each a tile of keys and one of values in 16 bits; behind them
+    //   16-bit caches: [DIM][128 rows as bits] rows that see a value which is not finite, [4] whether a wave found one, whether there is any
+    //   int8: two buffers of steps
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     lds_t const sTiles = (lds_t)0;  // smem's own address: the kernel has no other LDS. As a constant it goes into the reads' offsets.
-    constexpr uint32_t kRawBytes = kKeys * DIM, kBehind = CT == PT_I8 ? 2 * kTileBytes + 2 * kRawBytes : 4 * kTileBytes;
-    float *const sStep = (float *)(smem + kBehind);
-    unsigned long long *const sBad = (unsigned long long *)(sStep + 2 * kKeys);
-    float *const sUnit = (float *)(sBad + 1);
+    constexpr uint32_t kBehind = 4 * kTileBytes;
+    StepsOfTile *const sSteps = (StepsOfTile *)(smem + kBehind);
     uint32_t *const sPoison = (uint32_t *)(smem + kBehind), *const sHit = sPoison + 4 * DIM, *const sAny = sHit + 4;
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -287,13 +308,11 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         *base = (size_t)(uint32_t)__shfl((uint32_t)(offset >> 32), from, 64) << 32 | (uint32_t)__shfl((uint32_t)offset, from, 64);
         return 0;
     };
-    // Straight into LDS: a 16-bit cache's rows with their pieces permuted, an int8 cache's as they are
+    // 16-bit caches: straight into LDS, the rows' pieces permuted
     const uint32_t first_row = wave * kRowsAt + in_row;  // of load 0; the others' rows are 4 kRowsAt apart, which changes no permutation
-    float scale = 0.0f;                                  // int8: of key lane (wave 0: key, wave 1: value)
     auto fetch = [&](uint32_t k0, int32_t pages, lds_t to) {
-        constexpr uint32_t kApart = CT == PT_I8 ? kRawBytes : kTileBytes;
         const size_t offset = offset_of(k0, pages);
-        const uint32_t pk = 16 * (CT == PT_I8 ? chunk : chunk ^ swizzle_k<DIM>(first_row)), pv = 16 * (CT == PT_I8 ? chunk : chunk ^ swizzle_v<DIM>(first_row));
+        const uint32_t pk = 16 * (chunk ^ swizzle_k<DIM>(first_row)), pv = 16 * (chunk ^ swizzle_v<DIM>(first_row));
         lds_t const mine_to = to + wave * 1024;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
@@ -301,83 +320,93 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             const uint32_t add = row_at(offset, n, &base);
             const uint8_t *const kp = (const uint8_t *)a.pool.k + base, *const vp = (const uint8_t *)a.pool.v + base;
             __builtin_amdgcn_global_load_lds((gptr_t)(kp + (add + pk)), (lptr_t)(mine_to + n * 4096), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gptr_t)(vp + (add + pv)), (lptr_t)(mine_to + kApart + n * 4096), 16, 0, 0);
-        }
-        if (CT == PT_I8 && wave < 2) {
-            scale = pages < 0 ? INFINITY : (wave ? a.pool.vs : a.pool.ks)[offset / kRowBytes];
+            __builtin_amdgcn_global_load_lds((gptr_t)(vp + (add + pv)), (lptr_t)(mine_to + kTileBytes + n * 4096), 16, 0, 0);
         }
     };
-    // int8: what this wave fetched, from where it lies to fp16 tiles; and the steps. Those of values are multiples of a power of two
-    // that none exceeds; one that is not finite is taken out.
-    auto convert = [&](lds_t from, lds_t to) {
-        uint32_t me = lane;
-        asm volatile("" : "+v"(me));  // addresses are made anew: kept from tile to tile they would cost registers that the tile needs
-        const uint32_t chunk = me % kChunks;
+    // int8: into registers as it is stored, from where it goes to LDS as fp16 while the tile before is worked on (by way of LDS, and
+    // converted there between two barriers, 256 new tokens over 16384 keys took 176 us against 167; between the products, but
+    // with a barrier for keys and one for values, 182)
+    v4u raw[CT == PT_I8 ? kLoads : 1][2];
+    float scale = 0.0f;  // of key lane (wave 0: key, the others: value)
+    auto fetch_raw = [&](uint32_t k0, int32_t pages) {
+        const size_t offset = offset_of(k0, pages);
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const uint32_t rowk = (n * 4 + wave) * kRowsAt + me / kChunks;
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                const v4u w = *(const __attribute__((address_space(3))) v4u *)(from + kv * kRawBytes + wave * 1024 + n * 4096 + me * 16);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    v4u f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        f[i] = biased_to_f16(__builtin_amdgcn_perm(0x64646464u, w[2 * half + i / 2] ^ 0x80808080u, i & 1 ? 0x04030402 : 0x04010400));
-                    }
-                    const uint32_t piece = (2 * chunk + half) ^ (kv ? swizzle_v<DIM>(rowk) : swizzle_k<DIM>(rowk));
-                    *(__attribute__((address_space(3))) v4u *)(to + kv * kTileBytes + (rowk * kPieces + piece) * 16) = f;
-                }
-            }
+            size_t base;
+            const uint32_t add = row_at(offset, n, &base) + 16 * chunk;
+            raw[n][0] = *(const v4u *)((const uint8_t *)a.pool.k + base + add);
+            raw[n][1] = *(const v4u *)((const uint8_t *)a.pool.v + base + add);
         }
+        scale = (wave ? a.pool.vs : a.pool.ks)[offset / kRowBytes];
+        scale = pages < 0 ? INFINITY : scale;
+    };
+    // eight elements in each lane: piece p of 4 kLoads
+    uint32_t at_put_k = (first_row * kPieces + (2 * chunk ^ swizzle_k<DIM>(first_row))) * 16;
+    uint32_t at_put_v = (first_row * kPieces + (2 * chunk ^ swizzle_v<DIM>(first_row))) * 16;
+    auto convert = [&](int p, lds_t to) {
+        const int n = p / 4, kv = p / 2 % 2, half = p % 2;
+        const v4u w = raw[n][kv];
+        v4u f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[i] = biased_to_f16(__builtin_amdgcn_perm(0x64646464u, w[2 * half + i / 2] ^ 0x80808080u, i & 1 ? 0x04030402 : 0x04010400));
+        }
+        *(__attribute__((address_space(3))) v4u *)(to + kv * kTileBytes + n * 4 * kRowsAt * DIM * 2 + ((kv ? at_put_v : at_put_k) ^ (16 * half))) = f;
+    };
+    // The steps. Those of values are multiples of a power of two that none exceeds; one that is not finite is taken out.
+    auto put_steps = [&](StepsOfTile *to) {
         if (wave < 2) {
             float step = __builtin_amdgcn_rcpf(scale);
             if (wave == 1) {
                 const bool fine = step - step == 0.0f;  // neither infinite nor NaN
                 const unsigned long long not_fine = __ballot(!fine);
                 step = fine ? step : 0.0f;
-                float most = step;
-#pragma unroll
-                for (int off = 32; off; off >>= 1) {
-                    most = fmaxf(most, __shfl_xor(most, off, 64));
-                }
-                const float unit_of_tile = power_above(most);
+                const float unit_of_tile = power_above(wave_max_abs(step));
                 if (lane == 0) {
-                    *sBad = not_fine;
-                    *sUnit = unit_of_tile;
+                    to->bad = not_fine;
+                    to->unit = unit_of_tile;
                 }
                 step *= __builtin_amdgcn_rcpf(unit_of_tile);
             } else {
                 step *= score_scale;
             }
-            sStep[wave * kKeys + lane] = step;
+            to->step[wave][lane] = step;
         }
     };
 
     // where this lane reads in a tile: K pieces of row c, and for V (16 lanes read four keys of 16 d, lane e of them the d
-    // 4 (e % 4) .. + 3 of key e / 4, and get d e of all four)
-    uint32_t at_k[kSteps], at_v[kOut][2];
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-        at_k[st] = (c * kPieces + ((2 * st + h) ^ swizzle_k<DIM>(c))) * 16;
-    }
-#pragma unroll
-    for (int i = 0; i < kOut; ++i) {
-        const uint32_t e = lane & 15, sub = (lane >> 4) & 1, from = 4 * i + 2 * sub + e % 4 / 2;
+    // 4 (e % 4) .. + 3 of key e / 4, and get d e of all four); of the first step, the others' differ in two or three bits
+    static_assert(CT != PT_I8 || 4 * kLoads == kSteps, "a piece is converted at every step of the scores");
+    uint32_t at_k = (c * kPieces + (h ^ swizzle_k<DIM>(c))) * 16, at_v[2];
+    {
+        const uint32_t e = lane & 15, sub = (lane >> 4) & 1, from = 2 * sub + e % 4 / 2;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const uint32_t rowk = 4 * h + e / 4 + 8 * w;
-            at_v[i][w] = (rowk * kPieces + (from ^ swizzle_v<DIM>(rowk))) * 16 + 8 * (e % 2);
+            at_v[w] = (rowk * kPieces + (from ^ swizzle_v<DIM>(rowk))) * 16 + 8 * (e % 2);
         }
     }
 
     int32_t pages = -1, next = -1;
+    unsigned long long stored = 0;  // (bit i) key i of the tile has a page
     if (t0 < t1) {
         const uint32_t k0 = all.lo + t0 * kKeys;
         pages = page_of(k0, look_up(k0));
         next = look_up(k0 + kKeys);
-        fetch(k0, pages, CT == PT_I8 ? sTiles + 2 * kTileBytes : sTiles);
+        if (CT == PT_I8) {
+            fetch_raw(k0, pages);
+            stored = __ballot(pages >= 0);
+            pages = page_of(k0 + kKeys, next);
+            next = look_up(k0 + 2 * kKeys);
+#pragma unroll
+            for (int p = 0; p < 4 * kLoads; ++p) {
+                convert(p, sTiles);
+            }
+            put_steps(sSteps);
+            fetch_raw(k0 + kKeys, pages);
+        } else {
+            fetch(k0, pages, sTiles);
+        }
     }
     // queries (while the first tile is on its way)
     {
@@ -416,22 +445,22 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
     }
 
-    // One tile: `now` holds it, `ahead` is where the next one goes (int8: where this one lies as it is stored, too). (The compiler has to know that the two are apart, else it waits
-    // for the next tile's arrival before it reads this one.)
+    // One tile: `now` holds it, `ahead` is where the next one goes. (16-bit caches: the compiler has to know that the two are apart,
+    // else it waits for the next tile's arrival before it reads this one.)
     auto step_over = [&](uint32_t t, __attribute__((address_space(3))) uint8_t *__restrict now,
-                         __attribute__((address_space(3))) uint8_t *__restrict ahead) {
+                         __attribute__((address_space(3))) uint8_t *__restrict ahead, const StepsOfTile *steps, StepsOfTile *steps_ahead) {
         const uint32_t k0 = all.lo + t * kKeys;
-        const unsigned long long stored = __ballot(pages >= 0);
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile is there
-        __syncthreads();                     // everyone's; and everyone is done with the tile before
         if (CT == PT_I8) {
-            convert(ahead, now);
-            __syncthreads();
-        }
-        pages = page_of(k0 + kKeys, next);
-        next = look_up(k0 + 2 * kKeys);
-        if (t + 1 < t1) {
-            fetch(k0 + kKeys, pages, ahead);
+            barrier();  // the tile is there; and everyone is done with the tile before
+        } else {
+            stored = __ballot(pages >= 0);
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile is there
+            __syncthreads();                     // everyone's; and everyone is done with the tile before
+            pages = page_of(k0 + kKeys, next);
+            next = look_up(k0 + 2 * kKeys);
+            if (t + 1 < t1) {
+                fetch(k0 + kKeys, pages, ahead);
+            }
         }
         // does every row of the workgroup see every key of the tile?
         const bool whole = stored == ~0ull && k0 + kKeys <= all_hi && k0 >= all_lo;
@@ -491,10 +520,14 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
         constexpr int kRing = CT == PT_I8 || kWide ? 3 : 4;  // pairs of reads under way
         V kf[kRing][2];
+        uint32_t from = at_k;
+        if (CT == PT_I8) {
+            asm volatile("" : "+v"(from));  // addresses are made anew: kept from tile to tile they would cost registers that the tile needs
+        }
         auto keys = [&](int st) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                kf[st % kRing][i] = *(const __attribute__((address_space(3))) V *)(now + i * 32 * DIM * 2 + at_k[st]);
+                kf[st % kRing][i] = *(const __attribute__((address_space(3))) V *)(now + i * 32 * DIM * 2 + (from ^ 32 * st));
             }
         };
 #pragma unroll
@@ -516,6 +549,18 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 keys(st + kRing);
                 in_order();
             }
+            if (CT == PT_I8) {
+                convert(st, ahead);
+                in_order();
+            }
+        }
+        const unsigned long long stored_here = stored;
+        if (CT == PT_I8) {
+            put_steps(steps_ahead);
+            stored = __ballot(pages >= 0);
+            pages = page_of(k0 + 2 * kKeys, next);
+            next = look_up(k0 + 3 * kKeys);
+            fetch_raw(k0 + 2 * kKeys, pages);
         }
         V vv[2][kOut], ph[2], pl[2];
         Words<4> pw[2];
@@ -524,8 +569,8 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             struct {
                 v4s a, b;
             } w;
-            w.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(base + at_v[i][0]));
-            w.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(base + at_v[i][1]));
+            w.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(base + (at_v[0] ^ 64 * i)));
+            w.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(base + (at_v[1] ^ 64 * i)));
             vv[u & 1][i] = __builtin_bit_cast(V, w);
         };
 #pragma unroll
@@ -534,23 +579,28 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
         in_order();
         if (CT == PT_I8) {
+            v4f ks[3];
+            auto read = [&](int x) { ks[x % 3] = *(const v4f *)(steps->step[0] + 32 * (x / 4) + 8 * (x % 4) + 4 * h); };
+            read(0);
+            read(1);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const v4f ks = *(const v4f *)(sStep + 32 * i + 2 * j + 4 * h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[i][j + e] *= ks[e];
-                    }
+            for (int x = 0; x < 8; ++x) {
+                if (x + 2 < 8) {
+                    read(x + 2);
                 }
+                in_order();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[x / 4][4 * (x % 4) + e] *= ks[x % 3][e];
+                }
+                in_order();
             }
         }
         unsigned long long seen = ~0ull;
         if (!whole) {
             const uint32_t from = span.lo > k0 ? span.lo - k0 : 0, upto = span.hi > k0 ? span.hi - k0 : 0;  // keys of the tile this row sees
             seen = from >= kKeys || upto <= from ? 0 : (upto >= kKeys ? ~0ull : (1ull << upto) - 1) & (~0ull << from);
-            seen &= stored;
+            seen &= stored_here;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t half = (uint32_t)(seen >> (32 * i)) >> (4 * h);
@@ -567,7 +617,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             top = max_of(top, s[0][j], s[1][j]);
         }
         top *= xscale;
-        const float tile_unit = CT == PT_I8 ? *sUnit : 1.0f;
+        const float tile_unit = CT == PT_I8 ? steps->unit : 1.0f;
         if (__any(top > m + kSlack || (CT == PT_I8 && tile_unit > unit))) {
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const float up = fmaxf(top, m);
@@ -577,7 +627,9 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             if (CT == PT_I8) {
                 const float was = unit;
                 unit = fmaxf(tile_unit, unit);
-                corr *= was * __builtin_amdgcn_rcpf(unit);
+                float now_unit = unit;
+                asm volatile("" : "+v"(now_unit));  // (else the reciprocal below is shared with this one, and the way round this block copies the outputs)
+                corr *= was * __builtin_amdgcn_rcpf(now_unit);
             }
 #pragma unroll
             for (int i = 0; i < kOut; ++i) {
@@ -591,17 +643,22 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         const float shift = (CT == PT_I8 ? kLift + __builtin_amdgcn_logf(part) : kLift) - m;
         float sum = 0.0f;
         float p[8];
+        v4f vs[2][2];  // int8: steps of this group's and the next one's values
+        auto steps_of = [&](int u) {
+            vs[u & 1][0] = *(const v4f *)(steps->step[1] + 16 * u + 4 * h);
+            vs[u & 1][1] = *(const v4f *)(steps->step[1] + 16 * u + 8 + 4 * h);
+        };
+        if (CT == PT_I8) {
+            steps_of(0);
+            steps_of(1);
+        }
         auto weight = [&](int u, int j) {  // j and j + 1
-            v2f vs;
-            if (CT == PT_I8) {
-                vs = *(const v2f *)(sStep + kKeys + 16 * u + 8 * (j / 4) + 4 * h + j % 4);
-            }
 #pragma unroll
             for (int e = j; e < j + 2; ++e) {
                 p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u % 2) + e], xscale, shift));
                 if (CT == PT_I8) {
                     sum += p[e];
-                    p[e] *= vs[e - j];
+                    p[e] *= vs[u & 1][e / 4][e % 4];
                 } else if (kWide) {
                     l += p[e];
                 }
@@ -644,6 +701,9 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                     }
                     if (i == kOut - 1) {
                         ready(u + 1);
+                        if (CT == PT_I8 && u < 2) {
+                            steps_of(u + 2);
+                        }
                     }
                     in_order();
                 }
@@ -651,16 +711,29 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
         if (CT == PT_I8) {
             l += sum * __builtin_amdgcn_rcpf(part);
-            poisoned |= (*sBad & seen) != 0;
+            poisoned |= (steps->bad & seen) != 0;
         }
     };
-    for (uint32_t t = t0; t < t1; t += 2) {
-        step_over(t, sTiles, sTiles + 2 * kTileBytes);
-        if (t + 1 < t1) {
-            if (CT == PT_I8) {
-                step_over(t + 1, sTiles, sTiles + 2 * kTileBytes);
-            } else {
-                step_over(t + 1, sTiles + 2 * kTileBytes, sTiles);
+    if (CT == PT_I8) {
+        // (One body, the buffers told apart by a bit of the addresses. Two, as below, take more registers than there are: 177 us
+        // against 157 for 256 new tokens over 16384 keys.)
+        auto other = [&] {
+            at_put_k ^= 2 * kTileBytes;
+            at_put_v ^= 2 * kTileBytes;
+        };
+        other();
+        for (uint32_t t = t0, at = 0; t < t1; ++t, at ^= 1) {
+            step_over(t, sTiles, sTiles, sSteps + at, sSteps + (at ^ 1));
+            other();
+            at_k ^= 2 * kTileBytes;
+            at_v[0] ^= 2 * kTileBytes;
+            at_v[1] ^= 2 * kTileBytes;
+        }
+    } else {
+        for (uint32_t t = t0; t < t1; t += 2) {
+            step_over(t, sTiles, sTiles + 2 * kTileBytes, nullptr, nullptr);
+            if (t + 1 < t1) {
+                step_over(t + 1, sTiles + 2 * kTileBytes, sTiles, nullptr, nullptr);
             }
         }
     }

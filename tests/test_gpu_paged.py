@@ -331,6 +331,20 @@ def test_scales_below_zero_and_of_zero(prompt, act, cache):
         assert_attention(attend(c, prompt, scale=scale), c, scale)
 
 
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+def test_scales_of_an_int8_cache_of_either_sign_and_any_size(act, prompt):
+    """real = stored / scale, whatever the scale is: negative ones, and values 2^40 apart, the largest steps among the last keys"""
+    c = Case(act, "i8", 4, 2, 64, 16, (150, 40), (20, 1) if prompt else (1, 1), seed=32)
+    g = torch.Generator().manual_seed(33)
+    sign = 1 - 2 * torch.randint(0, 2, c.vs.shape, generator=g)
+    c.ks, c.vs = c.ks * sign, c.vs * sign.roll(1, 0)
+    assert_attention(attend(c, prompt), c)
+    c.vs = c.vs * 2.0 ** torch.randint(-20, 21, c.vs.shape, generator=g)
+    c.vs[c.table[0, :2].long()] *= 2.0 ** 30                                   # small values first
+    assert_attention(attend(c, prompt), c)
+
+
 @pytest.mark.parametrize("cache_type", ["f16", "i8"])
 def test_sequences_that_share_pages(cache_type):
     """a common beginning in the same pages, once in one sequence's own order and once twice in one table"""
