@@ -299,7 +299,9 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
                         wide = fmaxf(wide, __shfl_xor(wide, off, 64));
                     }
                     unit = power_above(wide);
-                    corr *= was * __builtin_amdgcn_rcpf(unit);
+                    float now_unit = unit;
+                    asm volatile("" : "+v"(now_unit));  // (else the reciprocal below is shared with this one, and the way round this block copies the outputs)
+                    corr *= was * __builtin_amdgcn_rcpf(now_unit);
                 }
 #pragma unroll
                 for (int t = 0; t < kVec; ++t) {
