@@ -14,7 +14,7 @@
 // 2^15, inside fp16; a weight of less than 2^-37 of the row's largest is lost. An int8 cache's steps (1 / scale) are part of
 // the weights, divided by a power of two that no step exceeds, so that they add nothing to that range.
 //
-// The tiles (of 128 keys) of all sequences stand in one row that is cut into equal shares, as many as workgroups fit the chip:
+// The tiles (of 128 keys) of all sequences stand in one row that is cut into equal shares, one to a workgroup, which fill the chip once:
 // every workgroup reads the same number of bytes, whatever the lengths are. They are read on the device, so a captured launch
 // serves any. A share may hold the end of one sequence, whole ones, and the beginning of another; a sequence that lies in one
 // share is written out, one that several hold leaves (maximum, sum, output) parts, which a second launch joins.
@@ -28,7 +28,7 @@ constexpr uint32_t kCus = 256;
 constexpr uint32_t kTileShift = 7;   // keys of one round of a workgroup's four waves: 128
 constexpr uint32_t kLeast = 1;       // fewest tiles in a share
 
-// workgroups of this kernel that a CU holds (registers)
+// workgroups of this kernel that a CU can hold (registers)
 template <int DIM>
 constexpr uint32_t per_cu()
 {
@@ -474,11 +474,10 @@ uint32_t columns(uint32_t heads, uint32_t kv_heads)
     return kv_heads * ((heads / kv_heads + 15) / 16);
 }
 
-// Shares of a column: of the numbers that fill the chip once to four times, the first that leaves no more than a tenth idle,
-// or else the one that leaves least.
-uint32_t shares_of(uint32_t heads, uint32_t kv_heads, uint32_t dim)
+// Shares of n columns with `fit` workgroups at a time: of the numbers that fill the chip once to four times, the first that
+// leaves no more than a tenth idle, or else the one that leaves least.
+uint32_t shares_of(uint32_t n, uint32_t fit)
 {
-    const uint32_t n = columns(heads, kv_heads), fit = kCus * (dim == 128 ? per_cu<128>() : per_cu<64>());
     uint32_t best = 1;
     double used = 0.0;
     for (uint32_t r = 1; r <= 4 && used < 0.9; ++r) {
@@ -489,6 +488,32 @@ uint32_t shares_of(uint32_t heads, uint32_t kv_heads, uint32_t dim)
         }
     }
     return best;
+}
+
+uint32_t most_per_cu(uint32_t dim)
+{
+    return dim == 128 ? per_cu<128>() : per_cu<64>();
+}
+
+// Workgroups that a CU is given. Where memory is what bounds it, one (head size 64: two, whose loads are half as large) brings
+// the bytes as fast as more, and leaves fewer parts to write and join: head size 128, one against two, 32 requests fp16 50.0
+// and 50.9 us, 64 int8 106.6 and 109.4, two long ones bf16 145.6 and 150.2, seven heads to a key head 29.3 and 32.6; head
+// size 64, two against three, fp32 over fp16 30.6 and 34.6, long bf16 81 and 84, 64 requests fp16 55.9 and 54.7. What an int8
+// cache has to be converted for with smaller heads, and for fp32's two parts, takes one more: head size 128, fp32, 36.2
+// against 38.9 with one; head size 64 37.8 against 40.2 with two. More waves than that spill or stand idle: head size 128,
+// three, 85 us for 32 requests; head size 64, four, 62.
+uint32_t wanted_per_cu(int act, int type, uint32_t dim)
+{
+    return (dim == 128 ? 1 : 2) + (type == PT_I8 && (act == PT_F32 || dim == 64));
+}
+
+// Few tiles, as far as the page table's width says, are spread over all that fit: eight requests of up to 2000 keys 14.3 us
+// against 15.0.
+uint32_t shares_for(const PagedAttentionArgs &a)
+{
+    const uint32_t n = columns(a.heads, a.pool.kv_heads), all = shares_of(n, kCus * most_per_cu(a.pool.dim));
+    const uint64_t tiles = (uint64_t)a.batch.batch * ((((uint64_t)a.batch.max_pages << a.pool.shift) >> kTileShift) + 1);
+    return tiles <= 2 * (uint64_t)all ? all : shares_of(n, kCus * wanted_per_cu(a.act, a.pool.type, a.pool.dim));
 }
 
 uint32_t tile_shift(const PagedPool &pool, const PagedBatch &b)
@@ -504,7 +529,7 @@ template <int ACT, int CT, int DIM>
 struct Decode {
     static hipError_t run(const PagedAttentionArgs &a, hipStream_t st)
     {
-        const uint32_t shares = shares_of(a.heads, a.pool.kv_heads, DIM), shift = tile_shift(a.pool, a.batch);
+        const uint32_t shares = shares_for(a), shift = tile_shift(a.pool, a.batch);
         const dim3 grid(shares, columns(a.heads, a.pool.kv_heads));
         if (a.pool.shift >= 4) {
             hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, true>), grid, dim3(256), 0, st, a, shares, shift);
@@ -525,7 +550,13 @@ struct Decode {
 
 size_t paged_decode_workspace(const PagedPool &pool, uint32_t heads)
 {
-    return (size_t)columns(heads, pool.kv_heads) * shares_of(heads, pool.kv_heads, pool.dim) * 2 * 16 * (pool.dim + 2) * sizeof(float);
+    const uint32_t n = columns(heads, pool.kv_heads);
+    uint32_t shares = 0;  // the most that a call may take
+    for (uint32_t per = 1; per <= most_per_cu(pool.dim); ++per) {
+        const uint32_t s = shares_of(n, kCus * per);
+        shares = s > shares ? s : shares;
+    }
+    return (size_t)n * shares * 2 * 16 * (pool.dim + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_decode(const PagedAttentionArgs &a, hipStream_t st)
