@@ -88,8 +88,12 @@ struct Step {
     uint32_t seen;
 };
 
-// PAGE16: pages of 16 keys and more, so that each 16-key half of a step lies in one page and its address is the wave's.
-template <int ACT, int CT, int DIM, bool PAGE16>
+// PAGE16: pages of 16 keys and more, so that each 16-key half of a step lies in one page and its address is the wave's (32 requests
+// fp16 50.9 us; with an address per lane, as smaller pages need it, 77.3).
+// ONCE: up to 16 heads share a key head, so that one workgroup reads a key for all of them, past the caches; more take a
+// workgroup per 16, which find it there (head size 128: 32 heads over 8, long bf16, 145 us past them and 166 through them;
+// 64 over 2 66.6 and 55.1, 71 over 1 102 and 90).
+template <int ACT, int CT, int DIM, bool PAGE16, bool ONCE>
 __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedAttentionArgs a, uint32_t shares, uint32_t shift)
 {
     typedef CacheOperand<CT> Op;
@@ -202,11 +206,11 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    Op::load_k(kb[h] + c * kRowBytes, g, n.kr[h]);
+                    Op::template load_k<ONCE>(kb[h] + c * kRowBytes, g, n.kr[h]);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    n.vr[j] = Op::template load_v<DIM>(vb[j >> 2] + (4 * g + (j & 3)) * kRowBytes, c);
+                    n.vr[j] = Op::template load_v<ONCE, DIM>(vb[j >> 2] + (4 * g + (j & 3)) * kRowBytes, c);
                 }
                 if (!whole) {
 #pragma unroll
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t key = k0 + 16 * h + c;
                     int64_t slot = key < to ? paged_slot(table, key, a.pool.shift, a.pool.pages, a.pool.kv_heads, kvh) : -1;
-                    Op::load_k((const uint8_t *)a.pool.k + (slot < 0 ? 0 : slot) * kRowBytes, g, n.kr[h]);
+                    Op::template load_k<ONCE>((const uint8_t *)a.pool.k + (slot < 0 ? 0 : slot) * kRowBytes, g, n.kr[h]);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
                         n.seen &= ~(1u << j);
                         slot = 0;
                     }
-                    n.vr[j] = Op::template load_v<DIM>((const uint8_t *)a.pool.v + slot * kRowBytes, c);
+                    n.vr[j] = Op::template load_v<ONCE, DIM>((const uint8_t *)a.pool.v + slot * kRowBytes, c);
                     if (CT == PT_I8) {
                         n.ksc[j >> 2][j & 3] = a.pool.ks[slot];
                         n.vsc[j >> 2][j & 3] = a.pool.vs[slot];
@@ -531,11 +535,10 @@ struct Decode {
     {
         const uint32_t shares = shares_for(a), shift = tile_shift(a.pool, a.batch);
         const dim3 grid(shares, columns(a.heads, a.pool.kv_heads));
-        if (a.pool.shift >= 4) {
-            hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, true>), grid, dim3(256), 0, st, a, shares, shift);
-        } else {
-            hipLaunchKernelGGL((paged_decode_kernel<ACT, CT, DIM, false>), grid, dim3(256), 0, st, a, shares, shift);
-        }
+        const bool once = a.heads / a.pool.kv_heads <= 16;
+        const auto kernel = a.pool.shift >= 4 ? (once ? paged_decode_kernel<ACT, CT, DIM, true, true> : paged_decode_kernel<ACT, CT, DIM, true, false>)
+                                              : (once ? paged_decode_kernel<ACT, CT, DIM, false, true> : paged_decode_kernel<ACT, CT, DIM, false, false>);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a, shares, shift);
         const hipError_t e = hipGetLastError();
         // a sequence that fits the smallest share and stands alone is never cut
         if (e != hipSuccess || (a.batch.batch == 1 && a.batch.max_pages << a.pool.shift <= kLeast << shift)) {

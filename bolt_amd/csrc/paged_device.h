@@ -197,25 +197,31 @@ struct Words<4> {
     uint32_t w[4];
 };
 
-// (read once: past the caches. A 2 GiB read goes at 7.0 TB/s so, at 6.2 through them.)
-template <int W>
+// ONCE: nobody else reads it, past the caches (a read of 2 GiB goes at 7.0 TB/s so, at 6.2 through them)
+template <bool ONCE, typename T>
+__device__ __forceinline__ T load_as(const void *p)
+{
+    return ONCE ? __builtin_nontemporal_load((const T *)p) : *(const T *)p;
+}
+
+template <int W, bool ONCE>
 __device__ __forceinline__ Words<W> load_words(const void *p)
 {
     Words<W> r;
     if (W == 4) {
-        const v4u v = __builtin_nontemporal_load((const v4u *)p);
+        const v4u v = load_as<ONCE, v4u>(p);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             r.w[i] = v[i];
         }
     } else if (W == 2) {
-        const v2u v = __builtin_nontemporal_load((const v2u *)p);
+        const v2u v = load_as<ONCE, v2u>(p);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             r.w[i] = v[i];
         }
     } else {
-        r.w[0] = __builtin_nontemporal_load((const uint32_t *)p);
+        r.w[0] = load_as<ONCE, uint32_t>(p);
     }
     return r;
 }
@@ -304,17 +310,17 @@ struct CacheOperand : Operand<CT> {
     using RawV = Words<DIM / 32>;
     static constexpr int kRawK(int dim) { return dim / 32; }
     static __device__ __forceinline__ uint32_t d_of(uint32_t s, uint32_t g) { return 32 * s + 8 * g; }
-    template <int N>
+    template <bool ONCE, int N>
     static __device__ __forceinline__ void load_k(const uint8_t *row, uint32_t g, Raw (&r)[N])
     {
 #pragma unroll
         for (int s = 0; s < N; ++s) {
-            r[s] = load_words<4>(row + 2 * d_of(s, g));
+            r[s] = load_words<4, ONCE>(row + 2 * d_of(s, g));
         }
     }
     static __device__ __forceinline__ V k_operand(const Raw *r, int s) { return __builtin_bit_cast(V, r[s]); }
-    template <int DIM>
-    static __device__ __forceinline__ RawV<DIM> load_v(const uint8_t *row, uint32_t c) { return load_words<DIM / 32>(row + c * (DIM / 8)); }
+    template <bool ONCE, int DIM>
+    static __device__ __forceinline__ RawV<DIM> load_v(const uint8_t *row, uint32_t c) { return load_words<DIM / 32, ONCE>(row + c * (DIM / 8)); }
     template <int DIM>
     static __device__ __forceinline__ RawV<DIM> zero_v() { return zero_words<DIM / 32>(); }
     template <int DIM>
@@ -351,12 +357,12 @@ struct CacheOperand<PT_I8> : Operand<PT_I8> {
     using RawV = Words<DIM / 64>;
     static constexpr int kRawK(int dim) { return dim / 64; }
     static __device__ __forceinline__ uint32_t d_of(uint32_t s, uint32_t g) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); }
-    template <int N>
+    template <bool ONCE, int N>
     static __device__ __forceinline__ void load_k(const uint8_t *row, uint32_t g, Raw (&r)[N])
     {
 #pragma unroll
         for (int s = 0; s < N; ++s) {
-            r[s] = load_words<4>(row + d_of(2 * s, g));
+            r[s] = load_words<4, ONCE>(row + d_of(2 * s, g));
         }
     }
     static __device__ __forceinline__ V k_operand(const Raw *r, int s)
@@ -368,8 +374,8 @@ struct CacheOperand<PT_I8> : Operand<PT_I8> {
         }
         return __builtin_bit_cast(V, w);
     }
-    template <int DIM>
-    static __device__ __forceinline__ RawV<DIM> load_v(const uint8_t *row, uint32_t c) { return load_words<DIM / 64>(row + c * (DIM / 16)); }
+    template <bool ONCE, int DIM>
+    static __device__ __forceinline__ RawV<DIM> load_v(const uint8_t *row, uint32_t c) { return load_words<DIM / 64, ONCE>(row + c * (DIM / 16)); }
     template <int DIM>
     static __device__ __forceinline__ RawV<DIM> zero_v() { return zero_words<DIM / 64>(); }
     template <int DIM>

@@ -69,7 +69,7 @@ def test_loops_stay_in_registers(prompt, decode):
     (two parts each) over int8 rows of 128, which have a few registers too many"""
     for asm, kernel in ((prompt, "paged_prompt_kernel"), (decode, "paged_decode_kernel")):
         found = {n: r for n, r in resources(asm).items() if kernel in n and "NumVgprs" in r}
-        assert len(found) == 24, sorted(found)
+        assert len(found) == (48 if kernel == "paged_decode_kernel" else 24), sorted(found)
         for n, r in found.items():
             wide = kernel == "paged_prompt_kernel" and args(n) == (0, 3, 128)
             assert r["ScratchSize"] <= (64 if wide else 0), (n, r)
