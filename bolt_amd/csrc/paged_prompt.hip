@@ -15,10 +15,11 @@
 // before theirs (a tile waits for one barrier and no load); its steps multiply scores and weights.
 //
 // What it costs. A wave issues 32 products of 32x32x16 a tile (head size 128; 36.5 cycles each alone, 44 with real data,
-// when the power limit lowers the clock) and some 250 vector instructions and 32 exponentials, and it does not overlap its
-// own products with them: two waves on every SIMD, from two workgroups, do. One prompt of 8192 tokens, 32 heads over 8, runs
-// at 1.0 PFLOP/s, where the library's 8192^3 product of the same type reaches 1.2. Head size 128 takes 220 to 230 registers
-// of the 256 that two waves leave each; more rows to a wave would halve the reads of LDS and do not fit.
+// when the clock falls) and some 200 vector instructions (int8: 390), 32 of them exponentials, and it does not overlap its
+// own products with them: two waves on every SIMD, from two workgroups, do. One prompt of 8192 tokens, 32 heads over 8, bf16,
+// takes 0.55 ms, 1.0 PFLOP/s, where the library's 8192^3 product of the same type reaches 1.2; 2 x 256 tokens over 27 k
+// int8 keys 0.156 ms, 0.72 PFLOP/s. Head size 128 takes 220 to 230 registers of the 256 that two waves leave each; more
+// rows to a wave would halve the reads of LDS and do not fit.
 // Where few tiles meet many keys, several workgroups share a tile's keys and a second launch joins their parts.
 #include <atomic>
 
@@ -36,7 +37,10 @@ typedef __attribute__((address_space(3))) void *lptr_t;
 typedef __attribute__((address_space(3))) uint8_t *lds_t;
 
 constexpr uint32_t kRows = 128, kKeys = 64;
-constexpr uint32_t kSpread = 512;  // workgroups below which a tile's keys are shared out
+// Workgroups (two a CU) below which a tile's keys are shared out, over about so many. 256 new tokens over 16384 int8 keys, 128 tiles
+// of rows: 153 us with 512, 204 with 256 (half the chip idle), 174 with 1024 (more parts written and read). Eight ragged
+// prompts of up to 1025 tokens have more tiles than that: 99 us with whole tiles, 153 with their keys cut in two.
+constexpr uint32_t kSpread = 512;
 constexpr uint32_t kLeast = 4;     // fewest key tiles per share
 constexpr float kLow = -1.7e38f;
 constexpr float kSlack = 2.0f, kLift = 13.0f;
@@ -288,7 +292,8 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     auto look_up = [&](uint32_t k0) -> int32_t { return table[min(k0 + lane, all.hi - 1) >> a.pool.shift]; };
     auto page_of = [&](uint32_t k0, int32_t found) -> int32_t { return k0 + lane < all.hi && (uint32_t)found < a.pool.pages ? found : -1; };
     // A wave's load n covers kRowsAt rows of the tile, from row (4n + wave) kRowsAt on. In pages of so many keys and more (PAGED) they
-    // lie side by side, so that their address is the wave's and what a lane adds to it is the same for every load. A key without
+    // lie side by side, so that their address is the wave's and what a lane adds to it is the same for every load (8192 tokens bf16
+    // 536 us; with an address per lane, as smaller pages need it, 568). A key without
     // a page is read from page 0: what it brings is masked, and taken out of the tile where it is not finite.
     constexpr uint32_t kRowsAt = rows_at<CT, DIM>(), kChunks = kRowBytes / 16;
     const uint32_t in_row = lane / kChunks, chunk = lane % kChunks;

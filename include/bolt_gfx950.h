@@ -554,8 +554,10 @@ EE bolt_gfx950_kv_cache_append(const BoltPagedKvCache *cache, const BoltPagedBat
     const BoltRotary *rotary);
 /* out = softmax(scale * q K^T) V per head, head h reading the keys of head h / (heads / kvHeads). A token at position p sees
  * the keys 0 .. p of its sequence, with window > 0 the last `window` of them; a row that sees no key becomes zeros. What the
- * cache holds elsewhere has no influence, infinities and NaN included. Scores, the softmax and its sums are fp32; with
- * fp32 activations every product is accurate to fp32 too. The result does not depend on what else is in the batch run
+ * cache holds elsewhere has no influence, infinities and NaN included; where a row sees a key or value that is infinite or NaN
+ * (or an int8 slot with a scale of zero or NaN), it shows what the formula makes of it, or NaN. An int8 slot stands for
+ * stored / scale, of either sign. fp32 numbers below the smallest normal one may count as zeros. Scores, the softmax and
+ * its sums are fp32; fp32 activations go into the products in two 16-bit parts (a relative error of 2^-21). The result does not depend on what else is in the batch run
  * beyond fp32 rounding of how the keys are split; the same call gives the same bytes.
  *   decode  one new token per sequence (offsets == NULL): the keys are split over the machine and the parts joined
  *   prompt  any number of new tokens per sequence (offsets != NULL), each seeing those before it; they must be stored
