@@ -30,7 +30,6 @@ namespace {
 
 constexpr uint32_t kCus = 256;
 constexpr uint32_t kTileShift = 7;   // keys of one round of a workgroup's four waves: 128
-constexpr uint32_t kLeast = 1;       // fewest tiles in a share
 
 // workgroups of this kernel that a CU can hold (registers)
 template <int DIM>
@@ -59,8 +58,7 @@ __device__ __forceinline__ uint32_t tiles_of(const PagedAttentionArgs &a, uint32
 // tiles per share, with `shares` of them to a key head's column
 __device__ __forceinline__ uint32_t tiles_per_share(uint32_t tiles, uint32_t shares)
 {
-    const uint32_t per = (tiles + shares - 1) / shares;
-    return per < kLeast ? kLeast : per;
+    return (tiles + shares - 1) / shares;
 }
 
 // A part: 16 rows of DIM values, 16 maxima, 16 sums. A share leaves two at most: of the sequence that its first tile belongs to
@@ -544,8 +542,8 @@ struct Decode {
                                               : (once ? paged_decode_kernel<ACT, CT, DIM, false, true> : paged_decode_kernel<ACT, CT, DIM, false, false>);
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a, shares, shift);
         const hipError_t e = hipGetLastError();
-        // a sequence that fits the smallest share and stands alone is never cut
-        if (e != hipSuccess || (a.batch.batch == 1 && a.batch.max_pages << a.pool.shift <= kLeast << shift)) {
+        // sequences of one tile are never cut
+        if (e != hipSuccess || a.batch.max_pages << a.pool.shift <= 1u << shift) {
             return e;
         }
         hipLaunchKernelGGL((paged_join_kernel<ACT, DIM>), dim3(a.heads, a.batch.batch), dim3(256), 0, st, a, shares, shift);

@@ -1,6 +1,7 @@
 """Host-side mirrors of the paged key / value cache entry points on torch CUDA tensors: append with position rotation,
 attention of one new token per sequence, attention of prompts. All arithmetic is in libbolt_gfx950.so; the calls enqueue
-on the library's stream (bolt_gfx950_set_stream) and return. What they allocate belongs to that stream.
+on the library's stream (bolt_gfx950_set_stream) and return. What they allocate belongs to that stream. For inference:
+nothing is recorded for a gradient.
 
     cache = PagedKvCache(k, v)                                   # [pages, kv_heads, page_size, head_dim]
     batch = PagedBatch(page_table, lengths)                      # lengths include the new tokens

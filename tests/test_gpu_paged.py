@@ -191,6 +191,7 @@ DECODE = [
     (40, 2, 128, 128, (700, 129), 100),
     (3, 3, 64, 4096, (1, 4097, 515), 33),
     (16, 8, 128, 64, (2500, 1, 0, 640), 1),
+    (8, 2, 128, 16, (5, 128, 0, 77), 0),                                       # a table of one tile
     (71, 1, 64, 16, (40, 90), 0),                                              # five tiles of queries, the last of seven
     (1024, 1024, 64, 16, (5, 140), 0),                                         # more columns than workgroups fit the chip
     (16, 16, 128, 16, tuple(i * 37 % 400 for i in range(67)), 0),              # shares that hold several sequences and parts of others
@@ -572,6 +573,37 @@ def test_captured_prompts_replayed_with_other_lengths(act, cache_type):
             assert torch.equal(bits(eager), bits(out))
     finally:
         capi.check(capi.lib().bolt_gfx950_set_stream(None), "set_stream")
+
+
+def test_first_call_of_a_kind_inside_a_capture():
+    """a process that has called bolt_gfx950_init and nothing else"""
+    import subprocess
+    import sys
+    code = """
+import sys; sys.path[:0] = %r
+import torch
+from bolt_amd import capi, host_paged as hp
+from checkers_paged import Case, assert_attention
+capi.check(capi.lib().bolt_gfx950_init(), "init")
+c = Case("f16", "f16", 4, 2, 64, 16, (50, 7), (20, 1), seed=34)
+cache, batch, q = c.gpu()
+out, side = torch.zeros_like(q), torch.cuda.Stream()
+ws = hp.paged_attention_workspace(cache, batch, 4)
+torch.cuda.synchronize()
+capi.check(capi.lib().bolt_gfx950_set_stream(side.cuda_stream), "set_stream")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    hp.paged_attention_prompt(cache, batch, q, out=out, workspace=ws)
+for _ in range(3):
+    out.zero_()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert_attention(out, c)
+print("captured")
+""" % (sys.path,)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
 
 
 def test_two_threads_at_once():
