@@ -47,7 +47,7 @@ __device__ __forceinline__ PagedSpan span_of(const PagedAttentionArgs &a, uint32
 }
 
 // Tiles of a sequence, counted from its first key rounded down to a step of 32; one where there is nothing to see (somebody
-// has to write the zeros). shift: kTileShift, more where the launch could have 2^31 of them.
+// has to write the zeros). shift: kTileShift, more where sequences are left whole or the launch could have 2^31 tiles.
 __device__ __forceinline__ uint32_t tiles_of(const PagedAttentionArgs &a, uint32_t b, uint32_t shift)
 {
     const PagedSpan s = span_of(a, b);
@@ -522,10 +522,29 @@ uint32_t shares_for(const PagedAttentionArgs &a)
     return tiles <= 2 * (uint64_t)all ? all : shares_of(n, kCus * wanted_per_cu(a.act, a.pool.type, a.pool.dim));
 }
 
-uint32_t tile_shift(const PagedPool &pool, const PagedBatch &b)
+// keys that a sequence sees at most, from its first one rounded down to a step of 32 on
+uint64_t most_seen(const PagedAttentionArgs &a)
 {
+    const uint64_t all = (uint64_t)a.batch.max_pages << a.pool.shift, in_window = (uint64_t)a.window + 31;
+    return a.window && in_window < all ? in_window : all;
+}
+
+// Sequences of few keys are left whole, a workgroup to each and nothing to join, where they fill the chip all the same: up to 512
+// keys (head size 128, 8 key heads, fp16, 32 sequences of up to 300 keys 9.6 us against 14.0 with their keys cut, 64 of up to
+// 500 21.4 against 27.1, a window of 300 11.6 against 17.7; head size 64, 12 heads, fp32, 32 of up to 300 9.9 and 12.8), and up to
+// 1024 where they also fill what a CU is given (32 of up to 1000 19.5 and 21.6, a window of 1000 23.7 and 30.4; head size 64,
+// where they do not, 20.1 and 19.2). Longer ones differ too much in length: 64 of up to 2000 keys 66.7 and 54.8.
+bool whole(const PagedAttentionArgs &a)
+{
+    const uint64_t seen = most_seen(a), groups = (uint64_t)a.batch.batch * columns(a.heads, a.pool.kv_heads);
+    return (seen <= 512 + 31 && groups >= kCus) || (seen <= 1024 + 31 && groups >= kCus * wanted_per_cu(a.act, a.pool.type, a.pool.dim));
+}
+
+uint32_t tile_shift(const PagedAttentionArgs &a)
+{
+    const uint64_t seen = most_seen(a), positions = (uint64_t)a.batch.max_pages << a.pool.shift;
     uint32_t shift = kTileShift;
-    while ((uint64_t)b.batch * ((((uint64_t)b.max_pages << pool.shift) >> shift) + 2) > 0x7fffffffull) {
+    while ((uint64_t)a.batch.batch * ((positions >> shift) + 2) > 0x7fffffffull || (whole(a) && 1u << shift < seen)) {
         ++shift;
     }
     return shift;
@@ -535,15 +554,16 @@ template <int ACT, int CT, int DIM>
 struct Decode {
     static hipError_t run(const PagedAttentionArgs &a, hipStream_t st)
     {
-        const uint32_t shares = shares_for(a), shift = tile_shift(a.pool, a.batch);
+        const uint32_t shift = tile_shift(a);
+        const bool cut = most_seen(a) > 1u << shift;  // sequences of one tile never are
+        const uint32_t shares = cut || !whole(a) ? shares_for(a) : a.batch.batch;
         const dim3 grid(shares, columns(a.heads, a.pool.kv_heads));
         const bool once = a.heads / a.pool.kv_heads <= 16;
         const auto kernel = a.pool.shift >= 4 ? (once ? paged_decode_kernel<ACT, CT, DIM, true, true> : paged_decode_kernel<ACT, CT, DIM, true, false>)
                                               : (once ? paged_decode_kernel<ACT, CT, DIM, false, true> : paged_decode_kernel<ACT, CT, DIM, false, false>);
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a, shares, shift);
         const hipError_t e = hipGetLastError();
-        // sequences of one tile are never cut
-        if (e != hipSuccess || a.batch.max_pages << a.pool.shift <= 1u << shift) {
+        if (e != hipSuccess || !cut) {
             return e;
         }
         hipLaunchKernelGGL((paged_join_kernel<ACT, DIM>), dim3(a.heads, a.batch.batch), dim3(256), 0, st, a, shares, shift);

@@ -195,7 +195,11 @@ DECODE = [
     (71, 1, 64, 16, (40, 90), 0),                                              # five tiles of queries, the last of seven
     (1024, 1024, 64, 16, (5, 140), 0),                                         # more columns than workgroups fit the chip
     (16, 16, 128, 16, tuple(i * 37 % 400 for i in range(67)), 0),              # shares that hold several sequences and parts of others
-    (2, 1, 64, 8, tuple(i * 53 % 270 for i in range(300)), 0),
+    (2, 1, 64, 8, tuple(i * 53 % 270 for i in range(300)), 0),                 # sequences left whole,
+    (8, 8, 128, 16, tuple(i * 211 % 1009 for i in range(33)), 0),
+    (12, 12, 64, 32, tuple(i * 977 % 2100 for i in range(24)), 500),           # those that a window makes short, too,
+    (8, 4, 128, 64, tuple(i * 977 % 2100 for i in range(70)), 1024),
+    (8, 4, 128, 64, tuple(i * 977 % 2100 for i in range(20)), 1025),           # and as many that are not
 ]
 
 
