@@ -92,6 +92,7 @@ struct Step {
 
 // PAGE16: pages of 16 keys and more, so that each 16-key half of a step lies in one page and its address is the wave's (32 requests
 // fp16 50.9 us; with an address per lane, as smaller pages need it, 77.3).
+// shares == 0: every sequence is one tile and has a workgroup.
 // ONCE: up to 16 heads share a key head, so that one workgroup reads a key for all of them, past the caches; more take a
 // workgroup per 16, which find it there (head size 128: 32 heads over 8, long bf16, 145 us past them and 166 through them;
 // 64 over 2 66.6 and 55.1, 71 over 1 102 and 90).
@@ -107,17 +108,20 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
 
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 15, g = lane >> 4;
-    auto tiles = [&](uint32_t i) { return tiles_of(a, i, shift); };
-    const Places all = places_of(a.batch.batch, lane, tiles);
-    const uint32_t per = tiles_per_share(all.sum, shares);
     const uint32_t share = blockIdx.x, group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
     const uint32_t kvh = blockIdx.y / qtiles, q0 = blockIdx.y % qtiles * 16;
     const uint32_t nq = group - q0 < 16 ? group - q0 : 16;
-    if ((uint64_t)share * per >= all.sum) {
-        return;
+    uint32_t per = 1, tile = share, before = share, b = share;  // tiles of a share; next tile of the row, those in front of its sequence
+    if (shares) {
+        auto tiles = [&](uint32_t i) { return tiles_of(a, i, shift); };
+        const Places all = places_of(a.batch.batch, lane, tiles);
+        per = tiles_per_share(all.sum, shares);
+        if ((uint64_t)share * per >= all.sum) {
+            return;
+        }
+        tile = share * per;
+        b = entry_at(all, a.batch.batch, lane, tile, tiles, &before);
     }
-    uint32_t tile = share * per, before;  // next tile of the row; those in front of its sequence
-    uint32_t b = entry_at(all, a.batch.batch, lane, tile, tiles, &before);
     const uint32_t end = tile + per;
     for (;;) {
         b = __builtin_amdgcn_readfirstlane(b);
@@ -556,8 +560,8 @@ struct Decode {
     {
         const uint32_t shift = tile_shift(a);
         const bool cut = most_seen(a) > 1u << shift;  // sequences of one tile never are
-        const uint32_t shares = cut || !whole(a) ? shares_for(a) : a.batch.batch;
-        const dim3 grid(shares, columns(a.heads, a.pool.kv_heads));
+        const uint32_t shares = cut || !whole(a) ? shares_for(a) : 0;
+        const dim3 grid(shares ? shares : a.batch.batch, columns(a.heads, a.pool.kv_heads));
         const bool once = a.heads / a.pool.kv_heads <= 16;
         const auto kernel = a.pool.shift >= 4 ? (once ? paged_decode_kernel<ACT, CT, DIM, true, true> : paged_decode_kernel<ACT, CT, DIM, true, false>)
                                               : (once ? paged_decode_kernel<ACT, CT, DIM, false, true> : paged_decode_kernel<ACT, CT, DIM, false, false>);

@@ -37,7 +37,7 @@ typedef __attribute__((address_space(3))) void *lptr_t;
 typedef __attribute__((address_space(3))) uint8_t *lds_t;
 
 constexpr uint32_t kRows = 128, kKeys = 64;
-// Workgroups (two a CU) below which a tile's keys are shared out, over about so many. 256 new tokens over 16384 int8 keys, 128 tiles
+// Workgroups (two a CU) below which a tile's keys are shared out, over about so many. 2 x 256 new tokens over 27 k int8 keys, 128 tiles
 // of rows: 153 us with 512, 204 with 256 (half the chip idle), 174 with 1024 (more parts written and read). Eight ragged
 // prompts of up to 1025 tokens have more tiles than that: 99 us with whole tiles, 153 with their keys cut in two.
 constexpr uint32_t kSpread = 512;
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
     };
     // int8: into registers as it is stored, from where it goes to LDS as fp16 while the tile before is worked on (by way of LDS, and
-    // converted there between two barriers, 256 new tokens over 16384 keys took 176 us against 167; between the products, but
+    // converted there between two barriers, 2 x 256 new tokens over 27 k keys took 176 us against 167; between the products, but
     // with a barrier for keys and one for values, 182)
     v4u raw[CT == PT_I8 ? kLoads : 1][2];
     float scale = 0.0f;  // of key lane (wave 0: key, the others: value)
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     };
     if (CT == PT_I8) {
         // (One body, the buffers told apart by a bit of the addresses. Two, as below, take more registers than there are: 177 us
-        // against 157 for 256 new tokens over 16384 keys.)
+        // against 157 for 2 x 256 new tokens over 27 k keys.)
         auto other = [&] {
             at_put_k ^= 2 * kTileBytes;
             at_put_v ^= 2 * kTileBytes;
