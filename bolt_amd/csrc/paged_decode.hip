@@ -424,17 +424,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionArgs a, u
     __shared__ __attribute__((aligned(16))) float sO[kWays][DIM];
     __shared__ float sL[kWays], sM[kWays];
     const uint32_t lane = threadIdx.x & 63, h = blockIdx.x, b = blockIdx.y;
-    auto tiles = [&](uint32_t i) { return tiles_of(a, i, shift); };
-    const Places all = places_of(a.batch.batch, lane, tiles);
-    const uint32_t per = tiles_per_share(all.sum, shares);
-    uint32_t before = 0, mine = 0;  // tiles in front of sequence b, its own
-    if (b < 64) {
-        mine = __builtin_amdgcn_readlane(all.first, b);
-        before = __builtin_amdgcn_readlane(all.upto, b) - mine;
-    } else {
-        mine = tiles(b);
-        before = places_of(b, lane, tiles).sum;
+    uint32_t sum_all = 0, before = 0, mine = 0;  // tiles of all sequences, in front of sequence b, its own: every lane's part first
+    for (uint32_t i = lane; i < a.batch.batch; i += 64) {
+        const uint32_t n = tiles_of(a, i, shift);
+        sum_all += n;
+        before += i < b ? n : 0;
+        mine = i == b ? n : mine;
     }
+    sum_all = __builtin_amdgcn_readlane(wave_scan_u32(sum_all), 63);
+    before = __builtin_amdgcn_readlane(wave_scan_u32(before), 63);
+    mine = __builtin_amdgcn_readlane(mine, b % 64);
+    const uint32_t per = tiles_per_share(sum_all, shares);
     const uint32_t first = before / per, count = (before + mine - 1) / per - first + 1;
     if (count == 1) {
         return;
