@@ -43,7 +43,7 @@ constexpr float kSlack = 2.0f, kLift = 13.0f;  // see above: 2^(kSlack + kLift) 
 
 __device__ __forceinline__ PagedSpan span_of(const PagedAttentionArgs &a, uint32_t b)
 {
-    return paged_span((int64_t)a.batch.lens[b] - 1, a.window, a.batch.max_pages << a.pool.shift);
+    return paged_span_newest(a.batch.lens[b], a.window, a.batch.max_pages << a.pool.shift);
 }
 
 // Tiles of a sequence, counted from its first key rounded down to a step of 32; one where there is nothing to see (somebody

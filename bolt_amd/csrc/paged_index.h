@@ -73,6 +73,17 @@ BG_HD inline PagedSpan paged_span(int64_t pos, uint32_t window, uint32_t capacit
     return r;
 }
 
+// The same for the newest token of a sequence of `len` keys, paged_span(len - 1, ..): 32 bits hold all of it
+BG_HD inline PagedSpan paged_span_newest(int32_t len, uint32_t window, uint32_t capacity)
+{
+    const uint32_t keys = len > 0 ? (uint32_t)len : 0;
+    PagedSpan r;
+    r.hi = keys < capacity ? keys : capacity;
+    r.lo = window && keys > window ? keys - window : 0;
+    r.lo = r.lo < r.hi ? r.lo : r.hi;
+    return r;
+}
+
 // Slot of a key in the pool, in units of head rows: ((page * kv_heads + head) * page_size + place), or -1 where the page
 // number is none of the pool's. key < max_pages << shift.
 BG_HD inline int64_t paged_slot(const int32_t *table_row, uint32_t key, uint32_t shift, uint32_t pages, uint32_t kv_heads, uint32_t head)

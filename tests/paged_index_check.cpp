@@ -52,6 +52,16 @@ int main()
             }
         }
     }
+    // the newest token's
+    const int32_t lengths[] = {low, -1, 0, 1, 2, 15, 16, 17, 100, high};
+    for (int32_t len : lengths) {
+        for (uint32_t w : windows) {
+            for (uint32_t capacity : {1u, 16u, 0x7fffffffu}) {
+                const PagedSpan r = paged_span_newest(len, w, capacity), q = paged_span((int64_t)len - 1, w, capacity);
+                WANT(r.lo == q.lo && r.hi == q.hi);
+            }
+        }
+    }
     // ragged rows: owners by search, with empty sequences, gaps in front and lists that descend or overrun
     const std::vector<std::vector<int32_t>> lists = {{0, 3, 3, 5}, {2, 2, 4, 9}, {5, 1, 9, 0}, {low, low, high, high}, {0, 0, 0, 0}};
     const std::vector<int32_t> three = {10, 20, high};
