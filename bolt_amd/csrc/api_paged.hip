@@ -185,6 +185,8 @@ EE attention(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataTyp
     a.ostride = outStride;
     a.heads = heads;
     a.window = window;
+    a.kv_heads = paged_divisor(a.pool.kv_heads);
+    a.group = paged_divisor(heads / a.pool.kv_heads);
     a.scale2 = scale * 1.44269504088896340736f;  // exp(x) = exp2(x log2(e))
     a.ws = workspace;
     HIP_TRY(decode ? launch_paged_decode(a, ctx().stream) : launch_paged_prompt(a, ctx().stream));

@@ -38,6 +38,7 @@ struct PagedAttentionArgs {
     void *out = nullptr;
     uint32_t qstride = 0, ostride = 0;      // elements between rows
     uint32_t heads = 0, window = 0;
+    PagedDivisor kv_heads, group;           // group: heads that share a key head
     float scale2 = 0;                       // score scale * log2(e)
     void *ws = nullptr;
 };

@@ -108,8 +108,7 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
 
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 15, g = lane >> 4;
-    const uint32_t share = blockIdx.x, group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
-    const uint32_t kvh = blockIdx.y / qtiles, q0 = blockIdx.y % qtiles * 16;
+    const uint32_t share = blockIdx.x, group = a.group.d, kvh = blockIdx.z, q0 = blockIdx.y * 16, column = kvh * ((group + 15) / 16) + blockIdx.y;
     const uint32_t nq = group - q0 < 16 ? group - q0 : 16;
     uint32_t per = 1, tile = share, before = share, b = share;  // tiles of a share; next tile of the row, those in front of its sequence
     if (shares) {
@@ -384,7 +383,7 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
             }
         }
         __syncthreads();
-        float *part = part_at(a, shares, blockIdx.y, share, tile != share * per, DIM);
+        float *part = part_at(a, shares, column, share, tile != share * per, DIM);
         for (uint32_t at = me; at < nq * (DIM / 4); at += 256) {
             const uint32_t r = at / (DIM / 4), d = at % (DIM / 4) * 4;
             const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
@@ -439,8 +438,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionArgs a, u
     if (count == 1) {
         return;
     }
-    const uint32_t group = a.heads / a.pool.kv_heads, qtiles = (group + 15) / 16;
-    const uint32_t kvh = h / group, in = h % group, r = in % 16;
+    const uint32_t qtiles = (a.group.d + 15) / 16, kvh = paged_div(h, a.group), in = h - kvh * a.group.d, r = in % 16;
     const float *part = part_at(a, shares, kvh * qtiles + in / 16, first, 0, DIM);
     const uint32_t slot = before % per != 0;  // of the first part; the others are the first of their share
     const uint32_t way = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
@@ -561,7 +559,7 @@ struct Decode {
         const uint32_t shift = tile_shift(a);
         const bool cut = most_seen(a) > 1u << shift;  // sequences of one tile never are
         const uint32_t shares = cut || !whole(a) ? shares_for(a) : 0;
-        const dim3 grid(shares ? shares : a.batch.batch, columns(a.heads, a.pool.kv_heads));
+        const dim3 grid(shares ? shares : a.batch.batch, (a.group.d + 15) / 16, a.pool.kv_heads);
         const bool once = a.heads / a.pool.kv_heads <= 16;
         const auto kernel = a.pool.shift >= 4 ? (once ? paged_decode_kernel<ACT, CT, DIM, true, true> : paged_decode_kernel<ACT, CT, DIM, true, false>)
                                               : (once ? paged_decode_kernel<ACT, CT, DIM, false, true> : paged_decode_kernel<ACT, CT, DIM, false, false>);

@@ -9,6 +9,29 @@
 
 namespace bg {
 
+// A divisor known to the host: quotients of numbers below 2^31 by one product. With s = ceil(log2 d) and
+// m = floor(2^(31+s) / d) + 1 = (2^(31+s) + e) / d, 0 < e <= d <= 2^s, n m / 2^(31+s) is n / d plus less than 1 / d.
+struct PagedDivisor {
+    uint32_t d = 1, m = 0x80000001u, shift = 31;
+};
+
+inline PagedDivisor paged_divisor(uint32_t d)
+{
+    PagedDivisor r;
+    r.d = d;
+    r.shift = 31;
+    while (1u << (r.shift - 31) < d) {
+        ++r.shift;
+    }
+    r.m = (uint32_t)(((uint64_t)1 << r.shift) / d + 1);
+    return r;
+}
+
+BG_HD inline uint32_t paged_div(uint32_t n, const PagedDivisor &d)
+{
+    return (uint32_t)((uint64_t)n * d.m >> d.shift);
+}
+
 struct PagedBatch {
     const int32_t *table = nullptr;    // [batch][max_pages] page numbers
     const int32_t *lens = nullptr;     // [batch] keys of each sequence, its new tokens included

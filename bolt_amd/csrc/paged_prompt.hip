@@ -46,20 +46,20 @@ constexpr float kLow = -1.7e38f;
 constexpr float kSlack = 2.0f, kLift = 13.0f;
 
 // rows (token, head) of a sequence in tiles of kRows; no more tokens than the buffers have rows, so that it all fits 31 bits
-__device__ __forceinline__ uint32_t rows_of(const PagedAttentionArgs &a, const PagedSeq &s, uint32_t group)
+__device__ __forceinline__ uint32_t rows_of(const PagedAttentionArgs &a, const PagedSeq &s)
 {
-    return (s.count < (int64_t)a.batch.rows ? (uint32_t)s.count : a.batch.rows) * group;
+    return (s.count < (int64_t)a.batch.rows ? (uint32_t)s.count : a.batch.rows) * a.group.d;
 }
 
 // Row tile number x of the launch: its sequence and its number there. What takes longest starts first: the longest sequence
 // (of up to 64, of more the last one), and of a sequence the last tile, which sees the most keys.
-__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t group, uint32_t x, uint32_t lane, uint32_t *b_out, uint32_t *tile, PagedSeq *seq)
+__device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t x, uint32_t lane, uint32_t *b_out, uint32_t *tile, PagedSeq *seq)
 {
     const uint32_t n = a.batch.batch;
     if (n <= 64) {  // everything that is needed is asked for at once
         const uint32_t mine = lane < n ? lane : n - 1;
         const int32_t first = a.batch.offsets[mine], next = a.batch.offsets[mine + 1], keys = lane < n ? a.batch.lens[mine] : -0x7fffffff - 1;
-        const uint32_t tiles = lane < n ? (rows_of(a, paged_seq_from(first, next, keys), group) + kRows - 1) / kRows : 0;
+        const uint32_t tiles = lane < n ? (rows_of(a, paged_seq_from(first, next, keys)) + kRows - 1) / kRows : 0;
         uint32_t before = 0;  // tiles of longer sequences, and of those in front that are as long
         for (uint32_t i = 0; i < n; ++i) {
             const int32_t other = __builtin_amdgcn_readlane(keys, i);
@@ -72,7 +72,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttentionArgs &a, uint32_t 
         *seq = paged_seq_from(__builtin_amdgcn_readlane(first, at), __builtin_amdgcn_readlane(next, at), __builtin_amdgcn_readlane(keys, at));
         return here != 0;
     }
-    auto count = [&](uint32_t i) { return (rows_of(a, paged_seq(a.batch, i), group) + kRows - 1) / kRows; };
+    auto count = [&](uint32_t i) { return (rows_of(a, paged_seq(a.batch, i)) + kRows - 1) / kRows; };
     const Places all = places_of(n, lane, count);
     if (x >= all.sum) {
         return false;
@@ -91,12 +91,12 @@ struct Reach {
     uint32_t lo, hi, tiles;
 };
 
-__device__ __forceinline__ Reach reach_of(const PagedAttentionArgs &a, const PagedSeq &s, uint32_t rows, uint32_t tile, uint32_t group)
+__device__ __forceinline__ Reach reach_of(const PagedAttentionArgs &a, const PagedSeq &s, uint32_t rows, uint32_t tile)
 {
     Reach r;
     const uint32_t r0 = tile * kRows, r1 = min(r0 + kRows, rows);
-    r.first = s.pos + r0 / group;
-    r.last = s.pos + (r1 - 1) / group;
+    r.first = s.pos + paged_div(r0, a.group);
+    r.last = s.pos + paged_div(r1 - 1, a.group);
     const uint32_t capacity = a.batch.max_pages << a.pool.shift;
     r.hi = paged_span(r.last, a.window, capacity).hi;
     r.lo = paged_span(r.first > 0 ? r.first : 0, a.window, capacity).lo & ~(kKeys - 1);
@@ -104,9 +104,9 @@ __device__ __forceinline__ Reach reach_of(const PagedAttentionArgs &a, const Pag
     return r;
 }
 
-__device__ __forceinline__ uint32_t tiles_per_share(uint32_t tiles, uint32_t shares)
+__device__ __forceinline__ uint32_t tiles_per_share(uint32_t tiles, const PagedDivisor &shares)
 {
-    const uint32_t n = (tiles + shares - 1) / shares;
+    const uint32_t n = paged_div(tiles + shares.d - 1, shares);
     return n < kLeast ? kLeast : n;
 }
 
@@ -223,7 +223,7 @@ constexpr uint32_t rows_at()
 }
 
 template <int ACT, int CT, int DIM, bool PAGED>
-__global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs a, uint32_t shares)
+__global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs a, PagedDivisor shares)
 {
     typedef Product<CT> Op;
     typedef typename Op::V V;
@@ -242,15 +242,15 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t c = lane & 31, h = lane >> 5;
-    const uint32_t kvh = blockIdx.x % a.pool.kv_heads, share = blockIdx.x / a.pool.kv_heads % shares, x = blockIdx.x / a.pool.kv_heads / shares;
-    const uint32_t group = a.heads / a.pool.kv_heads;
+    const uint32_t column = paged_div(blockIdx.x, a.kv_heads), kvh = blockIdx.x - column * a.kv_heads.d;
+    const uint32_t x = paged_div(column, shares), share = column - x * shares.d, group = a.group.d;
     uint32_t b, tile_index;
     PagedSeq seq;
-    if (!find_tile(a, group, x, lane, &b, &tile_index, &seq)) {
+    if (!find_tile(a, x, lane, &b, &tile_index, &seq)) {
         return;
     }
-    const uint32_t rows = rows_of(a, seq, group);
-    const Reach all = reach_of(a, seq, rows, tile_index, group);
+    const uint32_t rows = rows_of(a, seq);
+    const Reach all = reach_of(a, seq, rows, tile_index);
     const uint32_t per = tiles_per_share(all.tiles, shares);
     const uint32_t t0 = share * per, t1 = min(t0 + per, all.tiles);
     if (share && t0 >= all.tiles) {
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     const int32_t *table = a.batch.table + (size_t)b * a.batch.max_pages;
 
     // this lane's row
-    const uint32_t r = tile_index * kRows + 32 * wave + c, token = r / group;
+    const uint32_t r = tile_index * kRows + 32 * wave + c, token = paged_div(r, a.group);
     const int64_t row = seq.first + token, pos = seq.pos + token;
     const bool mine = r < rows && row >= 0 && row < (int64_t)a.batch.rows;
     const uint32_t head = kvh * group + (r - token * group);
@@ -773,7 +773,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
         return;
     }
-    float *const part = part_at(a, x, kvh, share, shares, DIM);
+    float *const part = part_at(a, x, kvh, share, shares.d, DIM);
     const uint32_t pr = 32 * wave + c;
 #pragma unroll
     for (int i = 0; i < kOut; ++i) {
@@ -791,17 +791,17 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
 
 // Joins the shares of a tile's keys: a workgroup per eight rows of a tile, DIM / 4 lanes to a row
 template <int ACT, int DIM>
-__global__ __launch_bounds__(8 * DIM / 4) void paged_prompt_join_kernel(PagedAttentionArgs a, uint32_t shares)
+__global__ __launch_bounds__(8 * DIM / 4) void paged_prompt_join_kernel(PagedAttentionArgs a, PagedDivisor shares)
 {
-    const uint32_t lane = threadIdx.x & 63, kvh = blockIdx.x % a.pool.kv_heads, x = blockIdx.x / a.pool.kv_heads;
-    const uint32_t group = a.heads / a.pool.kv_heads;
+    const uint32_t lane = threadIdx.x & 63, x = paged_div(blockIdx.x, a.kv_heads), kvh = blockIdx.x - x * a.kv_heads.d;
+    const uint32_t group = a.group.d;
     uint32_t b, tile_index;
     PagedSeq seq;
-    if (!find_tile(a, group, x, lane, &b, &tile_index, &seq)) {
+    if (!find_tile(a, x, lane, &b, &tile_index, &seq)) {
         return;
     }
-    const uint32_t rows = rows_of(a, seq, group);
-    const Reach all = reach_of(a, seq, rows, tile_index, group);
+    const uint32_t rows = rows_of(a, seq);
+    const Reach all = reach_of(a, seq, rows, tile_index);
     const uint32_t per = tiles_per_share(all.tiles, shares);
     if (per >= all.tiles) {
         return;
@@ -809,14 +809,15 @@ __global__ __launch_bounds__(8 * DIM / 4) void paged_prompt_join_kernel(PagedAtt
     const uint32_t count = (all.tiles + per - 1) / per;
     const uint32_t pr = blockIdx.y * 8 + threadIdx.x / (DIM / 4), d = threadIdx.x % (DIM / 4) * 4;
     const uint32_t r = tile_index * kRows + pr;
-    const int64_t row = seq.first + r / group;
+    const uint32_t token = paged_div(r, a.group);
+    const int64_t row = seq.first + token;
     if (r >= rows || row < 0 || row >= (int64_t)a.batch.rows) {
         return;
     }
     float top = kLow, sum = 0.0f;
     v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t i = 0; i < count; ++i) {
-        const float *const p = part_at(a, x, kvh, i, shares, DIM);
+        const float *const p = part_at(a, x, kvh, i, shares.d, DIM);
         const float m = p[kRows * DIM + pr], up = fmaxf(top, m);
         const float f = __builtin_amdgcn_exp2f(top - up), e = __builtin_amdgcn_exp2f(m - up);
         sum = sum * f + p[kRows * DIM + kRows + pr] * e;
@@ -824,7 +825,7 @@ __global__ __launch_bounds__(8 * DIM / 4) void paged_prompt_join_kernel(PagedAtt
         top = up;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    store_out4<ACT>(a.out, (size_t)row * a.ostride + (size_t)(kvh * group + r % group) * DIM + d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    store_out4<ACT>(a.out, (size_t)row * a.ostride + (size_t)(kvh * group + r - token * group) * DIM + d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
 }
 
 // row tiles that a launch may have, and how many workgroups share a tile's keys
@@ -878,12 +879,12 @@ struct Prompt {
             return e;
         }
         const uint64_t blocks = tiles * a.pool.kv_heads;
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, shares);
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)(blocks * shares)), dim3(256), lds, st, a, paged_divisor(shares));
         e = hipGetLastError();
         if (e != hipSuccess || shares == 1) {
             return e;
         }
-        hipLaunchKernelGGL((paged_prompt_join_kernel<ACT, DIM>), dim3((uint32_t)blocks, kRows / 8), dim3(8 * DIM / 4), 0, st, a, shares);
+        hipLaunchKernelGGL((paged_prompt_join_kernel<ACT, DIM>), dim3((uint32_t)blocks, kRows / 8), dim3(8 * DIM / 4), 0, st, a, paged_divisor(shares));
         return hipGetLastError();
     }
 };

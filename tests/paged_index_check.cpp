@@ -52,6 +52,13 @@ int main()
             }
         }
     }
+    // quotients by a product
+    for (uint32_t d = 1; d <= 16384; d = d < 300 ? d + 1 : d * 3 / 2 + 1) {
+        const PagedDivisor by = paged_divisor(d);
+        for (uint32_t n : {0u, 1u, d - 1, d, d + 1, 2 * d - 1, 2 * d, 1000 * d - 1, 1000 * d, 0x7fffffffu / d * d - 1, 0x7fffffffu / d * d, 0x7ffffffeu, 0x7fffffffu}) {
+            WANT(paged_div(n, by) == n / d);
+        }
+    }
     // the newest token's
     const int32_t lengths[] = {low, -1, 0, 1, 2, 15, 16, 17, 100, high};
     for (int32_t len : lengths) {
