@@ -262,6 +262,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
     // this lane's row
     const uint32_t r = tile_index * kRows + 32 * wave + c, token = paged_div(r, a.group);
     const int64_t row = seq.first + token, pos = seq.pos + token;
+    const bool idle = tile_index * kRows + 32 * wave >= rows;  // (the wave's)
     const bool mine = r < rows && row >= 0 && row < (int64_t)a.batch.rows;
     const uint32_t head = kvh * group + (r - token * group);
     const PagedSpan span = paged_span(mine ? pos : -1, a.window, all.hi);
@@ -516,6 +517,26 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 __syncthreads();
             }
         }
+        // int8: the next tile's steps into LDS, the one's behind it on their way
+        auto further = [&] {
+            put_steps(steps_ahead);
+            stored = __ballot(pages >= 0);
+            pages = page_of(k0 + 2 * kKeys, next);
+            next = look_up(k0 + 3 * kKeys);
+            fetch_raw(k0 + 2 * kKeys, pages);
+        };
+        // a wave without rows only brings its part of the tiles (32 sequences of up to 4 new tokens over up to 2000 keys 53 us, with
+        // all four at work on nothing 59)
+        if (idle) {
+            if (CT == PT_I8) {
+#pragma unroll
+                for (int p = 0; p < 4 * kLoads; ++p) {
+                    convert(p, ahead);
+                }
+                further();
+            }
+            return;
+        }
         // Scores. The order is written out (the compiler would wait for every read right behind it): six or eight reads ahead of the
         // products that use them.
         v16f s[2];
@@ -561,11 +582,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
         const unsigned long long stored_here = stored;
         if (CT == PT_I8) {
-            put_steps(steps_ahead);
-            stored = __ballot(pages >= 0);
-            pages = page_of(k0 + 2 * kKeys, next);
-            next = look_up(k0 + 3 * kKeys);
-            fetch_raw(k0 + 2 * kKeys, pages);
+            further();
         }
         V vv[2][kOut], ph[2], pl[2];
         Words<4> pw[2];
@@ -771,6 +788,9 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 store_out4<ACT>(a.out, at + 32 * i + 2 * j, o[i][j] * inv, o[i][j + 1] * inv, o[i][j + 2] * inv, o[i][j + 3] * inv);
             }
         }
+        return;
+    }
+    if (idle) {
         return;
     }
     float *const part = part_at(a, x, kvh, share, shares.d, DIM);
