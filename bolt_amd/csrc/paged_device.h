@@ -167,8 +167,9 @@ __device__ __forceinline__ float shift_into_f16(float top, int *e)
     return ldexpf(1.0f, 15 - x);
 }
 
-// the smallest power of two that is not below x, from kFirstUnit up to 2^120; 2^e, whose reciprocal is exact
-constexpr float kFirstUnit = 7.52316385e-37f;  // 2^-120
+// the smallest power of two that is not below x, from kFirstUnit up to 2^120; 2^e, whose reciprocal is exact, and 2^21 times which
+// fp32 holds
+constexpr float kFirstUnit = 7.88860905e-31f;  // 2^-100
 __device__ __forceinline__ float power_above(float x)
 {
     const uint32_t u = (__float_as_uint(x) + 0x7fffffu) & 0x7f800000u;

@@ -141,10 +141,13 @@ __device__ __forceinline__ float max_of(float a, float b, float c)
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
-// int8: the steps of a tile's keys (times the score scale) and values (over `unit`), values whose step is not finite, and the
-// power of two above the largest step
+// int8: the steps of a tile's keys (times the score scale) and values, values whose step is not finite, and the power of two above
+// the largest step. Values' steps three times: over `unit`, for rows that see the whole tile; as they are and times 2^-80, for
+// rows that do not, whose own largest step may be any number of powers of two below `unit`.
+enum { kStepK, kStepV, kStepOwn, kStepOwnLow };
+constexpr float kLowStep = 8.27180613e-25f;  // 2^-80
 struct StepsOfTile {
-    float step[2][kKeys];
+    float step[4][kKeys];
     unsigned long long bad;
     float unit, unused;
 };
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
         *(__attribute__((address_space(3))) v4u *)(to + kv * kTileBytes + n * 4 * kRowsAt * DIM * 2 + ((kv ? at_put_v : at_put_k) ^ (16 * half))) = f;
     };
-    // The steps. Those of values are multiples of a power of two that none exceeds; one that is not finite is taken out.
+    // The steps. One of a value that is not finite is taken out.
     auto put_steps = [&](StepsOfTile *to) {
         if (wave < 2) {
             float step = __builtin_amdgcn_rcpf(scale);
@@ -372,11 +375,13 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                     to->bad = not_fine;
                     to->unit = unit_of_tile;
                 }
+                to->step[kStepOwn][lane] = step;
+                to->step[kStepOwnLow][lane] = step * kLowStep;
                 step *= __builtin_amdgcn_rcpf(unit_of_tile);
             } else {
                 step *= score_scale;
             }
-            to->step[wave][lane] = step;
+            to->step[wave ? kStepV : kStepK][lane] = step;
         }
     };
 
@@ -471,7 +476,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         // does every row of the workgroup see every key of the tile?
         const bool whole = stored == ~0ull && k0 + kKeys <= all_hi && k0 >= all_lo;
         // A value that is infinite or NaN must not reach the rows that do not see its key (0 * inf): it is taken out of the tile, and
-        // the rows that do see it become NaN in the end. An int8 cache has it in the slot's step, which put8 has taken out.
+        // the rows that do see it become NaN in the end. An int8 cache has it in the slot's step, which put_steps has taken out.
         if (CT != PT_I8 && !whole) {
             constexpr uint32_t kExp = CT == PT_BF16 ? 0x7f80u : 0x7c00u;
             lds_t const base = now + kTileBytes;
@@ -602,7 +607,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         in_order();
         if (CT == PT_I8) {
             v4f ks[3];
-            auto read = [&](int x) { ks[x % 3] = *(const v4f *)(steps->step[0] + 32 * (x / 4) + 8 * (x % 4) + 4 * h); };
+            auto read = [&](int x) { ks[x % 3] = *(const v4f *)(steps->step[kStepK] + 32 * (x / 4) + 8 * (x % 4) + 4 * h); };
             read(0);
             read(1);
 #pragma unroll
@@ -619,6 +624,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             }
         }
         unsigned long long seen = ~0ull;
+        float tile_unit = CT == PT_I8 ? steps->unit : 1.0f;  // no step of a value that the row sees exceeds it
         if (!whole) {
             const uint32_t from = span.lo > k0 ? span.lo - k0 : 0, upto = span.hi > k0 ? span.hi - k0 : 0;  // keys of the tile this row sees
             seen = from >= kKeys || upto <= from ? 0 : (upto >= kKeys ? ~0ull : (1ull << upto) - 1) & (~0ull << from);
@@ -632,6 +638,22 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                     s[i][j] = sees ? s[i][j] : -INFINITY;
                 }
             }
+            if (CT == PT_I8) {
+                float wide = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const uint32_t some = (uint32_t)(seen >> (32 * (x / 4))) >> (8 * (x % 4) + 4 * h);
+                    const v4f step = *(const v4f *)(steps->step[kStepOwn] + 32 * (x / 4) + 8 * (x % 4) + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        wide = fmaxf(wide, some >> e & 1 ? fabsf(step[e]) : 0.0f);
+                    }
+                }
+                tile_unit = power_above(fmaxf(wide, __shfl_xor(wide, 32, 64)));
+            }
+        }
+        if (CT == PT_I8) {
+            poisoned |= (steps->bad & seen) != 0;
         }
         float top = -INFINITY;
 #pragma unroll
@@ -639,7 +661,6 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             top = max_of(top, s[0][j], s[1][j]);
         }
         top *= xscale;
-        const float tile_unit = CT == PT_I8 ? steps->unit : 1.0f;
         if (__any(top > m + kSlack || (CT == PT_I8 && tile_unit > unit))) {
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const float up = fmaxf(top, m);
@@ -659,16 +680,26 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             }
         }
         // Weights times values, 16 keys a step: behind every product stand the next step's reads and a share of its weights
-        // (int8: the tile's steps are multiples of its own power of two; what that is of the output's goes into the exponent, and
-        // out of the sum again. It ends at 2^-64, where a tile's values are far below what the output can hold of others.)
-        const float part = CT == PT_I8 ? fmaxf(tile_unit * __builtin_amdgcn_rcpf(unit), 5.42101086e-20f) : 1.0f;
+        // (int8: the steps that weights are multiplied by are over `unit` in the end. What is left of that beside the way they are stored
+        // goes into the exponent, and out of the sum again: the tile's power of two over `unit`, down to 2^-64, where a tile's values
+        // are far below what the output can hold of others; or, of steps as they are, 1 / unit, which fp32 holds a weight times
+        // where unit < 1, and of those times 2^-80 2^80 / unit. What a row does not see has a weight of zero.)
+        const float *steps_v = nullptr;
+        float part = 1.0f;
+        if (CT == PT_I8) {
+            part = __builtin_amdgcn_rcpf(unit);
+            const bool low = unit >= 1.0f;
+            const float own = low ? part * (1.0f / kLowStep) : part;
+            part = whole ? fmaxf(tile_unit * part, 5.42101086e-20f) : own;
+            steps_v = steps->step[kStepV] + (whole ? 0 : (low ? kStepOwnLow - kStepV : kStepOwn - kStepV) * kKeys);
+        }
         const float shift = (CT == PT_I8 ? kLift + __builtin_amdgcn_logf(part) : kLift) - m;
         float sum = 0.0f;
         float p[8];
         v4f vs[2][2];  // int8: steps of this group's and the next one's values
         auto steps_of = [&](int u) {
-            vs[u & 1][0] = *(const v4f *)(steps->step[1] + 16 * u + 4 * h);
-            vs[u & 1][1] = *(const v4f *)(steps->step[1] + 16 * u + 8 + 4 * h);
+            vs[u & 1][0] = *(const v4f *)(steps_v + 16 * u + 4 * h);
+            vs[u & 1][1] = *(const v4f *)(steps_v + 16 * u + 8 + 4 * h);
         };
         if (CT == PT_I8) {
             steps_of(0);
@@ -733,7 +764,6 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         }
         if (CT == PT_I8) {
             l += sum * __builtin_amdgcn_rcpf(part);
-            poisoned |= (steps->bad & seen) != 0;
         }
     };
     if (CT == PT_I8) {
@@ -779,8 +809,11 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         if (!mine) {
             return;
         }
+        uint32_t again = r;
+        asm volatile("" : "+v"(again));  // the row's place is worked out anew: kept over the loop it would cost registers
+        const uint32_t token_again = paged_div(again, a.group);
         const float inv = l == 0.0f ? 0.0f : unit / l;
-        const size_t at = (size_t)row * a.ostride + (size_t)head * DIM + 4 * h;
+        const size_t at = (size_t)(seq.first + token_again) * a.ostride + (size_t)(kvh * group + (again - token_again * group)) * DIM + 4 * h;
 #pragma unroll
         for (int i = 0; i < kOut; ++i) {
 #pragma unroll

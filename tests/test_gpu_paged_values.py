@@ -1,0 +1,65 @@
+"""Attention over a paged cache where the numbers themselves are the difficulty: slots that a row does not see but that are far
+larger than those it sees, values and steps at the upper end of their types, scores whose fp32 steps are larger than one.
+Against tests/checkers_paged.py (64 bits, within the bound that the roundings give)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+import torch  # noqa: E402
+
+from bolt_amd import capi, host_paged as hp  # noqa: E402
+from checkers_paged import COMBOS, TYPES, Case, assert_attention  # noqa: E402
+from test_gpu_paged import attend, bits, ready  # noqa: E402,F401
+
+PROMPT = pytest.mark.parametrize("prompt", [False, True])
+
+
+# ---- slots that a row does not see ------------------------------------------------------------------
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("page", [16, 2])
+@pytest.mark.parametrize("step", [2.0 ** 8, 1e12, 1e30, 2.0 ** 125])
+def test_large_finite_steps_of_later_tokens_change_nothing(act, page, step):
+    """the value step of one token in the middle of a prompt, and of every later one, far above the others': the rows before it
+    have the bytes of the cache without it, and the rows from it on what the formula gives"""
+    new, past, spot = 90, 3, 41
+    c = Case(act, "i8", 4, 2, 64, page, (new + past,), (new,), seed=41)
+    clean = attend(c, True)
+    assert_attention(clean, c)
+    for behind in (1, new - spot):
+        keep = c.vs.clone()
+        for p in range(spot + past, spot + past + behind):
+            c.vs[int(c.table[0, p // page]), :, p % page] = 1.0 / step
+        out = attend(c, True)
+        assert torch.equal(bits(out[:spot]), bits(clean[:spot])), (behind, step)
+        if 127 * step < torch.finfo(TYPES[act]).max:                           # (else the rows behind are infinite, or of no sign that the bound leaves)
+            assert_attention(out, c)
+        c.vs = keep
+
+
+@PROMPT
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("step", [2.0 ** 8, 1e12, 1e30, 2.0 ** 125])
+def test_large_finite_steps_in_front_of_a_window_change_nothing(act, prompt, step):
+    """slots that lie in the first tile that a window reaches into, in front of the window"""
+    new, window, total = (9 if prompt else 1), 30, 160
+    c = Case(act, "i8", 4, 2, 64, 16, (total,), (new,), seed=42, window=window)
+    clean = attend(c, prompt)
+    assert_attention(clean, c)
+    first = total - new + 1 - window                                           # the first key that any row sees
+    for p in range(first // 64 * 64, first):
+        c.vs[int(c.table[0, p // 16]), :, p % 16] = 1.0 / step
+    assert first % 32
+    assert torch.equal(bits(attend(c, prompt)), bits(clean))
+
+
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+def test_steps_of_all_sizes_along_a_prompt(act):
+    """steps that grow from token to token by a factor of four, and that fall: every row sees other ones, and the largest it sees
+    is its newest or its oldest"""
+    largest = 8.0 if act == "f16" else 56.0                                    # 127 times which is a number of the type
+    for grow in (2.0, -2.0):
+        c = Case(act, "i8", 4, 2, 64, 16, (57,), (57,), seed=43)
+        for p in range(57):
+            c.vs[int(c.table[0, p // 16]), :, p % 16] = 2.0 ** (grow * (28 - p) + 56 - largest)
+        assert_attention(attend(c, True), c)
