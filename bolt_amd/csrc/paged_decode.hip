@@ -373,13 +373,13 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
         l += __shfl_xor(l, 32, 64);
         if (eg == 0) {
             sM[wave][ec] = m;
-            sL[wave][ec] = l;
+            sL[wave][ec] = l * kPartScale<CT>;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int t = 0; t < kVec; t += 4) {
-                *(v4f *)(&sO[wave][ec * kRow + kVec * (4 * eg + i) + t]) = (v4f){o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]} * unit;
+                *(v4f *)(&sO[wave][ec * kRow + kVec * (4 * eg + i) + t]) = (v4f){o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]} * kPartScale<CT> * unit;
             }
         }
         __syncthreads();

@@ -167,14 +167,19 @@ __device__ __forceinline__ float shift_into_f16(float top, int *e)
     return ldexpf(1.0f, 15 - x);
 }
 
-// the smallest power of two that is not below x, from kFirstUnit up to 2^120; 2^e, whose reciprocal is exact, and 2^21 times which
-// fp32 holds
+// the smallest power of two that is not below x, from kFirstUnit up to 2^126, the largest whose reciprocal is a normal number (and
+// the largest step that a normal scale makes)
 constexpr float kFirstUnit = 7.88860905e-31f;  // 2^-100
 __device__ __forceinline__ float power_above(float x)
 {
     const uint32_t u = (__float_as_uint(x) + 0x7fffffu) & 0x7f800000u;
-    return fminf(fmaxf(__uint_as_float(u), kFirstUnit), 1.32922800e36f);
+    return fminf(fmaxf(__uint_as_float(u), kFirstUnit), 8.50705917e37f);
 }
+
+// what a part's outputs and sum are multiplied by before the former become multiples of 1 instead of `unit`: weights lie up to 2^15
+// above the formula's, and fp32 has to hold their products with the largest values
+template <int CT>
+constexpr float kPartScale = CT == PT_I8 ? 0x1p-15f : 1.0f;
 
 // four slots' factors from 4-byte aligned memory
 __device__ __forceinline__ v4f load_scales(const float *p)

@@ -827,18 +827,19 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         return;
     }
     float *const part = part_at(a, x, kvh, share, shares.d, DIM);
+    constexpr float down = kPartScale<CT>;
     const uint32_t pr = 32 * wave + c;
 #pragma unroll
     for (int i = 0; i < kOut; ++i) {
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
             *(v4f *)(part + (size_t)pr * DIM + 32 * i + 2 * j + 4 * h) =
-                (v4f){o[i][j] * unit, o[i][j + 1] * unit, o[i][j + 2] * unit, o[i][j + 3] * unit};
+                (v4f){o[i][j] * down * unit, o[i][j + 1] * down * unit, o[i][j + 2] * down * unit, o[i][j + 3] * down * unit};
         }
     }
     if (h == 0) {
         part[kRows * DIM + pr] = m;
-        part[kRows * DIM + kRows + pr] = l;
+        part[kRows * DIM + kRows + pr] = l * down;
     }
 }
 

@@ -63,3 +63,21 @@ def test_steps_of_all_sizes_along_a_prompt(act):
         for p in range(57):
             c.vs[int(c.table[0, p // 16]), :, p % 16] = 2.0 ** (grow * (28 - p) + 56 - largest)
         assert_attention(attend(c, True), c)
+
+
+# ---- values at the upper end of their types -----------------------------------------------------------
+def shares(act, cache, prompt, **kw):
+    """a case whose keys one workgroup has, and one whose keys several share"""
+    for total in (40, 3000):
+        yield Case(act, cache, 4, 2, 64, 16, (total,), (7,) if prompt else (1,), seed=44, **kw)
+
+
+@PROMPT
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("size,stored", [(100, 64), (110, 4), (116, 1), (126, 0)])
+def test_steps_up_to_the_largest(act, prompt, size, stored):
+    """one slot in 16 holds values of a step of 2^size, up to 2^116 (fp32 holds the sum of some 2^10 of them)"""
+    for c in shares(act, "i8", prompt):
+        c.vs[:, :, ::16] = torch.where(c.vs[:, :, ::16].isnan(), c.vs[:, :, ::16], 2.0 ** -size)
+        c.v[:, :, ::16] = c.v[:, :, ::16].sign() * stored
+        assert_attention(attend(c, prompt), c)
