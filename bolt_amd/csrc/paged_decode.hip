@@ -10,8 +10,10 @@
 //                       register with one byte permutation. Which d a result row means is then (DIM / 16) m + t.
 // Neither LDS nor a transposed copy of V is needed. Weights are split into two 16-bit parts (their rounding would
 // otherwise be as large as the output's); fp32 queries are, too, after a power of two brought their row into fp16's range.
-// The running maximum is only raised once a score exceeds it by 2 (base 2): weights are scaled by 2^13 and stay below
-// 2^15, inside fp16; a weight of less than 2^-37 of the row's largest is lost. An int8 cache's steps (1 / scale) are part of
+// The running maximum is only raised once a score exceeds it by 2 (base 2). Over an fp16 or int8 cache weights are scaled by 2^13
+// and stay below 2^15, inside fp16; a weight of less than 2^-37 of the row's largest is lost. Over a bf16 cache, whose values
+// reach as far as fp32's, they are scaled by 2^-2 and stay below 1, so that their products overflow only where the plain formula's
+// fp32 sums do. An int8 cache's steps (1 / scale) are part of
 // the weights, divided by a power of two that no step exceeds, so that they add nothing to that range.
 //
 // The tiles (of 128 keys) of all sequences stand in one row that is cut into equal shares, one to a workgroup, which fill the chip once:
@@ -39,7 +41,9 @@ constexpr uint32_t per_cu()
 }
 
 constexpr float kLow = -1.7e38f;     // running maximum before the first key
-constexpr float kSlack = 2.0f, kLift = 13.0f;  // see above: 2^(kSlack + kLift) fits fp16
+constexpr float kSlack = 2.0f;
+template <int CT>
+constexpr float kLift = CT == PT_BF16 ? -2.0f : 13.0f;  // see above: 2^(kSlack + kLift) fits fp16
 
 __device__ __forceinline__ PagedSpan span_of(const PagedAttentionArgs &a, uint32_t b)
 {
@@ -320,7 +324,7 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[j] = __builtin_amdgcn_exp2f(x[j] - m + kLift);
+                p[j] = __builtin_amdgcn_exp2f(x[j] - m + kLift<CT>);
                 l += p[j];
             }
             if (CT == PT_I8) {

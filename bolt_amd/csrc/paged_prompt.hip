@@ -43,7 +43,9 @@ constexpr uint32_t kRows = 128, kKeys = 64;
 constexpr uint32_t kSpread = 512;
 constexpr uint32_t kLeast = 4;     // fewest key tiles per share
 constexpr float kLow = -1.7e38f;
-constexpr float kSlack = 2.0f, kLift = 13.0f;
+constexpr float kSlack = 2.0f;
+template <int CT>
+constexpr float kLift = CT == PT_BF16 ? -2.0f : 13.0f;  // weights stay below 2^15, inside fp16; in bf16, below 1 (as in paged_decode.hip)
 
 // rows (token, head) of a sequence in tiles of kRows; no more tokens than the buffers have rows, so that it all fits 31 bits
 __device__ __forceinline__ uint32_t rows_of(const PagedAttentionArgs &a, const PagedSeq &s)
@@ -693,7 +695,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             part = whole ? fmaxf(tile_unit * part, 5.42101086e-20f) : own;
             steps_v = steps->step[kStepV] + (whole ? 0 : (low ? kStepOwnLow - kStepV : kStepOwn - kStepV) * kKeys);
         }
-        const float shift = (CT == PT_I8 ? kLift + __builtin_amdgcn_logf(part) : kLift) - m;
+        const float shift = (CT == PT_I8 ? kLift<CT> + __builtin_amdgcn_logf(part) : kLift<CT>) - m;
         float sum = 0.0f;
         float p[8];
         v4f vs[2][2];  // int8: steps of this group's and the next one's values

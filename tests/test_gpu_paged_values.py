@@ -81,3 +81,12 @@ def test_steps_up_to_the_largest(act, prompt, size, stored):
         c.vs[:, :, ::16] = torch.where(c.vs[:, :, ::16].isnan(), c.vs[:, :, ::16], 2.0 ** -size)
         c.v[:, :, ::16] = c.v[:, :, ::16].sign() * stored
         assert_attention(attend(c, prompt), c)
+
+
+@PROMPT
+@pytest.mark.parametrize("size", [1e34, 1e36, 2e37])
+def test_large_values_of_a_bf16_cache(prompt, size):
+    for c in shares("bf16", "bf16", prompt):
+        c.v = (c.v.float().clamp(-1, 1) * size).bfloat16()
+        c.q = (c.q.float() * 4).bfloat16()                                     # few keys have most of the weight
+        assert_attention(attend(c, prompt), c)
