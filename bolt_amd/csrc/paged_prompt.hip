@@ -143,6 +143,8 @@ __device__ __forceinline__ float max_of(float a, float b, float c)
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
+constexpr float kLargeScore = 4194304.0f;  // 2^22: half an fp32 step of it is 2^-2
+
 // int8: the steps of a tile's keys (times the score scale) and values, values whose step is not finite, and the power of two above
 // the largest step. Values' steps three times: over `unit`, for rows that see the whole tile; as they are and times 2^-80, for
 // rows that do not, whose own largest step may be any number of powers of two below `unit`.
@@ -681,6 +683,22 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
                 o[i] = o[i] * corr;
             }
         }
+        // A weight's exponent is s * factor + shift in one instruction. Its product is not rounded as that in the maximum m was, and in
+        // the shift m meets small numbers: above 2^23 either is off by a whole and more, weights leave fp16 and differ from tile to
+        // tile. Of scores that large (a row's own: others keep their bytes) the maximum is taken away first (of
+        // -inf, where a row sees nothing of the tile, too).
+        float factor = xscale, off = m;
+        if (fabsf(top) > kLargeScore) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    s[i][j] = s[i][j] * xscale - m;
+                }
+            }
+            factor = 1.0f;
+            off = 0.0f;
+        }
         // Weights times values, 16 keys a step: behind every product stand the next step's reads and a share of its weights
         // (int8: the steps that weights are multiplied by are over `unit` in the end. What is left of that beside the way they are stored
         // goes into the exponent, and out of the sum again: the tile's power of two over `unit`, down to 2^-64, where a tile's values
@@ -695,7 +713,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             part = whole ? fmaxf(tile_unit * part, 5.42101086e-20f) : own;
             steps_v = steps->step[kStepV] + (whole ? 0 : (low ? kStepOwnLow - kStepV : kStepOwn - kStepV) * kKeys);
         }
-        const float shift = (CT == PT_I8 ? kLift<CT> + __builtin_amdgcn_logf(part) : kLift<CT>) - m;
+        const float shift = (CT == PT_I8 ? kLift<CT> + __builtin_amdgcn_logf(part) : kLift<CT>) - off;
         float sum = 0.0f;
         float p[8];
         v4f vs[2][2];  // int8: steps of this group's and the next one's values
@@ -710,7 +728,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         auto weight = [&](int u, int j) {  // j and j + 1
 #pragma unroll
             for (int e = j; e < j + 2; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u % 2) + e], xscale, shift));
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u % 2) + e], factor, shift));
                 if (CT == PT_I8) {
                     sum += p[e];
                     p[e] *= vs[u & 1][e / 4][e % 4];

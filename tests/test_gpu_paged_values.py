@@ -90,3 +90,28 @@ def test_large_values_of_a_bf16_cache(prompt, size):
         c.v = (c.v.float().clamp(-1, 1) * size).bfloat16()
         c.q = (c.q.float() * 4).bfloat16()                                     # few keys have most of the weight
         assert_attention(attend(c, prompt), c)
+
+
+# ---- scores -------------------------------------------------------------------------------------------
+@PROMPT
+@pytest.mark.parametrize("act,cache", COMBOS)
+@pytest.mark.parametrize("size", [3e7, 3e8, 1e9, -1e9, 7e10])
+def test_scores_whose_steps_are_larger_than_one(act, cache, prompt, size):
+    """|scores| of 10^7 to 10^9: fp32's steps there are 2 to 64. Every key of a sequence is the same, so that the weights are equal
+    whatever the score is"""
+    c = Case(act, cache, 4, 2, 64, 16, (150, 40), (20, 1) if prompt else (1, 1), seed=45)
+    own = c.k[int(c.table[0, 0]), :, :1].clone()                               # [kv, 1, dim] of a slot that has values
+    c.k = own.expand(c.pages, *own.shape).expand(-1, -1, c.page, -1).contiguous()
+    if c.ks is not None:
+        c.ks[:] = 50.0
+    c.q = c.q[:1, :1].expand_as(c.q).contiguous()
+    score = float((c.q[0, 0].double() @ (own[0, 0].double() / (1 if c.ks is None else 50.0))))
+    scale = float(np.float32(size / score))
+    out = attend(c, prompt, scale=scale).double().cpu().numpy()
+    even = Case(act, cache, 4, 2, 64, 16, (150, 40), c.new, seed=45)
+    even.q = torch.zeros_like(c.q)                                             # the same weights: all scores zero
+    ref, bound = even.attention()
+    mine = np.zeros(c.rows, dtype=bool)
+    mine[:int(c.offsets[-1])] = True
+    # heads of the second key head have other scores, equal among their keys all the same
+    assert (np.abs(out - ref) <= bound)[mine].all()
