@@ -43,9 +43,14 @@ constexpr uint32_t kRows = 128, kKeys = 64;
 constexpr uint32_t kSpread = 512;
 constexpr uint32_t kLeast = 4;     // fewest key tiles per share
 constexpr float kLow = -1.7e38f;
-constexpr float kSlack = 2.0f;
+// A row's running maximum is raised once a score exceeds it by kSlack (base 2), and by nothing but what the row sees, whatever
+// the wave's others do: what they see must not change how it is rounded. Weights are scaled by 2^kLift and stay below 2^15.75,
+// inside fp16; in bf16, whose values reach as far as fp32's, below 1. (Raising outputs costs, so that bf16 takes as much slack as is
+// of use: 8192 tokens 543 us, with 2 560.)
 template <int CT>
-constexpr float kLift = CT == PT_BF16 ? -2.0f : 13.0f;  // weights stay below 2^15, inside fp16; in bf16, below 1 (as in paged_decode.hip)
+constexpr float kSlack = CT == PT_BF16 ? 8.0f : 2.75f;
+template <int CT>
+constexpr float kLift = CT == PT_BF16 ? -8.0f : 13.0f;
 
 // rows (token, head) of a sequence in tiles of kRows; no more tokens than the buffers have rows, so that it all fits 31 bits
 __device__ __forceinline__ uint32_t rows_of(const PagedAttentionArgs &a, const PagedSeq &s)
@@ -143,7 +148,7 @@ __device__ __forceinline__ float max_of(float a, float b, float c)
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
-constexpr float kLargeScore = 4194304.0f;  // 2^22: half an fp32 step of it is 2^-2
+constexpr float kLargeScore = 262144.0f;  // 2^18: half an fp32 step of it is 2^-6
 
 // int8: the steps of a tile's keys (times the score scale) and values, values whose step is not finite, and the power of two above
 // the largest step. Values' steps three times: over `unit`, for rows that see the whole tile; as they are and times 2^-80, for
@@ -665,9 +670,9 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             top = max_of(top, s[0][j], s[1][j]);
         }
         top *= xscale;
-        if (__any(top > m + kSlack || (CT == PT_I8 && tile_unit > unit))) {
+        if (__any(top > m + kSlack<CT> || (CT == PT_I8 && tile_unit > unit))) {
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float up = fmaxf(top, m);
+            const float up = top > m + kSlack<CT> ? top : m;
             float corr = __builtin_amdgcn_exp2f(m - up);
             l *= corr;
             m = up;

@@ -115,3 +115,20 @@ def test_scores_whose_steps_are_larger_than_one(act, cache, prompt, size):
     mine[:int(c.offsets[-1])] = True
     # heads of the second key head have other scores, equal among their keys all the same
     assert (np.abs(out - ref) <= bound)[mine].all()
+
+
+@pytest.mark.parametrize("act,cache", COMBOS)
+def test_keys_of_later_tokens_do_not_change_how_a_row_is_rounded(act, cache):
+    """one later token after another gets a key whose scores are some forty times the others': the rows before it, in the same
+    tile and the same wave, keep their bytes"""
+    new, past = 150, 3
+    c = Case(act, cache, 8, 2, 64, 16, (new + past,), (new,), seed=46)
+    clean = attend(c, True)
+    assert_attention(clean, c)
+    for spot in (20, 69, 77, 90, 101, 130, 149):
+        page, slot = int(c.table[0, (spot + past) // 16]), (spot + past) % 16
+        target = c.ks if cache == "i8" else c.k
+        keep = target.clone()
+        target[page, :, slot] *= 1 / 40 if cache == "i8" else 40
+        assert torch.equal(bits(attend(c, True)[:spot]), bits(clean[:spot])), spot
+        target.copy_(keep)
