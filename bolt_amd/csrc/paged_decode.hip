@@ -40,7 +40,7 @@ constexpr uint32_t per_cu()
     return DIM == 128 ? 2 : 3;
 }
 
-constexpr float kLow = -1.7e38f;     // running maximum before the first key
+constexpr float kLow = -3.40282347e38f;  // running maximum before the first key: no score that is a number lies below
 constexpr float kSlack = 2.0f;
 template <int CT>
 constexpr float kLift = CT == PT_BF16 ? -2.0f : 13.0f;  // see above: 2^(kSlack + kLift) fits fp16

@@ -42,7 +42,7 @@ constexpr uint32_t kRows = 128, kKeys = 64;
 // prompts of up to 1025 tokens have more tiles than that: 99 us with whole tiles, 153 with their keys cut in two.
 constexpr uint32_t kSpread = 512;
 constexpr uint32_t kLeast = 4;     // fewest key tiles per share
-constexpr float kLow = -1.7e38f;
+constexpr float kLow = -3.40282347e38f;  // running maximum before the first key: no score that is a number lies below
 // A row's running maximum is raised once a score exceeds it by kSlack (base 2), and by nothing but what the row sees, whatever
 // the wave's others do: what they see must not change how it is rounded. Weights are scaled by 2^kLift and stay below 2^15.75,
 // inside fp16; in bf16, whose values reach as far as fp32's, below 1. (Raising outputs costs, so that bf16 takes as much slack as is

@@ -132,3 +132,20 @@ def test_keys_of_later_tokens_do_not_change_how_a_row_is_rounded(act, cache):
         target[page, :, slot] *= 1 / 40 if cache == "i8" else 40
         assert torch.equal(bits(attend(c, True)[:spot]), bits(clean[:spot])), spot
         target.copy_(keep)
+
+
+@PROMPT
+@pytest.mark.parametrize("size", [-0.9, -2.0, -2.3])
+def test_scores_close_to_the_lowest_number(prompt, size):
+    """every key's score is the same, size times 10^38: the weights are equal"""
+    for total in (40, 3000):
+        c = Case("bf16", "bf16", 4, 2, 64, 16, (total,), (7,) if prompt else (1,), seed=47)
+        c.k[c.k.isfinite()] = 0.0
+        c.k[..., 5] = torch.where(c.k[..., 5].isnan(), c.k[..., 5], 1e19)
+        even = Case("bf16", "bf16", 4, 2, 64, 16, (total,), c.new, seed=47)
+        even.q = torch.zeros_like(c.q)
+        c.q = torch.zeros_like(c.q)
+        c.q[..., 5] = size * 1e19
+        out = attend(c, prompt, scale=1.0).double().cpu().numpy()
+        ref, bound = even.attention()
+        assert (np.abs(out - ref) <= bound).all()
