@@ -375,6 +375,14 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
         const uint32_t ec = me & 15, eg = me >> 4 & 3;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
+        // A sum of zero: the wave has seen no key, which a maximum of -inf says of it, or only scores of -inf
+        if (__any(l == 0.0f)) {
+            bool any = false;
+            for (uint32_t key = from + 32 * wave + (lane & 31); key < to; key += 128) {
+                any |= key >= span.lo && (uint32_t)table[key >> a.pool.shift] < a.pool.pages;
+            }
+            m = l == 0.0f && !__any(any) ? -INFINITY : m;
+        }
         if (eg == 0) {
             sM[wave][ec] = m;
             sL[wave][ec] = l * kPartScale<CT>;
@@ -395,12 +403,12 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
             v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = __builtin_amdgcn_exp2f(sM[w][r] - top);
+                const float f = __builtin_amdgcn_exp2f(sM[w][r] - fmaxf(top, kLow));
                 sum += sL[w][r] * f;
                 v += *(const v4f *)(&sO[w][r * kRow + d]) * f;
             }
             if (whole_sequence) {
-                v = sum == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
+                v = top == -INFINITY ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
                 store_out4<ACT>(a.out, (size_t)b * a.ostride + (size_t)(kvh * group + q0 + r) * DIM + d, v);
             } else {
                 *(v4f *)(part + r * DIM + d) = v;
@@ -446,12 +454,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionArgs a, u
     const float *part = part_at(a, shares, kvh * qtiles + in / 16, first, 0, DIM);
     const uint32_t slot = before % per != 0;  // of the first part; the others are the first of their share
     const uint32_t way = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
-    float top = kLow, sum = 0.0f;
+    float top = -INFINITY, sum = 0.0f;
     v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t i = way; i < count; i += kWays) {
         const float *p = part + ((size_t)2 * i + (i ? 0 : slot)) * 16 * (DIM + 2);
         const float m = p[16 * DIM + r], up = fmaxf(top, m);
-        const float f = __builtin_amdgcn_exp2f(top - up), e = __builtin_amdgcn_exp2f(m - up);
+        const float from = fmaxf(up, kLow), f = __builtin_amdgcn_exp2f(top - from), e = __builtin_amdgcn_exp2f(m - from);
         sum = sum * f + p[16 * DIM + 16 + r] * e;
         v = v * f + *(const v4f *)(p + r * DIM + d) * e;
         top = up;
@@ -472,11 +480,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionArgs a, u
         v = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t w = 0; w < kWays; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sM[w] - up);
+            const float f = __builtin_amdgcn_exp2f(sM[w] - fmaxf(up, kLow));
             sum += sL[w] * f;
             v += *(const v4f *)(&sO[w][d]) * f;
         }
-        v = sum == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
+        v = up == -INFINITY ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
         store_out4<ACT>(a.out, (size_t)b * a.ostride + (size_t)h * DIM + d, v);
     }
 }

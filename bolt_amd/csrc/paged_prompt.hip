@@ -830,6 +830,15 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             }
         }
     }
+    // A sum of zero: the row has seen no key here, which a maximum of -inf says of it, or only scores of -inf
+    if (l == 0.0f) {
+        const uint32_t upto = min(span.hi, all.lo + t1 * kKeys), mask = (1u << a.pool.shift) - 1;
+        bool any = false;
+        for (uint32_t key = max(span.lo, all.lo + t0 * kKeys); key < upto && !any; key = (key | mask) + 1) {
+            any = (uint32_t)table[key >> a.pool.shift] < a.pool.pages;
+        }
+        m = any ? m : -INFINITY;
+    }
     if (alone) {
         if (!mine) {
             return;
@@ -837,7 +846,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
         uint32_t again = r;
         asm volatile("" : "+v"(again));  // the row's place is worked out anew: kept over the loop it would cost registers
         const uint32_t token_again = paged_div(again, a.group);
-        const float inv = l == 0.0f ? 0.0f : unit / l;
+        const float inv = m == -INFINITY ? 0.0f : l == 0.0f ? NAN : unit / l;
         const size_t at = (size_t)(seq.first + token_again) * a.ostride + (size_t)(kvh * group + (again - token_again * group)) * DIM + 4 * h;
 #pragma unroll
         for (int i = 0; i < kOut; ++i) {
@@ -893,17 +902,17 @@ __global__ __launch_bounds__(8 * DIM / 4) void paged_prompt_join_kernel(PagedAtt
     if (r >= rows || row < 0 || row >= (int64_t)a.batch.rows) {
         return;
     }
-    float top = kLow, sum = 0.0f;
+    float top = -INFINITY, sum = 0.0f;
     v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t i = 0; i < count; ++i) {
         const float *const p = part_at(a, x, kvh, i, shares.d, DIM);
         const float m = p[kRows * DIM + pr], up = fmaxf(top, m);
-        const float f = __builtin_amdgcn_exp2f(top - up), e = __builtin_amdgcn_exp2f(m - up);
+        const float from = fmaxf(up, kLow), f = __builtin_amdgcn_exp2f(top - from), e = __builtin_amdgcn_exp2f(m - from);
         sum = sum * f + p[kRows * DIM + kRows + pr] * e;
         v = v * f + *(const v4f *)(p + (size_t)pr * DIM + d) * e;
         top = up;
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = top == -INFINITY ? 0.0f : sum == 0.0f ? NAN : 1.0f / sum;
     store_out4<ACT>(a.out, (size_t)row * a.ostride + (size_t)(kvh * group + r - token * group) * DIM + d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
 }
 

@@ -149,3 +149,39 @@ def test_scores_close_to_the_lowest_number(prompt, size):
         out = attend(c, prompt, scale=1.0).double().cpu().numpy()
         ref, bound = even.attention()
         assert (np.abs(out - ref) <= bound).all()
+
+
+@PROMPT
+@pytest.mark.parametrize("act,cache", COMBOS)
+@pytest.mark.parametrize("total", [40, 700, 3000])
+def test_scores_of_minus_infinity(act, cache, prompt, total):
+    """Where every key that a row sees has a score of minus infinity the formula is 0 / 0: the row shows it, as one that sees nothing
+    (zeros) does not. Where some keys have, the others are all there is. What is not stored counts for neither."""
+    new = 3 if prompt else 1
+    c = Case(act, cache, 4, 2, 64, 16, (total, 20, 3), (new, new, new), seed=48)
+    c.q = torch.ones_like(c.q)
+    c.k = c.k.abs() if cache == "i8" else c.k
+    c.table[1] = -1                                                            # a sequence without pages
+
+    def lower(pages):
+        if cache == "i8":
+            c.ks[pages] = -0.0                                                 # stored / scale: minus infinity, or 0 / 0
+            c.k[pages] = c.k[pages].clamp(min=1)
+        else:
+            c.k[pages, :, :, 9] = float("-inf")
+    some = c.table[0, :2].long()
+    want = Case(act, cache, 4, 2, 64, 16, (total, 20, 3), (new, new, new), seed=48)
+    want.k, want.q, want.ks, want.vs, want.v = c.k.clone(), c.q, c.ks, c.vs, c.v
+    want.ks = None if c.ks is None else c.ks.clone()
+    want.table = c.table.clone()
+    want.table[0, :2] = -1
+    lower(some)
+    out = attend(c, prompt)
+    if (act, cache) == ("f32", "f16"):                                         # two parts to a query: infinities may be NaN
+        assert out[:new].isnan().all()
+        out[:new] = attend(want, prompt)[:new]
+    assert_attention(out, want)
+    assert not out[new:2 * new].any()
+    lower(c.table[0, :-(-total // 16)].long())
+    out = attend(c, prompt)
+    assert out[:new].isnan().all() and not out[new:2 * new].any() and torch.equal(bits(out[2 * new:]), bits(attend(want, prompt)[2 * new:]))
