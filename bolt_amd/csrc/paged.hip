@@ -62,10 +62,11 @@ __global__ void paged_append_kernel(PagedAppendArgs a)
         s = paged_seq_from(__builtin_amdgcn_readlane(first, b), __builtin_amdgcn_readlane(next, b), __builtin_amdgcn_readlane(len, b));
     }
     const int64_t i = (int64_t)row - s.first, pos = s.pos + i;
-    if (i < 0 || i >= s.count || pos < 0 || pos >= (int64_t)a.batch.max_pages << a.pool.shift || (a.rot && pos >= (int64_t)a.angles)) {
+    if (i < 0 || i >= s.count || pos < 0 || (a.rot && pos >= (int64_t)a.angles)) {
         return;
     }
-    const int64_t slot0 = paged_slot(a.batch.table + (size_t)b * a.batch.max_pages, (uint32_t)pos, a.pool.shift, a.pool.pages, kvh, 0);
+    // (without a slot nothing is stored; the query is turned all the same)
+    const int64_t slot0 = pos >= (int64_t)a.batch.max_pages << a.pool.shift ? -1 : paged_slot(a.batch.table + (size_t)b * a.batch.max_pages, (uint32_t)pos, a.pool.shift, a.pool.pages, kvh, 0);
     for (uint32_t item = threadIdx.x; item < heads * kLanes;) {
         const uint32_t l = n.l, h = n.h, e0 = n.e0, e1 = n.e1;
         const bool is_q = n.is_q, is_v = n.is_v, turned = n.turned;

@@ -122,7 +122,8 @@ def _here(cache, batch):
 
 def kv_cache_append(cache, batch, k, v, q=None, rotary=None, q_out=None):
     """k, v: [rows, kv_heads, head_dim], q: [rows, heads, head_dim], rows any number of elements apart. Returns q_out, the
-    rotated queries (None without q). Rows that belong to no sequence are left as they are in q_out."""
+    rotated queries (None without q). Rows that belong to no sequence, or whose position lies behind the angles, are left as they are
+    in q_out (where the call makes q_out, they hold anything): the angles have to reach as far as the lengths do."""
     _here(cache, batch)
     device, dtype, shape = cache.device, k.dtype, (batch.rows, cache.kv_heads, cache.head_dim)
     if rotary is not None and rotary.device != device:

@@ -546,9 +546,11 @@ typedef struct {
 /* Stores k and v, rows of kvHeads heads, at their positions; keys are rotated on the way (rotary == NULL: not). With heads
  * > 0 the queries are rotated too, from q to qOut (which may be q itself). Every step is one fp32 operation,
  * a' = a cos - b sin, b' = b cos + a sin, rounded once to the stored type; an int8 slot gets
- * s = (1 / max|x|) * 127 (the reciprocal first; 1 for a row of zeros) and rne(x * s). A token whose position lies behind the
- * tables of angles is left out like one without a page. Slots must be distinct: two sequences that append to a shared
- * page race. */
+ * s = (1 / max|x|) * 127 (the reciprocal first; 1 for a row of zeros) and rne(x * s).
+ * A token without a slot (a page number that is none of the pool's, a position behind the page table) is not stored, and its query
+ * is turned like any other. One in front of its sequence or behind the tables of angles is left out: not stored, and its row of
+ * qOut is not written. The attention calls know nothing of angles and take such a row as they find it, so the tables have to
+ * reach as far as the lengths do. Slots must be distinct: two sequences that append to a shared page race. */
 EE bolt_gfx950_kv_cache_append(const BoltPagedKvCache *cache, const BoltPagedBatch *batch, DataType dt, const void *k,
     U32 kStride, const void *v, U32 vStride, U32 heads, const void *q, U32 qStride, void *qOut, U32 qOutStride,
     const BoltRotary *rotary);

@@ -9,10 +9,45 @@ pytestmark = pytest.mark.gpu
 import torch  # noqa: E402
 
 from bolt_amd import capi, host_paged as hp  # noqa: E402
-from checkers_paged import COMBOS, TYPES, Case, assert_attention  # noqa: E402
-from test_gpu_paged import attend, bits, ready  # noqa: E402,F401
+from checkers_paged import COMBOS, TYPES, Case, assert_attention, rotated  # noqa: E402
+from test_gpu_paged import angles, attend, bits, ready, sync  # noqa: E402,F401
 
 PROMPT = pytest.mark.parametrize("prompt", [False, True])
+
+
+# ---- append -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("act,cache", [("f32", "f16"), ("bf16", "i8"), ("f16", "f16")])
+def test_a_token_without_a_slot_has_a_query_all_the_same(act, cache, turned):
+    """Positions behind the page table, like page numbers outside the pool: nothing is stored, and the query is turned as any other.
+    Positions in front of the sequence, and behind the angles where there are any, leave qOut as it is."""
+    angles_for = 40
+    c = Case(act, cache, 4, 2, 64, 8, (30, 20, 3), (26, 20, 5), seed=49, max_pages=2)
+    c.table[1, 0] = c.pages + 7
+    pc, pb, _ = c.gpu()
+    g = torch.Generator().manual_seed(50)
+    q, k = (torch.randn(c.rows, h, 64, generator=g).to(TYPES[act]) for h in (4, 2))
+    cos, sin = angles(angles_for, 64)
+    out = torch.full_like(q, 9.0).cuda()
+    for limit in (angles_for, 18) if turned else (angles_for,):
+        out.fill_(9.0)
+        r = hp.Rotary(cos[:limit].cuda(), sin[:limit].cuda()) if turned else None
+        hp.kv_cache_append(pc, pb, k.cuda(), k.cuda(), q.cuda(), r, out)
+        sync()
+        pos = torch.tensor([t - n + i for t, n in zip(c.lengths, c.new) for i in range(n)])
+        left = (pos < 0) | (turned & (pos >= limit))
+        at = pos.clamp(0, limit - 1)
+        want = (rotated(q.float(), cos[at], sin[at], False) if turned else q.float()).to(TYPES[act])
+        want[left] = 9.0
+        assert torch.equal(bits(out), bits(want))
+    stored = torch.zeros(c.pages, c.page, dtype=torch.bool)
+    for b in range(3):
+        for p in range(c.lengths[b] - c.new[b], 16):
+            if 0 <= p < c.lengths[b] and int(c.table[b, p // 8]) < c.pages:
+                stored[int(c.table[b, p // 8]), p % 8] = True
+    for now, was in zip(pc.keep, (c.k, c.v, c.ks, c.vs)):
+        if was is not None:
+            assert torch.equal(bits(now.transpose(1, 2)[~stored.cuda()]), bits(was.transpose(1, 2)[~stored]))
 
 
 # ---- slots that a row does not see ------------------------------------------------------------------
