@@ -24,6 +24,15 @@ def test_index_arithmetic_on_the_host():
         assert subprocess.check_output([exe]).decode() == "ok\n"
 
 
+def test_index_arithmetic_reads_nothing_outside_its_lists():
+    """the same program with address checks: offsets, lengths and table rows are on the heap there"""
+    with tempfile.TemporaryDirectory() as d:
+        exe = os.path.join(d, "check")
+        subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-Wall", "-Werror", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                               os.path.join(HERE, "paged_index_check.cpp"), "-o", exe])
+        assert subprocess.check_output([exe]).decode() == "ok\n"
+
+
 def pool(**kw):
     c = BoltPagedKvCache(DT_F16, 10, 16, 2, 64, P, P, None, None)
     for k, v in kw.items():
