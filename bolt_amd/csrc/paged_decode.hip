@@ -13,8 +13,9 @@
 // The running maximum is only raised once a score exceeds it by 2 (base 2). Over an fp16 or int8 cache weights are scaled by 2^13
 // and stay below 2^15, inside fp16; a weight of less than 2^-37 of the row's largest is lost. Over a bf16 cache, whose values
 // reach as far as fp32's, they are scaled by 2^-2 and stay below 1, so that their products overflow only where the plain formula's
-// fp32 sums do. An int8 cache's steps (1 / scale) are part of
-// the weights, divided by a power of two that no step exceeds, so that they add nothing to that range.
+// fp32 sums do. An int8 cache's steps (1 /
+// scale) are part of the weights, divided by a power of two that no step seen so far exceeds: nothing leaves fp16 upwards, and a slot
+// whose step is 2^k times another's takes k of the other's 37 powers of two.
 //
 // The tiles (of 128 keys) of all sequences stand in one row that is cut into equal shares, one to a workgroup, which fill the chip once:
 // every workgroup reads the same number of bytes, whatever the lengths are. They are read on the device, so a captured launch

@@ -730,6 +730,9 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             steps_of(0);
             steps_of(1);
         }
+        // Weights of 16-bit activations are rounded once, which leaves an error of the order of the output's own rounding. Two parts, as
+        // fp32 activations have, would double these products: 8192 tokens bf16 717 us against 540, ragged prompts fp16 120 and 97,
+        // 2 x 256 tokens over 27 k int8 keys 195 and 158. Over a 16-bit cache the sum takes the rounded ones, so that they add up to one.
         auto weight = [&](int u, int j) {  // j and j + 1
 #pragma unroll
             for (int e = j; e < j + 2; ++e) {

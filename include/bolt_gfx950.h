@@ -558,9 +558,15 @@ EE bolt_gfx950_kv_cache_append(const BoltPagedKvCache *cache, const BoltPagedBat
  * the keys 0 .. p of its sequence, with window > 0 the last `window` of them; a row that sees no key becomes zeros. What the
  * cache holds elsewhere has no influence, infinities and NaN included; where a row sees a key or value that is infinite or NaN
  * (or an int8 slot with a scale of zero or NaN), it shows what the formula makes of it, or NaN. An int8 slot stands for
- * stored / scale, of either sign. fp32 numbers below the smallest normal one may count as zeros. Scores, the softmax and
- * its sums are fp32; fp32 activations go into the products in two 16-bit parts (a relative error of 2^-21). The result does not depend on what else is in the batch run
- * beyond fp32 rounding of how the keys are split; the same call gives the same bytes.
+ * stored / scale, of either sign. fp32 numbers below the smallest normal one may count as zeros. The result does not
+ * depend on what else is in the batch run beyond fp32 rounding of how the keys are split; the same call gives the same bytes.
+ * Numbers: scores, maxima and all sums are fp32; the products' factors have 16 bits. fp32 queries go in as two parts (a relative error
+ * of 2^-21), and so do the weights, but for prompts with 16-bit activations: two parts lose 2^-21 of a weight, over a bf16 cache
+ * 2^-15; those prompts round it once, to fp16 (2^-11 of it) or, over a bf16 cache, bf16 (2^-8), and over a 16-bit cache divide by the
+ * sum of the rounded ones. Over an fp16 or int8 cache a weight ends at 2^-37 of the row's largest: n keys add up to n 2^-37 times the
+ * largest |value| to the error, over int8 n 2^-37 times 254 / the smallest |scale| among the slots that the row sees (a slot of
+ * zeros counts like any other, with a scale of 1 from append). Outputs are infinite where the sums of weight / largest weight (over
+ * int8 up to four times that) times value leave fp32.
  *   decode  one new token per sequence (offsets == NULL): the keys are split over the machine and the parts joined
  *   prompt  any number of new tokens per sequence (offsets != NULL), each seeing those before it; they must be stored
  *           (bolt_gfx950_kv_cache_append) before the call
