@@ -298,7 +298,7 @@ __global__ __launch_bounds__(256, per_cu<DIM>()) void paged_decode_kernel(PagedA
                     wide = fmaxf(wide, fabsf(step[j]));
                 }
             }
-            if (__any(top > m + kSlack || (CT == PT_I8 && wide > unit))) {
+            if (__any(top - m > kSlack || (CT == PT_I8 && wide > unit))) {
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
                 const float up = fmaxf(top, m);

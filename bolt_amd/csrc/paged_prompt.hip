@@ -43,7 +43,8 @@ constexpr uint32_t kRows = 128, kKeys = 64;
 constexpr uint32_t kSpread = 512;
 constexpr uint32_t kLeast = 4;     // fewest key tiles per share
 constexpr float kLow = -3.40282347e38f;  // running maximum before the first key: no score that is a number lies below
-// A row's running maximum is raised once a score exceeds it by kSlack (base 2), and by nothing but what the row sees, whatever
+// A row's running maximum is raised once a score exceeds it by kSlack (base 2; the difference is exact where it counts, m + kSlack need
+// not be), and by nothing but what the row sees, whatever
 // the wave's others do: what they see must not change how it is rounded. Weights are scaled by 2^kLift and stay below 2^15.75,
 // inside fp16; in bf16, whose values reach as far as fp32's, below 1. (Raising outputs costs, so that bf16 takes as much slack as is
 // of use: 8192 tokens 543 us, with 2 560.)
@@ -670,9 +671,9 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedAttentionArgs
             top = max_of(top, s[0][j], s[1][j]);
         }
         top *= xscale;
-        if (__any(top > m + kSlack<CT> || (CT == PT_I8 && tile_unit > unit))) {
+        if (__any(top - m > kSlack<CT> || (CT == PT_I8 && tile_unit > unit))) {
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float up = top > m + kSlack<CT> ? top : m;
+            const float up = top - m > kSlack<CT> ? top : m;
             float corr = __builtin_amdgcn_exp2f(m - up);
             l *= corr;
             m = up;

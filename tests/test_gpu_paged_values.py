@@ -220,3 +220,21 @@ def test_scores_of_minus_infinity(act, cache, prompt, total):
     lower(c.table[0, :-(-total // 16)].long())
     out = attend(c, prompt)
     assert out[:new].isnan().all() and not out[new:2 * new].any() and torch.equal(bits(out[2 * new:]), bits(attend(want, prompt)[2 * new:]))
+
+
+@PROMPT
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_scores_that_rise_by_one_step_of_four(prompt, act):
+    """Scores of 4e7 to 6e7 (to the base 2), where fp32's steps are 4, rising by one step behind the first tile: a weight of 16 times the first
+    ones', which is inside the formula's range and has to be inside the kernels'"""
+    for a in range(36000, 60000, 1500):
+        c = Case(act, "f16", 4, 2, 64, 16, (200,), (20,) if prompt else (1,), seed=51)
+        c.q = torch.zeros_like(c.q)
+        c.q[..., :2] = 1.0
+        c.k[c.k.isfinite()] = 0.0
+        own = torch.tensor([int(c.table[0, p // 16]) * 16 + p % 16 for p in range(200)])
+        k = torch.zeros(c.pages * 16, 2, 64, dtype=torch.float16)
+        k[own, :, 0] = float(a // 32 * 32)                                     # a number of the type
+        k[own[64:], :, 1] = 2.0 ** -8
+        c.k = k.view(c.pages, 16, 2, 64).transpose(1, 2).contiguous()
+        assert_attention(attend(c, prompt, scale=1024 / 1.4426950408889634), c, 1024 / 1.4426950408889634)
