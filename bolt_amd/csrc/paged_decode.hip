@@ -496,7 +496,8 @@ uint32_t columns(uint32_t heads, uint32_t kv_heads)
 }
 
 // Shares of n columns with `fit` workgroups at a time: of the numbers that fill the chip once to four times, the first that
-// leaves no more than a tenth idle, or else the one that leaves least.
+// leaves no more than a tenth idle, or else the one that leaves least. (96 key heads of 128, 1 x 20 k keys: 157 us, where the first
+// that leaves no more than three tenths idle takes 175 and the one that leaves least 159; 6 ragged requests 114, 129 and 114.)
 uint32_t shares_of(uint32_t n, uint32_t fit)
 {
     uint32_t best = 1;
@@ -519,7 +520,7 @@ uint32_t most_per_cu(uint32_t dim)
 // Workgroups that a CU is given. Where memory is what bounds it, one (head size 64: two, whose loads are half as large) brings
 // the bytes as fast as more, and leaves fewer parts to write and join: head size 128, one against two, 32 requests fp16 50.0
 // and 50.9 us, 64 int8 106.6 and 109.4, two long ones bf16 145.6 and 150.2, seven heads to a key head 29.3 and 32.6; head
-// size 64, two against three, fp32 over fp16 30.6 and 34.6, long bf16 81 and 84, 64 requests fp16 55.9 and 54.7. What an int8
+// size 64, two against three, fp32 over fp16 30.6 and 34.6, long bf16 81 and 84, and, the other way, 64 requests fp16 55.9 and 54.7. What an int8
 // cache has to be converted for with smaller heads, and for fp32's two parts, takes one more: head size 128, fp32, 36.2
 // against 38.9 with one; head size 64 37.8 against 40.2 with two. More waves than that spill or stand idle: head size 128,
 // three, 85 us for 32 requests; head size 64, four, 62.

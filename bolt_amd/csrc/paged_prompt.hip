@@ -15,10 +15,10 @@
 // before theirs (a tile waits for one barrier and no load); its steps multiply scores and weights.
 //
 // What it costs. A wave issues 32 products of 32x32x16 a tile (head size 128; 36.5 cycles each alone, 44 with real data,
-// when the clock falls) and some 200 vector instructions (int8: 390), 32 of them exponentials, and it does not overlap its
+// when the clock falls) and some 200 vector instructions (int8: 400), 32 of them exponentials, and it does not overlap its
 // own products with them: two waves on every SIMD, from two workgroups, do. One prompt of 8192 tokens, 32 heads over 8, bf16,
 // takes 0.55 ms, 1.0 PFLOP/s, where the library's 8192^3 product of the same type reaches 1.2; 2 x 256 tokens over 27 k
-// int8 keys 0.156 ms, 0.72 PFLOP/s. Head size 128 takes 220 to 230 registers of the 256 that two waves leave each; more
+// int8 keys 0.158 ms, 0.71 PFLOP/s. Head size 128 takes 215 to 242 registers of the 256 that two waves leave each; more
 // rows to a wave would halve the reads of LDS and do not fit.
 // Where few tiles meet many keys, several workgroups share a tile's keys and a second launch joins their parts.
 #include <atomic>
@@ -41,7 +41,9 @@ constexpr uint32_t kRows = 128, kKeys = 64;
 // of rows: 153 us with 512, 204 with 256 (half the chip idle), 174 with 1024 (more parts written and read). Eight ragged
 // prompts of up to 1025 tokens have more tiles than that: 99 us with whole tiles, 153 with their keys cut in two.
 constexpr uint32_t kSpread = 512;
-constexpr uint32_t kLeast = 4;     // fewest key tiles per share
+// Fewest key tiles per share. 20 tokens over 2000 keys, fp16, 32 heads over 8: 15.1 us with 4, 14.9 with 2, 22.2 with 1 (more parts to
+// write and join than keys to share), 19.2 with 8; 100 over 700: 17.1, 16.5, 21.5, 19.6.
+constexpr uint32_t kLeast = 4;
 constexpr float kLow = -3.40282347e38f;  // running maximum before the first key: no score that is a number lies below
 // A row's running maximum is raised once a score exceeds it by kSlack (base 2; the difference is exact where it counts, m + kSlack need
 // not be), and by nothing but what the row sees, whatever
